@@ -412,6 +412,90 @@ tb_status tb_decode_margin(const float *logits_dev, int64_t vocab, const int64_t
 tb_status tb_decode_advance(const int64_t *idx_dev, int32_t *ids_dev, int32_t *pos_dev, int32_t *history_dev,
                             int64_t max_seq, tb_stream stream);
 
+/* ------------------------------------------- paged key/value cache, batched decode -- */
+
+/* One layer's cache as pages of page_size tokens scattered over two pools, for
+ * a batch of sequences that grow independently (no counterpart in the
+ * reference, whose cache is one sequence's [max_seq, kv_heads, head_dim] array,
+ * src/core/kv_cache.cpp:5-19).  Element d of head h of token slot t of page p
+ * lies at p * page_stride + t * token_stride + h * head_stride + d in both
+ * pools, so pages may be laid out token by token (as the reference's cache) or
+ * head by head.  Strides are in elements; each covers head_dim at least, and
+ * the pools and the strides in bytes are multiples of 16. */
+typedef struct tb_paged_cache {
+  void *k, *v;        /* device: the pools */
+  int32_t dtype;      /* TB_F32, TB_F16 or TB_BF16 */
+  int32_t page_size;  /* tokens per page: a power of two */
+  int64_t n_pages, kv_heads, head_dim;
+  int64_t page_stride, token_stride, head_stride;
+} tb_paged_cache;
+/* The sequences of a call.  Position t of sequence b is slot t % page_size of
+ * page table[b * table_stride + t / page_size].  lens and table are read when
+ * the kernel runs, so a captured call can be replayed as sequences grow. */
+typedef struct tb_paged_batch {
+  int64_t batch;
+  const int32_t *lens;   /* device [batch]: keys of each sequence, a call's own new tokens included */
+  const int32_t *table;  /* device [batch, max_pages] page ids */
+  int64_t max_pages, table_stride;
+} tb_paged_batch;
+
+/* RoPE of queries and keys and the append of keys and values to a paged cache,
+ * for any mix of prompts and single tokens in one launch: tb_rope_kv_append for
+ * a batch.  Tokens starts_dev[b] .. starts_dev[b + 1] - 1 are sequence b's last
+ * tokens, in order: the last one has position lens[b] - 1.  starts_dev NULL:
+ * tokens == batch and token b is sequence b's newest; lens[b] == 0 then marks an
+ * empty slot, whose rows are left as they are.  So are the rows at and after
+ * starts_dev[batch].  starts_dev begins with 0 and does not decrease.
+ *   q_out[t] = R(p) q[t],  K[p] = R(p) k[t],  V[p] = v[t]
+ * with the rotation of tb_rope (tables [rope_max_seq, head_dim / 2]); both
+ * tables NULL: no rotation.  q [tokens, heads, head_dim], k and v [tokens,
+ * kv_heads, head_dim], rows ldq, ldk, ldv, ldq_out elements apart.  heads 0: no
+ * queries (q and q_out unused).  q_out may be q; k is not modified.  act_dtype,
+ * the type of q, q_out, k and v, is TB_F32 or the cache's; the rotation is
+ * computed in fp32 and rounded once.  head_dim a multiple of 16, at most 256;
+ * rows 16-byte aligned.  A token whose position lies outside the tables, or
+ * whose page id lies outside the pool, sets bit 1 of the device error word and
+ * none of its rows is written.  Two sequences of a call must not share the page
+ * that either of them writes. */
+tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_paged_batch *seqs, int act_dtype,
+                               const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk, const void *v_dev,
+                               int64_t ldv, int64_t tokens, int64_t heads, const int32_t *starts_dev,
+                               const float *cos_dev, const float *sin_dev, int64_t rope_max_seq, void *q_out_dev,
+                               int64_t ldq_out, tb_stream stream);
+
+/* Bytes of the workspace of the two calls below (host arithmetic, no device
+ * needed).  Zero the workspace once before its first use and keep it: every
+ * call leaves it ready for the next.  It must be 256-byte aligned, and calls
+ * that can overlap on the GPU need one each. */
+tb_status tb_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                             size_t *bytes_out);
+/* Attention of one query token per sequence (tb_attention_decode for a batch
+ * and a paged cache): out[b, h] = sum over t < lens[b] of softmax_t(scale
+ * q[b, h] . K_b[t]) V_b[t], query head h reading key/value head h / (heads /
+ * kv_heads).  lens[b] == 0 gives zeros.  q and out [batch, heads, head_dim],
+ * rows ldq and ldo elements apart, 16-byte aligned; act_dtype, their type, is
+ * TB_F32 or the cache's.  head_dim 64 or 128, any number of query heads per
+ * key/value head.  Accumulated in fp32; TB_F32 results are accurate to fp32 (no
+ * operand is rounded below 22 bits).  Keys, values and queries in use are
+ * finite; what lies behind a sequence's last key is never used.  A length
+ * below 0 or above max_pages * page_size counts as 0, a page id outside the
+ * pool reads as zeros, and both set bit 1 of the device error word.  The result
+ * does not depend on what else runs (fixed order of every sum). */
+tb_status tb_paged_attention_decode(const tb_paged_cache *cache, const tb_paged_batch *seqs, int act_dtype,
+                                    const void *q_dev, int64_t ldq, int64_t heads, float scale, void *out_dev,
+                                    int64_t ldo, void *workspace_dev, size_t workspace_bytes, tb_stream stream);
+/* The same for a batch whose sequences all begin with one common prefix of
+ * prefix_len tokens, held once: its pages are prefix_table_dev[0 ..
+ * ceil(prefix_len / page_size) - 1], and seqs describes what follows it
+ * (lens[b] >= 0 keys of each sequence behind the prefix, in pages of their
+ * own; token i there has position prefix_len + i).  Every key and value of the
+ * prefix is read once for all sequences.  prefix_len 0 is
+ * tb_paged_attention_decode. */
+tb_status tb_paged_attention_shared(const tb_paged_cache *cache, const tb_paged_batch *seqs,
+                                    const int32_t *prefix_table_dev, int64_t prefix_len, int act_dtype,
+                                    const void *q_dev, int64_t ldq, int64_t heads, float scale, void *out_dev,
+                                    int64_t ldo, void *workspace_dev, size_t workspace_bytes, tb_stream stream);
+
 /* Causal grouped-query attention of a prompt in one launch: the 32-head loop
  * of MultiHeadAttention::forward (src/nn/attention.cpp:104-141) for S query
  * tokens at positions pos0 .. pos0 + S - 1 whose keys and values are already

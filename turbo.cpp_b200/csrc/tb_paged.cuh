@@ -1,0 +1,151 @@
+// tb_paged.cuh -- what the kernels over the paged key/value cache share.
+#pragma once
+
+#include "tb_internal.cuh"
+
+namespace tb {
+
+// Activation rows (queries, new keys and values, outputs) of a run-time type.
+struct ActRows {
+  const void *p;
+  int64_t ld;  // elements between rows
+  int dtype;
+};
+
+// The device side of tb_paged_cache / tb_paged_batch.
+struct PagedPools {
+  const char *k, *v;
+  int64_t page_stride, token_stride, head_stride;  // bytes
+  uint32_t n_pages;
+  int shift, mask;  // position t: slot t & mask of its page t >> shift
+};
+struct PagedSeqs {
+  const int32_t *lens, *table;
+  int64_t table_stride;
+  int batch;
+  int max_len;  // max_pages * page_size
+};
+
+// Byte offset of a key/value head's row at slot t & mask of page `id`, or -1
+// where the page id lies outside the pool: the only way from a page table to
+// an address.
+__host__ __device__ inline int64_t row_offset(const PagedPools &p, int32_t id, int t, int64_t head) {
+  if ((uint32_t)id >= p.n_pages) return -1;
+  return id * p.page_stride + (t & p.mask) * p.token_stride + head * p.head_stride;
+}
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Checks and converts the two descriptors; `who` names the entry point.
+tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_dtype, const char *who,
+                     PagedPools *pools, PagedSeqs *seqs);
+
+// One row-tile's share of the prefix: unnormalised outputs acc[D] with their
+// running maximum m (of scale * log2(e) * q.k) and sum l, per row and split.
+// Row r of key/value head h, split s: acc at ((h * rows + r) * splits + s) * D.
+struct PrefixParts {
+  float *acc;
+  float2 *ml;
+  int rows;    // batch * group
+  int splits;  // 0: no prefix
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int src_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16-byte words of a row as floats (F32: 4, F16 and BF16: 8); exact.
+template <int DT>
+struct Word;
+template <>
+struct Word<TB_F32> {
+  static constexpr int n = 4, size = 4;
+  static __device__ __forceinline__ void get(const uint4 &w, float (&f)[4]) {
+    f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float *f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Word<TB_F16> {
+  static constexpr int n = 8, size = 2;
+  static __device__ __forceinline__ void get(const uint4 &w, float (&f)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 put(const float *f) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+template <>
+struct Word<TB_BF16> {
+  static constexpr int n = 8, size = 2;
+  static __device__ __forceinline__ void get(const uint4 &w, float (&f)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 put(const float *f) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+// N consecutive activations (N = 4 or 8) starting at element i, as floats.
+template <int N>
+__device__ __forceinline__ void load_act(const void *p, int64_t i, int dtype, float (&f)[N]) {
+  if (dtype == TB_F32) {
+    const uint4 *s = reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + i);
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+      float g[4];
+      Word<TB_F32>::get(s[k], g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * k + e] = g[e];
+    }
+  } else {  // 16-bit activations meet 16-bit caches only, whose words hold 8 elements
+    static_assert(N == 4 || N == 8, "");
+    if constexpr (N == 8) {
+      const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+      if (dtype == TB_F16) Word<TB_F16>::get(w, f);
+      else Word<TB_BF16>::get(w, f);
+    }
+  }
+}
+
+__device__ __forceinline__ void store_act1(void *p, int64_t i, int dtype, float x) {
+  if (dtype == TB_F32) static_cast<float *>(p)[i] = x;
+  else if (dtype == TB_F16) static_cast<__half *>(p)[i] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+}
+
+}  // namespace tb

@@ -1,0 +1,238 @@
+// tb_paged_append.cu -- tb_rope_paged_append: RoPE of a call's queries and keys
+// and the append of its keys and values to a paged cache, one launch for any
+// mix of prompts and single tokens.
+//
+//   q_out = R(p) q,  K[p] = R(p) k,  V[p] = v,
+//   R(p): y0 = x0 c - x1 s, y1 = x0 s + x1 c for the pairs (i, i + head_dim/2),
+// with tb_rope's fused multiply-adds in fp32, so an fp32 cache holds what
+// tb_rope and tb_copy would have put there bit for bit.
+//
+// It moves every element once and computes next to nothing, so bytes bound it.
+// A thread takes eight elements of a head's first half and the eight they are
+// paired with (16- or 32-byte loads and stores); a warp takes 32 such pairs of
+// one token, so that the token's sequence, position and page are found once per
+// warp: a 32-way search of `starts` by ballot, then one table entry.  The data
+// loads do not depend on that chain and are issued before it.
+#include <algorithm>
+
+#include "tb_paged.cuh"
+
+namespace tb {
+
+tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_dtype, const char *who,
+                     PagedPools *pools, PagedSeqs *seqs) {
+  if (!c || !b) return fail(TB_EINVAL, "%s: null descriptor", who);
+  if (c->dtype != TB_F32 && c->dtype != TB_F16 && c->dtype != TB_BF16)
+    return fail(TB_EINVAL, "%s: cache dtype %d (fp32, fp16 or bf16)", who, c->dtype);
+  if (act_dtype != TB_F32 && act_dtype != c->dtype)
+    return fail(TB_EINVAL, "%s: activations are fp32 or of the cache's type", who);
+  const int size = dtype_size(c->dtype);
+  if (c->page_size <= 0 || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(TB_EINVAL, "%s: page_size %d is not a power of two", who, c->page_size);
+  if (c->n_pages < 0 || c->n_pages > 0x7FFFFFFF || c->kv_heads <= 0 || c->kv_heads > 4096 || c->head_dim <= 0 ||
+      c->head_dim > 4096)
+    return fail(TB_EINVAL, "%s: bad cache extents", who);
+  const int64_t ext[3] = {c->n_pages, c->page_size, c->kv_heads};
+  const int64_t str[3] = {c->page_stride, c->token_stride, c->head_stride};
+  for (int i = 0; i < 3; ++i) {
+    if (ext[i] <= 1) continue;  // the stride of a single element is never used
+    if (str[i] < c->head_dim || str[i] > (int64_t(1) << 40) || str[i] * size % 16 != 0)
+      return fail(TB_EINVAL, "%s: cache strides must cover head_dim and be multiples of 16 bytes", who);
+  }
+  if (c->n_pages > 0 && (!c->k || !c->v)) return fail(TB_EINVAL, "%s: null pool", who);
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(TB_EINVAL, "%s: the pools must be 16-byte aligned", who);
+  if (b->batch < 0 || b->batch > (1 << 20) || b->max_pages < 0 || b->max_pages > 0x7FFFFFFF / c->page_size ||
+      b->table_stride < b->max_pages)
+    return fail(TB_EINVAL, "%s: bad batch extents", who);
+  if (b->batch > 0 && (!b->lens || (b->max_pages > 0 && !b->table)))
+    return fail(TB_EINVAL, "%s: null lengths or page table", who);
+  pools->k = static_cast<const char *>(c->k);
+  pools->v = static_cast<const char *>(c->v);
+  pools->page_stride = c->n_pages > 1 ? c->page_stride * size : 0;
+  pools->token_stride = c->page_size > 1 ? c->token_stride * size : 0;
+  pools->head_stride = c->kv_heads > 1 ? c->head_stride * size : 0;
+  pools->n_pages = (uint32_t)c->n_pages;
+  pools->mask = c->page_size - 1;
+  pools->shift = 0;
+  while ((1 << pools->shift) < c->page_size) ++pools->shift;
+  seqs->lens = b->lens;
+  seqs->table = b->table;
+  seqs->table_stride = b->table_stride;
+  seqs->batch = (int)b->batch;
+  seqs->max_len = (int)(b->max_pages * c->page_size);
+  return TB_OK;
+}
+
+namespace {
+
+struct AppendArgs {
+  ActRows q, k, v;
+  void *q_out;
+  int64_t ldq_out;
+  int64_t tokens;
+  int heads, kv_heads, dim;
+  int per_head;   // threads per head: dim / 16
+  int per_token;  // warps per token
+  const int32_t *starts;
+  const float *cos_t, *sin_t;  // null: no rotation
+  int rope_max_seq;
+  PagedPools pools;
+  PagedSeqs seqs;
+};
+
+template <int DT>
+__device__ __forceinline__ void put8(void *p, const float (&f)[8]) {
+  uint4 *d = static_cast<uint4 *>(p);
+  if constexpr (DT == TB_F32) {
+    d[0] = Word<TB_F32>::put(f);
+    d[1] = Word<TB_F32>::put(f + 4);
+  } else {
+    d[0] = Word<DT>::put(f);
+  }
+}
+
+// ACT, CT: types of the activations and of the cache.
+template <int ACT, int CT>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, uint32_t *__restrict__ err) {
+  constexpr int AS = Word<ACT>::size, CS = Word<CT>::size;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = a.tokens * a.per_token;
+  const int half = a.dim / 2;
+  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
+    const int64_t t = w / a.per_token;
+    const int u = (int)(w - t * a.per_token) * 32 + lane;
+    const int head = u / a.per_head, i = (u - head * a.per_head) * 8;
+    // 0: query, 1: key, 2: value, 3: none
+    const int kind = head < a.heads ? 0 : head < a.heads + a.kv_heads ? 1 : head < a.heads + 2 * a.kv_heads ? 2 : 3;
+    const int h = kind == 0 ? head : kind == 1 ? head - a.heads : head - a.heads - a.kv_heads;
+    const ActRows &src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    float x0[8], x1[8];
+    if (kind < 3) {
+      const int64_t at = t * src.ld + (int64_t)h * a.dim + i;
+      load_act<8>(src.p, at, ACT, x0);
+      load_act<8>(src.p, at + half, ACT, x1);
+    }
+    // the token's sequence: the last b with starts[b] <= t
+    int b = (int)t, pos;
+    bool have = true;
+    if (a.starts) {
+      int lo = 0, n = a.seqs.batch;  // candidates lo .. lo + n - 1
+      while (n > 1) {
+        const int step = (n + 31) / 32;
+        const int c = lo + lane * step;
+        const bool le = c < lo + n && __ldg(a.starts + c) <= t;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, le) | 1u);
+        lo += k * step;
+        n = min(step, n - k * step);
+      }
+      b = lo;
+      const int end = __ldg(a.starts + b + 1);
+      const int len = __ldg(a.seqs.lens + b);
+      have = t < end && t >= __ldg(a.starts + b);
+      pos = len - (int)(end - t);
+    } else {
+      const int len = __ldg(a.seqs.lens + b);
+      have = len != 0;
+      pos = len - 1;
+    }
+    if (!have) continue;  // an empty slot, or a row behind the last sequence
+    bool ok = pos >= 0 && pos < a.seqs.max_len && (!a.cos_t || pos < a.rope_max_seq);
+    int64_t row = -1;
+    if (ok) {
+      const int32_t id = __ldg(a.seqs.table + (int64_t)b * a.seqs.table_stride + (pos >> a.pools.shift));
+      row = row_offset(a.pools, id, pos, kind == 1 || kind == 2 ? h : 0);
+      ok = row >= 0;
+    }
+    if (!ok) {
+      if (lane == 0) atomicOr(err, ERR_INDEX);
+      continue;
+    }
+    if (kind == 3) continue;
+    if (kind < 2 && a.cos_t) {
+      float c[8], s[8];
+      load_act<8>(a.cos_t, (int64_t)pos * half + i, TB_F32, c);
+      load_act<8>(a.sin_t, (int64_t)pos * half + i, TB_F32, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y0 = __fmaf_rn(x0[e], c[e], -__fmul_rn(x1[e], s[e]));
+        x1[e] = __fmaf_rn(x0[e], s[e], __fmul_rn(x1[e], c[e]));
+        x0[e] = y0;
+      }
+    }
+    if (kind == 0) {
+      char *d = static_cast<char *>(a.q_out) + (t * a.ldq_out + (int64_t)h * a.dim + i) * AS;
+      put8<ACT>(d, x0);
+      put8<ACT>(d + half * AS, x1);
+    } else {
+      char *d = const_cast<char *>(kind == 1 ? a.pools.k : a.pools.v) + row + i * CS;
+      put8<CT>(d, x0);
+      put8<CT>(d + half * CS, x1);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_paged_batch *seqs, int act_dtype,
+                                          const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk,
+                                          const void *v_dev, int64_t ldv, int64_t tokens, int64_t heads,
+                                          const int32_t *starts_dev, const float *cos_dev, const float *sin_dev,
+                                          int64_t rope_max_seq, void *q_out_dev, int64_t ldq_out, tb_stream stream) {
+  AppendArgs a = {};
+  TB_TRY(paged_args(cache, seqs, act_dtype, "tb_rope_paged_append", &a.pools, &a.seqs));
+  const int64_t D = cache->head_dim, KVH = cache->kv_heads;
+  if (D % 16 != 0 || D > 256)
+    return fail(TB_EINVAL, "tb_rope_paged_append: head_dim %lld (a multiple of 16, at most 256)", (long long)D);
+  if (tokens < 0 || tokens > 0x7FFFFFFF || heads < 0 || heads > 65536)
+    return fail(TB_EINVAL, "tb_rope_paged_append: bad extents");
+  if (!starts_dev && tokens != seqs->batch)
+    return fail(TB_EINVAL, "tb_rope_paged_append: without starts, tokens must equal batch");
+  if ((cos_dev == nullptr) != (sin_dev == nullptr))
+    return fail(TB_EINVAL, "tb_rope_paged_append: one RoPE table without the other");
+  if (cos_dev && (rope_max_seq <= 0 || rope_max_seq > 0x7FFFFFFF))
+    return fail(TB_EINVAL, "tb_rope_paged_append: bad table length");
+  if (tokens == 0 || seqs->batch == 0) return TB_OK;
+  const int as = dtype_size(act_dtype);
+  if (!k_dev || !v_dev || (heads > 0 && (!q_dev || !q_out_dev)))
+    return fail(TB_EINVAL, "tb_rope_paged_append: null pointer");
+  if (ldk < KVH * D || ldv < KVH * D || (heads > 0 && (ldq < heads * D || ldq_out < heads * D)))
+    return fail(TB_EINVAL, "tb_rope_paged_append: row strides too small");
+  if (!aligned16(k_dev) || !aligned16(v_dev) || ldk * as % 16 != 0 || ldv * as % 16 != 0 ||
+      (heads > 0 && (!aligned16(q_dev) || !aligned16(q_out_dev) || ldq * as % 16 != 0 || ldq_out * as % 16 != 0)) ||
+      !aligned16(cos_dev) || !aligned16(sin_dev))
+    return fail(TB_EINVAL, "tb_rope_paged_append: rows and tables must be 16-byte aligned");
+  DeviceState *st;
+  TB_TRY(device_state(&st));
+  a.q = {q_dev, ldq, act_dtype};
+  a.k = {k_dev, ldk, act_dtype};
+  a.v = {v_dev, ldv, act_dtype};
+  a.q_out = q_out_dev;
+  a.ldq_out = ldq_out;
+  a.tokens = tokens;
+  a.heads = (int)heads;
+  a.kv_heads = (int)KVH;
+  a.dim = (int)D;
+  a.per_head = (int)(D / 16);
+  a.per_token = (int)(((heads + 2 * KVH) * a.per_head + 31) / 32);
+  a.starts = starts_dev;
+  a.cos_t = cos_dev;
+  a.sin_t = sin_dev;
+  a.rope_max_seq = (int)rope_max_seq;
+  const int64_t threads = tokens * a.per_token * 32;
+  cudaStream_t s = as_stream(stream);
+#define TB_APPEND(ACT, CT)                                                             \
+  do {                                                                                 \
+    auto kern = paged_append_kernel<ACT, CT>;                                          \
+    kern<<<wave_grid(kern, 256, threads, st->sm_count), 256, 0, s>>>(a, st->err_word); \
+    return check_launch("tb_rope_paged_append");                                       \
+  } while (0)
+  if (act_dtype == TB_F16) TB_APPEND(TB_F16, TB_F16);
+  if (act_dtype == TB_BF16) TB_APPEND(TB_BF16, TB_BF16);
+  if (cache->dtype == TB_F16) TB_APPEND(TB_F32, TB_F16);
+  if (cache->dtype == TB_BF16) TB_APPEND(TB_F32, TB_BF16);
+  TB_APPEND(TB_F32, TB_F32);
+#undef TB_APPEND
+}

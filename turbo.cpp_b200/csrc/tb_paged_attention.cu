@@ -1,0 +1,689 @@
+// tb_paged_attention.cu -- attention of one query token per sequence over a
+// paged key/value cache: tb_paged_attention_decode and, for a batch behind a
+// common prefix, tb_paged_attention_shared.
+//
+// Mathematics.  Per sequence b and head: s_t = scale q.k_t, out = sum_t
+// exp(s_t - m) v_t / sum_t exp(s_t - m).  Keys are taken tile by tile with the
+// running maximum m and sum l, so every key and value is read once; partial
+// results (m, l, acc) of key ranges join as acc = sum_i acc_i exp(m_i - M),
+// l = sum_i l_i exp(m_i - M), M = max_i m_i, always in the order of the keys.
+// Exponents are base 2 (scale * log2 e folded in).
+//
+// Accuracy.  Both products run on the tensor cores as kind tf32 (m16n8k8,
+// fp32 accumulation).  An fp16 or bf16 key or value is exact in tf32; an fp32
+// number x is hi + lo, its leading 11 bits and the rest rounded to 11: 22 bits.  The
+// sixteen rows of the instruction are eight heads twice: row g the hi part and
+// row g + 8 the lo part of query (or probability) row g, which the same thread
+// holds, so the second part costs no instruction where a key/value head has at
+// most eight query heads and its sum is one addition.  fp32 keys and values
+// take a second instruction for their lo part.  Products are summed inside the
+// tensor core over at most 16 keys and then added to fp32 registers.
+//
+// Layout.  A CTA of eight warps holds a tile of T keys and values in shared
+// memory (three tiles in flight by cp.async, 16-byte words swizzled by row so
+// that every 16-byte fragment load is free of bank conflicts).  HW warps take
+// eight query heads each, KW = 8 / HW take T / KW keys each; each warp keeps
+// its own (m, l, acc), joined once per item.  The order of head_dim inside the
+// dot product and of the output columns is chosen so that each thread's
+// fragments are whole 16-byte words of a row.
+//
+// Work split.  An item is one (sequence, key/value head, group of 8 HW query
+// heads); its unit of work is one tile.  The grid is one wave; CTA c takes the
+// units [c U / n, (c + 1) U / n) of all U, found on the device from the
+// lengths, so uneven batches and single long sequences fill the GPU alike and a
+// captured launch follows the lengths.  An item cut by a CTA boundary leaves
+// partial results in the workspace; the last of its CTAs to finish (a counter
+// per first CTA, reset by that CTA) joins them.
+#include <algorithm>
+
+#include "tb_paged.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int kMaxCtas = 320;                    // of a decode launch (counters and partial slots)
+constexpr int64_t kPrefixRows = 2 * 148 * 128;   // extra (row, split) pairs of prefix partials
+constexpr int kThreads = 256;
+constexpr int kWarps = 8;
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+  PagedPools pools;
+  PagedSeqs seqs;
+  ActRows q;
+  void *out;
+  int64_t ldo;
+  int kv_heads, group, head_groups;  // head_groups: items per (sequence, key/value head)
+  float scale2;                      // scale * log2(e)
+  int max_ctas;
+  int *counters;   // [kMaxCtas], zero between launches
+  float *slot_acc; // [2 kMaxCtas][8 HW][D]
+  float2 *slot_ml; // [2 kMaxCtas][8 HW]
+  PrefixParts prefix;
+  const int32_t *prefix_table;  // prefix kernel
+  int prefix_len;
+};
+
+// x = hi + lo: hi the leading 11 bits (cut off, so that it neither overflows nor
+// differs from x in sign: an infinite sum keeps its sign), lo the rest to
+// nearest: |x - hi - lo| <= 2^-22 |x|.
+__device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
+__device__ __forceinline__ float tf32_rn(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return __uint_as_float(r);
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], float b0, float b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+        "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+// CT: cache type, D: head_dim, HW: warps across query heads.
+template <int CT, int D, int HW>
+struct Cfg {
+  static constexpr int EPC = Word<CT>::n;         // elements per 16-byte word
+  static constexpr int RB = D * Word<CT>::size;   // bytes per row
+  static constexpr int CPR = RB / 16;             // words per row
+  static constexpr int T = RB > 256 ? 64 : 128;   // keys per tile
+  static constexpr int KW = kWarps / HW;          // warps across keys
+  static constexpr int KPW = T / KW;              // keys per warp and tile
+  static constexpr int NT = KPW >= 16 ? 2 : 1;    // 8-key blocks per step
+  static constexpr int R = 8 * HW;                // rows (query heads) per item
+  static constexpr int STAGE = 2 * T * RB;
+  static constexpr int MERGE = kWarps * 8 * (D + 2) * 4;
+  static constexpr int SMEM = kStages * STAGE + MERGE;
+  static constexpr int JD = D / 4 / EPC;  // 16-byte words of a key per thread
+  static constexpr int JV = D / 8 / EPC;  // 16-byte words of a value per thread and key
+};
+
+// One warp's queries (A fragments of the first product) and running state.
+template <int D>
+struct WarpState {
+  float qa[D / 8][4];
+  float acc[D / 8][2];
+  float m, l;
+};
+
+// Copies tile `tile` of a sequence's keys and values into a stage; rows at and
+// behind len (and rows of a page outside the pool) become zeros.
+template <class C>
+__device__ __forceinline__ void load_tile(uint32_t stage, const PagedPools &p, const int32_t *table, int len, int tile,
+                                          int kvh, uint32_t *err) {
+  constexpr int RPP = kThreads / C::CPR;  // rows per pass
+  const int c = threadIdx.x % C::CPR, r0 = threadIdx.x / C::CPR;
+#pragma unroll
+  for (int i = 0; i < C::T / RPP; ++i) {
+    const int r = r0 + i * RPP, t = tile * C::T + r;
+    int bytes = 0;
+    int64_t off = 0;
+    if (t < len) {
+      const int64_t row = row_offset(p, __ldg(table + (t >> p.shift)), t, kvh);
+      if (row >= 0) {
+        bytes = 16;
+        off = row + c * 16;
+      } else if (c == 0) {
+        atomicOr(err, ERR_INDEX);
+      }
+    }
+    const uint32_t dst = stage + r * C::RB + ((c ^ (r & 7)) << 4);
+    cp_async16(dst, p.k + off, bytes);
+    cp_async16(dst + C::T * C::RB, p.v + off, bytes);
+  }
+}
+
+// The queries of this warp's eight rows as hi and lo parts.  row_at(r) gives
+// the element offset of row r of the item, or -1 where there is none.
+template <class C, int D, class RowAt>
+__device__ __forceinline__ void load_q(WarpState<D> &s, const ActRows &q, int hw, RowAt row_at) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t at = row_at(hw * 8 + g);
+#pragma unroll
+  for (int j = 0; j < C::JD; ++j) {
+    const int c = 8 * (j >> 1) + 2 * t + (j & 1);
+    float f[C::EPC];
+#pragma unroll
+    for (int e = 0; e < C::EPC; ++e) f[e] = 0.f;
+    if (at >= 0) load_act<C::EPC>(q.p, at + c * C::EPC, q.dtype, f);
+#pragma unroll
+    for (int e = 0; e < C::EPC / 2; ++e) {
+      float(&a)[4] = s.qa[j * (C::EPC / 2) + e];
+      a[0] = tf32_hi(f[2 * e]);
+      a[1] = tf32_rn(f[2 * e] - a[0]);
+      a[2] = tf32_hi(f[2 * e + 1]);
+      a[3] = tf32_rn(f[2 * e + 1] - a[2]);
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void reset(WarpState<D> &s) {
+  s.m = -INFINITY;
+  s.l = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j) s.acc[j][0] = s.acc[j][1] = 0.f;
+}
+
+// This warp's keys of a tile in shared memory: n valid keys in the tile.
+template <int CT, class C, int D>
+__device__ __forceinline__ void warp_tile(WarpState<D> &s, uint32_t stage, int n, int kw, float scale2) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int STEP = 8 * C::NT;
+  const int k0 = kw * C::KPW;
+  for (int k = k0; k < min(n, k0 + C::KPW); k += STEP) {
+    // scores: thread holds keys k + 8 b + 2 t, + 1 of row g (c0, c1: hi part of q; c2, c3: lo part)
+    float p[C::NT][2];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < C::NT; ++b) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      const int row = k + 8 * b + g;
+      const uint32_t base = stage + row * C::RB;
+#pragma unroll
+      for (int j = 0; j < C::JD; ++j) {
+        const int w = 8 * (j >> 1) + 2 * t + (j & 1);
+        float f[C::EPC];
+        Word<CT>::get(lds128(base + ((w ^ (row & 7)) << 4)), f);
+#pragma unroll
+        for (int e = 0; e < C::EPC / 2; ++e) {
+          const float(&a)[4] = s.qa[j * (C::EPC / 2) + e];
+          if constexpr (CT == TB_F32) {
+            const float h0 = tf32_hi(f[2 * e]), h1 = tf32_hi(f[2 * e + 1]);
+            mma_tf32(c, a, h0, h1);
+            mma_tf32(c, a, tf32_rn(f[2 * e] - h0), tf32_rn(f[2 * e + 1] - h1));
+          } else {
+            mma_tf32(c, a, f[2 * e], f[2 * e + 1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float v = (c[i] + c[i + 2]) * scale2;
+        p[b][i] = k + 8 * b + 2 * t + i < n ? v : -INFINITY;
+        mx = fmaxf(mx, p[b][i]);
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float m = fmaxf(s.m, mx);
+    const float ms = m == -INFINITY ? 0.f : m;  // all scores -inf so far: exp2(-inf - 0) = 0, not NaN
+    const float alpha = ex2(s.m - ms);
+    s.m = m;
+    float sum = 0.f;
+    float pa[C::NT][4];
+#pragma unroll
+    for (int b = 0; b < C::NT; ++b) {
+      const float e0 = ex2(p[b][0] - ms), e1 = ex2(p[b][1] - ms);
+      sum += e0 + e1;
+      pa[b][0] = tf32_hi(e0);
+      pa[b][1] = tf32_rn(e0 - pa[b][0]);
+      pa[b][2] = tf32_hi(e1);
+      pa[b][3] = tf32_rn(e1 - pa[b][2]);
+    }
+    s.l = fmaf(s.l, alpha, sum);
+    // acc = acc alpha + p V; the instruction's k index t is key 2 t, t + 4 is key 2 t + 1
+#pragma unroll
+    for (int j = 0; j < C::JV; ++j) {
+      float f[C::NT][2][C::EPC];
+#pragma unroll
+      for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = k + 8 * b + 2 * t + i;
+          Word<CT>::get(lds128(stage + C::T * C::RB + row * C::RB + (((g + 8 * j) ^ (row & 7)) << 4)), f[b][i]);
+        }
+#pragma unroll
+      for (int e = 0; e < C::EPC; ++e) {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < C::NT; ++b) {
+          if constexpr (CT == TB_F32) {
+            const float h0 = tf32_hi(f[b][0][e]), h1 = tf32_hi(f[b][1][e]);
+            mma_tf32(c, pa[b], h0, h1);
+            mma_tf32(c, pa[b], tf32_rn(f[b][0][e] - h0), tf32_rn(f[b][1][e] - h1));
+          } else {
+            mma_tf32(c, pa[b], f[b][0][e], f[b][1][e]);
+          }
+        }
+        float(&o)[2] = s.acc[j * C::EPC + e];
+        o[0] = fmaf(o[0], alpha, c[0] + c[2]);
+        o[1] = fmaf(o[1], alpha, c[1] + c[3]);
+      }
+    }
+  }
+}
+
+// Leaves the warp's (m, l, acc) in the merge buffer: acc[8 warps][8 rows][D],
+// then ml[8][8].
+template <class C, int D>
+__device__ __forceinline__ void leave(const WarpState<D> &s, float *merge) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float l = s.l;
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  float *row = merge + (warp * 8 + g) * D;
+  // output column n of block (j, e) is element (n + 8 j) EPC + e; this thread holds n = 2 t, 2 t + 1
+#pragma unroll
+  for (int j = 0; j < C::JV; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < C::EPC; ++e) row[(2 * t + i + 8 * j) * C::EPC + e] = s.acc[j * C::EPC + e][i];
+  if (t == 0) reinterpret_cast<float2 *>(merge + kWarps * 8 * D)[warp * 8 + g] = make_float2(s.m, l);
+}
+
+// Running join of partial results of one row, N of its elements per thread.
+template <int N>
+struct Join {
+  float m = -INFINITY, l = 0.f, acc[N];
+  __device__ __forceinline__ Join() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  }
+  template <class Get>
+  __device__ __forceinline__ void add(float2 ml, Get get) {
+    const float mn = fmaxf(m, ml.x);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    const float a = ex2(m - ms), w = ex2(ml.x - ms);
+    m = mn;
+    l = fmaf(l, a, ml.y * w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(acc[i], a, get(i) * w);
+  }
+};
+
+// The warps' results of row `row` of an item, joined; thread `sub` of TPR
+// takes elements sub + TPR i.
+template <class C, int D, int N>
+__device__ __forceinline__ void join_warps(Join<N> &j, const float *merge, int row, int sub) {
+  constexpr int TPR = kThreads / C::R;
+  const int hw = row >> 3, g = row & 7;
+  const float2 *ml = reinterpret_cast<const float2 *>(merge + kWarps * 8 * D);
+#pragma unroll
+  for (int kw = 0; kw < C::KW; ++kw) {
+    const int w = kw * (kWarps / C::KW) + hw;  // warp index: kw HW + hw
+    const float *a = merge + (w * 8 + g) * D + sub;
+    j.add(ml[w * 8 + g], [&](int i) { return a[i * TPR]; });
+  }
+}
+
+// Where a CTA stands in the list of all units: item (b, i) and a tile of it.
+struct Walk {
+  int b, i, tile, tiles, len;
+};
+
+template <class C>
+__device__ __forceinline__ int tiles_of(int len) {
+  return max(1, (len + C::T - 1) / C::T);
+}
+
+__device__ __forceinline__ int seq_len(const PagedSeqs &s, int b) {
+  const int len = __ldg(s.lens + b);
+  return len < 0 || len > s.max_len ? 0 : len;
+}
+
+template <class C>
+__device__ __forceinline__ void walk_on(Walk &w, const PagedSeqs &s, int items) {
+  if (++w.tile < w.tiles) return;
+  w.tile = 0;
+  if (++w.i < items) return;
+  w.i = 0;
+  if (++w.b < s.batch) {
+    w.len = seq_len(s, w.b);
+    w.tiles = tiles_of<C>(w.len);
+  }
+}
+
+template <int CT, int D, int HW>
+__global__ void __launch_bounds__(kThreads) paged_decode_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
+  using C = Cfg<CT, D, HW>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t warp_sum[kWarps];
+  __shared__ Walk first;
+  __shared__ int64_t total_s;
+  __shared__ int last_s;
+  float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
+  const uint32_t stages = smem_addr(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hw = warp % HW, kw = warp / HW;
+  const int items = a.kv_heads * a.head_groups;
+
+  // ---- the units of all sequences, and this CTA's share
+  const int per = (a.seqs.batch + kThreads - 1) / kThreads;
+  const int b0 = min(a.seqs.batch, tid * per), b1 = min(a.seqs.batch, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int len = __ldg(a.seqs.lens + b);
+    if (blockIdx.x == 0 && (len < 0 || len > a.seqs.max_len)) atomicOr(err, ERR_INDEX);
+    mine += (int64_t)tiles_of<C>(seq_len(a.seqs, b)) * items;
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  const int64_t n_ctas = min((int64_t)a.max_ctas, total);
+  if (blockIdx.x >= n_ctas) return;
+  const int64_t u0 = blockIdx.x * total / n_ctas, u1 = (blockIdx.x + 1) * total / n_ctas;
+  if (u0 >= before && u0 < before + mine) {
+    int64_t u = u0 - before;
+    int b = b0;
+    Walk w;
+    for (;; ++b) {
+      w.len = seq_len(a.seqs, b);
+      w.tiles = tiles_of<C>(w.len);
+      const int64_t n = (int64_t)w.tiles * items;
+      if (u < n) break;
+      u -= n;
+    }
+    w.b = b;
+    w.i = (int)(u / w.tiles);
+    w.tile = (int)(u - (int64_t)w.i * w.tiles);
+    first = w;
+  }
+  __syncthreads();
+  Walk load = first, cur = first;
+
+  // ---- the pipeline: tiles ahead of the one in use
+  auto issue = [&](int64_t u) {
+    if (u < u1) {
+      load_tile<C>(stages + (uint32_t)((u - u0) % kStages) * C::STAGE, a.pools,
+                   a.seqs.table + (int64_t)load.b * a.seqs.table_stride, load.len, load.tile,
+                   load.i / a.head_groups, err);
+      walk_on<C>(load, a.seqs, items);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
+
+  WarpState<D> s;
+  int64_t item0 = u0 - cur.tile;  // first unit of the current item
+  for (int64_t u = u0; u < u1; ++u) {
+    const int kvh = cur.i / a.head_groups, hg = cur.i - kvh * a.head_groups;
+    if (u == u0 || cur.tile == 0) {
+      item0 = u - cur.tile;
+      reset(s);
+      load_q<C>(s, a.q, hw, [&](int r) -> int64_t {
+        const int gi = hg * C::R + r;
+        return gi < a.group ? (int64_t)cur.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
+      });
+    }
+    cp_async_wait<kStages - 2>();
+    __syncthreads();  // tile u is in shared memory, and tile u - 1 is no longer read
+    issue(u + kStages - 1);
+    warp_tile<CT, C>(s, stages + (uint32_t)((u - u0) % kStages) * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw,
+                     a.scale2);
+    if (cur.tile + 1 == cur.tiles || u + 1 == u1) {  // this CTA's part of the item is done
+      const int64_t item1 = item0 + cur.tiles;
+      leave<C>(s, merge);
+      __syncthreads();
+      constexpr int TPR = kThreads / C::R, N = D / TPR;
+      const int row = tid / TPR, sub = tid % TPR;
+      const int gi = hg * C::R + row;
+      Join<N> j;
+      join_warps<C, D>(j, merge, row, sub);
+      // the CTAs that share the item: owners of its first and last unit
+      const int64_t c0 = ((item0 + 1) * n_ctas - 1) / total, c1 = (item1 * n_ctas - 1) / total;
+      bool finish = true;
+      if (c0 != c1) {
+        const int64_t slot = 2 * blockIdx.x + (u0 >= item0 ? 0 : 1);
+        float *acc = a.slot_acc + (slot * C::R + row) * D + sub;
+#pragma unroll
+        for (int i = 0; i < N; ++i) __stcg(acc + i * TPR, j.acc[i]);
+        if (sub == 0) __stcg(a.slot_ml + slot * C::R + row, make_float2(j.m, j.l));
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const int before_me = atomicAdd(a.counters + c0, 1);
+          last_s = before_me == (int)(c1 - c0);
+          if (last_s) a.counters[c0] = 0;  // ready for the next launch
+        }
+        __syncthreads();
+        finish = last_s != 0;
+        if (finish) {
+          __threadfence();
+          j = Join<N>();
+          for (int64_t c = c0; c <= c1; ++c) {
+            const int64_t cs = 2 * c + (c * total / n_ctas >= item0 ? 0 : 1);
+            const float *pa = a.slot_acc + (cs * C::R + row) * D + sub;
+            j.add(__ldcg(a.slot_ml + cs * C::R + row), [&](int i) { return __ldcg(pa + i * TPR); });
+          }
+        }
+      }
+      if (finish && gi < a.group) {
+        bool none = cur.len == 0;
+        if (a.prefix.splits > 0) {
+          none = false;
+          const int64_t pr = (int64_t)kvh * a.prefix.rows + (int64_t)cur.b * a.group + gi;
+          for (int p = 0; p < a.prefix.splits; ++p) {
+            const float *pa = a.prefix.acc + (pr * a.prefix.splits + p) * D + sub;
+            j.add(__ldcg(a.prefix.ml + pr * a.prefix.splits + p), [&](int i) { return __ldcg(pa + i * TPR); });
+          }
+        }
+        const int64_t at = (int64_t)cur.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + sub;
+#pragma unroll
+        for (int i = 0; i < N; ++i) store_act1(a.out, at + i * TPR, a.q.dtype, none ? 0.f : __fdiv_rn(j.acc[i], j.l));
+      }
+      // the merge buffer is written again only after the next tile's barrier
+    }
+    walk_on<C>(cur, a.seqs, items);
+  }
+}
+
+// The prefix: item (split, row tile, key/value head), rows = the queries of all
+// sequences' heads of that key/value head, R of them per CTA.
+template <int CT, int D, int HW>
+__global__ void __launch_bounds__(kThreads) paged_prefix_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
+  using C = Cfg<CT, D, HW>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
+  const uint32_t stages = smem_addr(smem);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int hw = warp % HW, kw = warp / HW;
+  const int split = blockIdx.x, rt = blockIdx.y, kvh = blockIdx.z;
+  const int tiles = (a.prefix_len + C::T - 1) / C::T;
+  const int t0 = (int)((int64_t)split * tiles / a.prefix.splits);
+  const int t1 = (int)((int64_t)(split + 1) * tiles / a.prefix.splits);
+  auto issue = [&](int t) {
+    if (t < t1)
+      load_tile<C>(stages + (uint32_t)((t - t0) % kStages) * C::STAGE, a.pools, a.prefix_table, a.prefix_len, t, kvh, err);
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(t0 + i);
+  WarpState<D> s;
+  reset(s);
+  load_q<C>(s, a.q, hw, [&](int r) -> int64_t {
+    const int row = rt * C::R + r;
+    if (row >= a.prefix.rows) return -1;
+    const int b = row / a.group;
+    return (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D;
+  });
+  for (int t = t0; t < t1; ++t) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();
+    issue(t + kStages - 1);
+    warp_tile<CT, C>(s, stages + (uint32_t)((t - t0) % kStages) * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw,
+                     a.scale2);
+  }
+  leave<C>(s, merge);
+  __syncthreads();
+  constexpr int TPR = kThreads / C::R, N = D / TPR;
+  const int r = tid / TPR, sub = tid % TPR, row = rt * C::R + r;
+  if (row >= a.prefix.rows) return;
+  Join<N> j;
+  join_warps<C, D>(j, merge, r, sub);
+  const int64_t at = ((int64_t)kvh * a.prefix.rows + row) * a.prefix.splits + split;
+#pragma unroll
+  for (int i = 0; i < N; ++i) a.prefix.acc[at * D + sub + i * TPR] = j.acc[i];
+  if (sub == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
+}
+
+// Warps across query heads: the fewest that take the rows in one item, so that
+// as many warps as possible split the keys (up to 8 rows 1, 16: 2, 32: 4).
+int head_warps(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8; }
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+struct Layout {
+  size_t slot_acc, slot_ml, prefix_acc, prefix_ml, bytes;
+};
+Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
+  const size_t slots = 2 * kMaxCtas * 8 * (size_t)head_warps(heads / kv_heads);
+  const size_t rows = (size_t)(batch * heads + kPrefixRows);
+  Layout l;
+  l.slot_acc = up256(kMaxCtas * sizeof(int));
+  l.slot_ml = l.slot_acc + up256(slots * D * sizeof(float));
+  l.prefix_acc = l.slot_ml + up256(slots * sizeof(float2));
+  l.prefix_ml = l.prefix_acc + up256(rows * D * sizeof(float));
+  l.bytes = l.prefix_ml + up256(rows * sizeof(float2));
+  return l;
+}
+
+template <int CT, int D, int HW>
+tb_status launch_decode(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
+  using C = Cfg<CT, D, HW>;
+  auto kern = paged_decode_kernel<CT, D, HW>;
+  TB_TRY(ensure_smem_for(kern, C::SMEM));
+  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kThreads, C::SMEM);
+  a.max_ctas = std::min(ctas, kMaxCtas);
+  kern<<<a.max_ctas, kThreads, C::SMEM, s>>>(a, st->err_word);
+  return check_launch(who);
+}
+
+template <int CT, int D, int HW>
+tb_status launch_prefix(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
+  using C = Cfg<CT, D, HW>;
+  auto kern = paged_prefix_kernel<CT, D, HW>;
+  TB_TRY(ensure_smem_for(kern, C::SMEM));
+  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kThreads, C::SMEM);
+  const int row_tiles = (a.prefix.rows + C::R - 1) / C::R;
+  const int64_t items = (int64_t)row_tiles * a.kv_heads;
+  const int tiles = (a.prefix_len + C::T - 1) / C::T;
+  // one wave of CTAs, as far as the workspace holds its results
+  int64_t splits = std::min<int64_t>(tiles, std::max<int64_t>(1, ctas / items));
+  splits = std::min(splits, 1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads));
+  a.prefix.splits = (int)splits;
+  if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
+  kern<<<dim3((unsigned)splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kThreads, C::SMEM, s>>>(a, st->err_word);
+  return check_launch(who);
+}
+
+template <int CT, int D>
+tb_status run(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
+  if (a.prefix_len > 0) {
+    switch (head_warps(a.prefix.rows)) {
+      case 1: TB_TRY((launch_prefix<CT, D, 1>(a, st, s, who))); break;
+      case 2: TB_TRY((launch_prefix<CT, D, 2>(a, st, s, who))); break;
+      case 4: TB_TRY((launch_prefix<CT, D, 4>(a, st, s, who))); break;
+      default: TB_TRY((launch_prefix<CT, D, 8>(a, st, s, who))); break;
+    }
+  }
+  const int hw = head_warps(a.group);
+  a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
+  switch (hw) {
+    case 1: return launch_decode<CT, D, 1>(a, st, s, who);
+    case 2: return launch_decode<CT, D, 2>(a, st, s, who);
+    case 4: return launch_decode<CT, D, 4>(a, st, s, who);
+    default: return launch_decode<CT, D, 8>(a, st, s, who);
+  }
+}
+
+tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, const int32_t *prefix_table,
+                    int64_t prefix_len, int act_dtype, const void *q, int64_t ldq, int64_t heads, float scale,
+                    void *out, int64_t ldo, void *ws, size_t ws_bytes, cudaStream_t stream, const char *who) {
+  AttnArgs a = {};
+  TB_TRY(paged_args(cache, seqs, act_dtype, who, &a.pools, &a.seqs));
+  const int64_t D = cache->head_dim, KVH = cache->kv_heads, B = seqs->batch;
+  if (D != 64 && D != 128) return fail(TB_EINVAL, "%s: head_dim %lld (64 or 128)", who, (long long)D);
+  if (heads <= 0 || heads > 65536 || heads % KVH != 0)
+    return fail(TB_EINVAL, "%s: heads must be a positive multiple of kv_heads", who);
+  if (B * heads > (1 << 24)) return fail(TB_EINVAL, "%s: more than 2^24 query rows", who);
+  if (prefix_len < 0 || prefix_len > 0x7FFFFFFF - 65536) return fail(TB_EINVAL, "%s: bad prefix length", who);
+  if (B == 0) return TB_OK;
+  if (!q || !out || !ws || (prefix_len > 0 && !prefix_table)) return fail(TB_EINVAL, "%s: null pointer", who);
+  const int as = dtype_size(act_dtype);
+  if (ldq < heads * D || ldo < heads * D) return fail(TB_EINVAL, "%s: row strides too small", who);
+  if (!aligned16(q) || !aligned16(out) || ldq * as % 16 != 0 || ldo * as % 16 != 0)
+    return fail(TB_EINVAL, "%s: rows must be 16-byte aligned", who);
+  if ((reinterpret_cast<uintptr_t>(ws) & 255) != 0) return fail(TB_EINVAL, "%s: the workspace must be 256-byte aligned", who);
+  const Layout l = layout_of(B, heads, KVH, D);
+  if (ws_bytes < l.bytes)
+    return fail(TB_EINVAL, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, l.bytes);
+  DeviceState *st;
+  TB_TRY(device_state(&st));
+  char *w = static_cast<char *>(ws);
+  a.q = {q, ldq, act_dtype};
+  a.out = out;
+  a.ldo = ldo;
+  a.kv_heads = (int)KVH;
+  a.group = (int)(heads / KVH);
+  a.scale2 = scale * kLog2e;
+  a.counters = reinterpret_cast<int *>(w);
+  a.slot_acc = reinterpret_cast<float *>(w + l.slot_acc);
+  a.slot_ml = reinterpret_cast<float2 *>(w + l.slot_ml);
+  a.prefix.acc = reinterpret_cast<float *>(w + l.prefix_acc);
+  a.prefix.ml = reinterpret_cast<float2 *>(w + l.prefix_ml);
+  a.prefix.rows = (int)(B * a.group);
+  a.prefix_table = prefix_table;
+  a.prefix_len = (int)prefix_len;
+  switch (cache->dtype) {
+    case TB_F32: return D == 64 ? run<TB_F32, 64>(a, st, stream, who) : run<TB_F32, 128>(a, st, stream, who);
+    case TB_F16: return D == 64 ? run<TB_F16, 64>(a, st, stream, who) : run<TB_F16, 128>(a, st, stream, who);
+    default: return D == 64 ? run<TB_BF16, 64>(a, st, stream, who) : run<TB_BF16, 128>(a, st, stream, who);
+  }
+}
+
+}  // namespace
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" {
+
+tb_status tb_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                             size_t *bytes_out) {
+  if (!bytes_out) return fail(TB_EINVAL, "tb_paged_attention_workspace_bytes: null pointer");
+  if (batch < 0 || heads <= 0 || heads > 65536 || kv_heads <= 0 || heads % kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128) || batch > (1 << 20) || batch * heads > (1 << 24))
+    return fail(TB_EINVAL, "tb_paged_attention_workspace_bytes: bad extents");
+  *bytes_out = layout_of(batch, heads, kv_heads, head_dim).bytes;
+  return TB_OK;
+}
+
+tb_status tb_paged_attention_decode(const tb_paged_cache *cache, const tb_paged_batch *seqs, int act_dtype,
+                                    const void *q, int64_t ldq, int64_t heads, float scale, void *out, int64_t ldo,
+                                    void *workspace, size_t workspace_bytes, tb_stream stream) {
+  return attention(cache, seqs, nullptr, 0, act_dtype, q, ldq, heads, scale, out, ldo, workspace, workspace_bytes,
+                   as_stream(stream), "tb_paged_attention_decode");
+}
+
+tb_status tb_paged_attention_shared(const tb_paged_cache *cache, const tb_paged_batch *seqs,
+                                    const int32_t *prefix_table, int64_t prefix_len, int act_dtype, const void *q,
+                                    int64_t ldq, int64_t heads, float scale, void *out, int64_t ldo, void *workspace,
+                                    size_t workspace_bytes, tb_stream stream) {
+  return attention(cache, seqs, prefix_table, prefix_len, act_dtype, q, ldq, heads, scale, out, ldo, workspace,
+                   workspace_bytes, as_stream(stream), "tb_paged_attention_shared");
+}
+
+}  // extern "C"

@@ -36,12 +36,28 @@ class View(ctypes.Structure):
                 ("strides", ctypes.c_int64 * MAX_RANK)]
 
 
+class PagedCache(ctypes.Structure):
+    """tb_paged_cache: the pools, their type, extents and strides (elements)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("n_pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("page_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class PagedBatch(ctypes.Structure):
+    """tb_paged_batch: lengths and page table of a batch of sequences."""
+    _fields_ = [("batch", ctypes.c_int64), ("lens", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("max_pages", ctypes.c_int64), ("table_stride", ctypes.c_int64)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
 _VP = ctypes.POINTER(View)
+_PC = ctypes.POINTER(PagedCache)
+_PB = ctypes.POINTER(PagedBatch)
 
 SIGNATURES = {
     "tb_init": [_I],
@@ -93,6 +109,10 @@ SIGNATURES = {
     "tb_gemv_q8_0_row_sharded": [_P, _P, _I64, _P, _I64, _P, _P],
     "tb_decode_workspace_bytes": [_P, ctypes.POINTER(_SZ)],
     "tb_attention_prefill": [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, _I64, _P],
+    "tb_rope_paged_append": [_PC, _PB, _I, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P],
+    "tb_paged_attention_workspace_bytes": [_I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)],
+    "tb_paged_attention_decode": [_PC, _PB, _I, _P, _I64, _I64, _F, _P, _I64, _P, _SZ, _P],
+    "tb_paged_attention_shared": [_PC, _PB, _P, _I64, _I, _P, _I64, _I64, _F, _P, _I64, _P, _SZ, _P],
     "tb_decode_step_persistent": [_P, _P],
     "tb_rope_at": [_VP, _P, _P, _I64, _I64, _P, _P],
     "tb_kv_append": [_P, _P, _P, _P, _I64, _I64, _P, _P],
@@ -190,6 +210,36 @@ def view(base, offset=None, shape=None, strides=None, dtype=None):
         v.shape[i] = int(s)
         v.strides[i] = int(st)
     return v
+
+
+def paged_cache(k, v):
+    """A tb_paged_cache over two pools given as torch tensors [pages,
+    page_size, kv_heads, head_dim] (permuted views of head-major pools
+    included).  The caller keeps the tensors."""
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4:
+        raise ValueError("paged_cache: k and v need the same 4-d shape, strides and type")
+    if k.shape[3] > 1 and k.stride(3) != 1:
+        raise ValueError("paged_cache: the elements of a head must be contiguous")
+    c = PagedCache()
+    c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), dtype_code(k)
+    c.n_pages, c.page_size, c.kv_heads, c.head_dim = k.shape
+    c.page_stride, c.token_stride, c.head_stride = k.stride()[:3]
+    return c
+
+
+def paged_batch(lens, table):
+    """A tb_paged_batch over int32 tensors lens [batch] and table [batch,
+    max_pages].  The caller keeps the tensors."""
+    import torch
+    if lens.dtype != torch.int32 or table.dtype != torch.int32:
+        raise ValueError("paged_batch: lens and table are int32")
+    if lens.dim() != 1 or not lens.is_contiguous() or table.dim() != 2 or table.shape[0] != lens.shape[0] or (
+            table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("paged_batch: lens [batch], table [batch, max_pages] with contiguous rows")
+    b = PagedBatch()
+    b.batch, b.lens, b.table = lens.shape[0], lens.data_ptr(), table.data_ptr()
+    b.max_pages, b.table_stride = table.shape[1], max(table.stride(0), table.shape[1])
+    return b
 
 
 def byref(v):

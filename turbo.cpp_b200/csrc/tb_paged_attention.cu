@@ -9,23 +9,29 @@
 // l = sum_i l_i exp(m_i - M), M = max_i m_i, always in the order of the keys.
 // Exponents are base 2 (scale * log2 e folded in).
 //
-// Accuracy.  Both products run on the tensor cores as kind tf32 (m16n8k8,
-// fp32 accumulation).  An fp16 or bf16 key or value is exact in tf32; an fp32
-// number x is hi + lo, its leading 11 bits and the rest rounded to 11: 22 bits.  The
-// sixteen rows of the instruction are eight heads twice: row g the hi part and
-// row g + 8 the lo part of query (or probability) row g, which the same thread
-// holds, so the second part costs no instruction where a key/value head has at
-// most eight query heads and its sum is one addition.  fp32 keys and values
-// take a second instruction for their lo part.  Products are summed inside the
-// tensor core over at most 16 keys and then added to fp32 registers.
+// Accuracy.  Both products run on the tensor cores with fp32 accumulation, the
+// keys and values as they are stored, queries and probabilities in parts, so
+// that no rounding below 22 bits happens before the result's own:
+//   fp16 cache  m16n8k16; an fp32 query is hi + lo in fp16 after a power of two
+//               per row (fp16's range), a probability times 2^15 likewise
+//   bf16 cache  m16n8k16; an fp32 query is three bf16 parts; probabilities
+//               three parts with fp32 activations, two with bf16 ones
+//   fp32 cache  m16n8k8 in tf32: queries, keys, probabilities and values all
+//               as hi + lo (the leading 11 bits and the rest rounded to 11)
+// The sixteen rows of the instruction are eight heads twice: row g holds one
+// part and row g + 8 the next part of query (or probability) row g, which the
+// same thread holds, so a second part costs no instruction where a key/value
+// head has at most eight query heads, and their sum is one addition.  16-bit
+// queries are exact in one part.  Products are summed inside the tensor core
+// over 16 keys and then added to fp32 registers.
 //
 // Layout.  A CTA of eight warps holds a tile of T keys and values in shared
 // memory (three tiles in flight by cp.async, 16-byte words swizzled by row so
 // that every 16-byte fragment load is free of bank conflicts).  HW warps take
 // eight query heads each, KW = 8 / HW take T / KW keys each; each warp keeps
 // its own (m, l, acc), joined once per item.  The order of head_dim inside the
-// dot product and of the output columns is chosen so that each thread's
-// fragments are whole 16-byte words of a row.
+// dot product is chosen so that each thread's fragments are whole 16-byte words
+// of a key; 16-bit values are read transposed by ldmatrix.
 //
 // Work split.  An item is one (sequence, key/value head, group of 8 HW query
 // heads); its unit of work is one tile.  The grid is one wave; CTA c takes the
@@ -76,7 +82,7 @@ __device__ __forceinline__ float tf32_rn(float x) {
 }
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], float b0, float b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -84,15 +90,64 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], flo
         "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 
+template <int CT>
+__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (CT == TB_F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
-// CT: cache type, D: head_dim, HW: warps across query heads.
-template <int CT, int D, int HW>
+// Four 8 x 8 blocks of 16-bit elements, transposed; lane i names row i % 8 of block i / 8.
+__device__ __forceinline__ uint4 ldmatrix_t(uint32_t addr) {
+  uint4 v;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Two floats as one register of type CT, to nearest, and what is left of them.
+template <int CT>
+__device__ __forceinline__ uint32_t pack_rest(float &x, float &y) {
+  uint32_t u;
+  if constexpr (CT == TB_F16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    u = *reinterpret_cast<const uint32_t *>(&h);
+    const float2 f = __half22float2(h);
+    x -= f.x, y -= f.y;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    u = *reinterpret_cast<const uint32_t *>(&h);
+    x -= __uint_as_float(u << 16), y -= __uint_as_float(u & 0xFFFF0000u);
+  }
+  return u;
+}
+
+// CT: cache type, D: head_dim, HW: warps across query heads, A32: fp32 activations.
+template <int CT_, int D, int HW, bool A32>
 struct Cfg {
+  static constexpr int CT = CT_;
+  // 16-bit caches: instructions per block (each takes two parts of a row)
+  static constexpr int QT = CT == TB_BF16 && A32 ? 2 : 1;
+  static constexpr int QR = A32 ? 4 : 2;          // registers of a query fragment (16-bit queries: no second part)
+  static constexpr float PSCALE = CT == TB_F16 ? 32768.f : 1.f;  // of probabilities, for fp16's range
   static constexpr int EPC = Word<CT>::n;         // elements per 16-byte word
   static constexpr int RB = D * Word<CT>::size;   // bytes per row
   static constexpr int CPR = RB / 16;             // words per row
@@ -109,9 +164,11 @@ struct Cfg {
 };
 
 // One warp's queries (A fragments of the first product) and running state.
-template <int D>
+template <class C, int D>
 struct WarpState {
-  float qa[D / 8][4];
+  float qa[C::CT == TB_F32 ? D / 8 : 1][4];
+  uint32_t qh[C::CT == TB_F32 ? 1 : D / 16][C::QT][C::QR];
+  float scale2;  // scale * log2(e) over the power of two in the queries' row
   float acc[D / 8][2];
   float m, l;
 };
@@ -143,32 +200,74 @@ __device__ __forceinline__ void load_tile(uint32_t stage, const PagedPools &p, c
   }
 }
 
-// The queries of this warp's eight rows as hi and lo parts.  row_at(r) gives
-// the element offset of row r of the item, or -1 where there is none.
+// The queries of this warp's eight rows in parts.  row_at(r) gives the element
+// offset of row r of the item, or -1 where there is none.
 template <class C, int D, class RowAt>
-__device__ __forceinline__ void load_q(WarpState<D> &s, const ActRows &q, int hw, RowAt row_at) {
+__device__ __forceinline__ void load_q(WarpState<C, D> &s, const ActRows &q, float scale2, int hw, RowAt row_at) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t at = row_at(hw * 8 + g);
+  float f[C::JD][C::EPC];
 #pragma unroll
   for (int j = 0; j < C::JD; ++j) {
     const int c = 8 * (j >> 1) + 2 * t + (j & 1);
-    float f[C::EPC];
 #pragma unroll
-    for (int e = 0; e < C::EPC; ++e) f[e] = 0.f;
-    if (at >= 0) load_act<C::EPC>(q.p, at + c * C::EPC, q.dtype, f);
+    for (int e = 0; e < C::EPC; ++e) f[j][e] = 0.f;
+    if (at >= 0) load_act<C::EPC>(q.p, at + c * C::EPC, C::QR == 4 ? TB_F32 : C::CT, f[j]);
+  }
+  s.scale2 = scale2;
+  if constexpr (C::CT == TB_F16 && C::QR == 4) {
+    float mx = 0.f;
 #pragma unroll
-    for (int e = 0; e < C::EPC / 2; ++e) {
-      float(&a)[4] = s.qa[j * (C::EPC / 2) + e];
-      a[0] = tf32_hi(f[2 * e]);
-      a[1] = tf32_rn(f[2 * e] - a[0]);
-      a[2] = tf32_hi(f[2 * e + 1]);
-      a[3] = tf32_rn(f[2 * e + 1] - a[2]);
+    for (int j = 0; j < C::JD; ++j)
+#pragma unroll
+      for (int e = 0; e < C::EPC; ++e) mx = fmaxf(mx, fabsf(f[j][e]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // the power of two that brings the row's maximum into [2^14, 2^15); none for 0, inf, NaN
+    const int E = (int)(__float_as_uint(mx) >> 23);
+    const int e = mx == 0.f || E == 255 ? 0 : min(max(141 - E, -126), 126);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    s.scale2 = scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int j = 0; j < C::JD; ++j)
+#pragma unroll
+      for (int k = 0; k < C::EPC; ++k) f[j][k] *= up;
+  }
+#pragma unroll
+  for (int j = 0; j < C::JD; ++j) {
+    if constexpr (C::CT == TB_F32) {
+#pragma unroll
+      for (int e = 0; e < C::EPC / 2; ++e) {
+        float(&a)[4] = s.qa[j * (C::EPC / 2) + e];
+        a[0] = tf32_hi(f[j][2 * e]);
+        a[1] = tf32_rn(f[j][2 * e] - a[0]);
+        a[2] = tf32_hi(f[j][2 * e + 1]);
+        a[3] = tf32_rn(f[j][2 * e + 1] - a[2]);
+      }
+    } else {
+      // instruction e of a 16-byte word takes its elements 4 e .. 4 e + 3
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int p = 0; p < C::QT; ++p) {
+          uint32_t(&a)[C::QR] = s.qh[2 * j + e][p];
+          float(&x)[C::EPC] = f[j];
+          if constexpr (C::QR == 2) {
+            a[0] = pack_rest<C::CT>(x[4 * e], x[4 * e + 1]);
+            a[1] = pack_rest<C::CT>(x[4 * e + 2], x[4 * e + 3]);
+          } else {
+            a[0] = pack_rest<C::CT>(x[4 * e], x[4 * e + 1]);
+            a[2] = pack_rest<C::CT>(x[4 * e + 2], x[4 * e + 3]);
+            a[1] = pack_rest<C::CT>(x[4 * e], x[4 * e + 1]);
+            a[3] = pack_rest<C::CT>(x[4 * e + 2], x[4 * e + 3]);
+          }
+        }
     }
   }
 }
 
-template <int D>
-__device__ __forceinline__ void reset(WarpState<D> &s) {
+template <class C, int D>
+__device__ __forceinline__ void reset(WarpState<C, D> &s) {
   s.m = -INFINITY;
   s.l = 0.f;
 #pragma unroll
@@ -176,44 +275,66 @@ __device__ __forceinline__ void reset(WarpState<D> &s) {
 }
 
 // This warp's keys of a tile in shared memory: n valid keys in the tile.
-template <int CT, class C, int D>
-__device__ __forceinline__ void warp_tile(WarpState<D> &s, uint32_t stage, int n, int kw, float scale2) {
+template <class C, int D>
+__device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, int n, int kw) {
+  constexpr int CT = C::CT;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   constexpr int STEP = 8 * C::NT;
   const int k0 = kw * C::KPW;
   for (int k = k0; k < min(n, k0 + C::KPW); k += STEP) {
-    // scores: thread holds keys k + 8 b + 2 t, + 1 of row g (c0, c1: hi part of q; c2, c3: lo part)
+    // scores: thread holds keys k + 8 b + 2 t, + 1 of row g (c0, c1: first part of q; c2, c3: second)
+    float c[C::NT][4];
+#pragma unroll
+    for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[b][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < C::JD; ++j) {
+      const int w = 8 * (j >> 1) + 2 * t + (j & 1);
+      uint4 u[C::NT];
+#pragma unroll
+      for (int b = 0; b < C::NT; ++b) {
+        const int row = k + 8 * b + g;
+        u[b] = lds128(stage + row * C::RB + ((w ^ (row & 7)) << 4));
+      }
+      if constexpr (CT == TB_F32) {
+#pragma unroll
+        for (int b = 0; b < C::NT; ++b) {
+          float f[4];
+          Word<TB_F32>::get(u[b], f);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float(&a)[4] = s.qa[2 * j + e];
+            const float h0 = tf32_hi(f[2 * e]), h1 = tf32_hi(f[2 * e + 1]);
+            mma_tf32(c[b], a, h0, h1);
+            mma_tf32(c[b], a, tf32_rn(f[2 * e] - h0), tf32_rn(f[2 * e + 1] - h1));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < C::QT; ++p)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int b = 0; b < C::NT; ++b) {
+              const uint32_t(&q)[C::QR] = s.qh[2 * j + e][p];
+              uint32_t a[4];
+              if constexpr (C::QR == 2) a[0] = q[0], a[1] = 0u, a[2] = q[1], a[3] = 0u;
+              else a[0] = q[0], a[1] = q[1], a[2] = q[2], a[3] = q[3];
+              mma_16<CT>(c[b], a, e ? u[b].z : u[b].x, e ? u[b].w : u[b].y);
+            }
+      }
+    }
     float p[C::NT][2];
     float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < C::NT; ++b) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      const int row = k + 8 * b + g;
-      const uint32_t base = stage + row * C::RB;
-#pragma unroll
-      for (int j = 0; j < C::JD; ++j) {
-        const int w = 8 * (j >> 1) + 2 * t + (j & 1);
-        float f[C::EPC];
-        Word<CT>::get(lds128(base + ((w ^ (row & 7)) << 4)), f);
-#pragma unroll
-        for (int e = 0; e < C::EPC / 2; ++e) {
-          const float(&a)[4] = s.qa[j * (C::EPC / 2) + e];
-          if constexpr (CT == TB_F32) {
-            const float h0 = tf32_hi(f[2 * e]), h1 = tf32_hi(f[2 * e + 1]);
-            mma_tf32(c, a, h0, h1);
-            mma_tf32(c, a, tf32_rn(f[2 * e] - h0), tf32_rn(f[2 * e + 1] - h1));
-          } else {
-            mma_tf32(c, a, f[2 * e], f[2 * e + 1]);
-          }
-        }
-      }
+    for (int b = 0; b < C::NT; ++b)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float v = (c[i] + c[i + 2]) * scale2;
+        const float v = (C::QR == 4 ? c[b][i] + c[b][i + 2] : c[b][i]) * s.scale2;
         p[b][i] = k + 8 * b + 2 * t + i < n ? v : -INFINITY;
         mx = fmaxf(mx, p[b][i]);
       }
-    }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const float m = fmaxf(s.m, mx);
@@ -221,44 +342,82 @@ __device__ __forceinline__ void warp_tile(WarpState<D> &s, uint32_t stage, int n
     const float alpha = ex2(s.m - ms);
     s.m = m;
     float sum = 0.f;
-    float pa[C::NT][4];
 #pragma unroll
-    for (int b = 0; b < C::NT; ++b) {
-      const float e0 = ex2(p[b][0] - ms), e1 = ex2(p[b][1] - ms);
-      sum += e0 + e1;
-      pa[b][0] = tf32_hi(e0);
-      pa[b][1] = tf32_rn(e0 - pa[b][0]);
-      pa[b][2] = tf32_hi(e1);
-      pa[b][3] = tf32_rn(e1 - pa[b][2]);
-    }
+    for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        p[b][i] = ex2(p[b][i] - ms);
+        sum += p[b][i];
+      }
     s.l = fmaf(s.l, alpha, sum);
-    // acc = acc alpha + p V; the instruction's k index t is key 2 t, t + 4 is key 2 t + 1
+    // acc = acc alpha + p V
+    const uint32_t vt = stage + C::T * C::RB;
+    if constexpr (CT == TB_F32) {
+      // the instruction's k index t is key 2 t, t + 4 is key 2 t + 1; output column n of block (j, e) is element
+      // (n + 8 j) EPC + e
+      float pa[C::NT][4];
 #pragma unroll
-    for (int j = 0; j < C::JV; ++j) {
-      float f[C::NT][2][C::EPC];
+      for (int b = 0; b < C::NT; ++b) {
+        pa[b][0] = tf32_hi(p[b][0]);
+        pa[b][1] = tf32_rn(p[b][0] - pa[b][0]);
+        pa[b][2] = tf32_hi(p[b][1]);
+        pa[b][3] = tf32_rn(p[b][1] - pa[b][2]);
+      }
 #pragma unroll
-      for (int b = 0; b < C::NT; ++b)
+      for (int j = 0; j < C::JV; ++j) {
+        float f[C::NT][2][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = k + 8 * b + 2 * t + i;
-          Word<CT>::get(lds128(stage + C::T * C::RB + row * C::RB + (((g + 8 * j) ^ (row & 7)) << 4)), f[b][i]);
-        }
+        for (int b = 0; b < C::NT; ++b)
 #pragma unroll
-      for (int e = 0; e < C::EPC; ++e) {
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int b = 0; b < C::NT; ++b) {
-          if constexpr (CT == TB_F32) {
-            const float h0 = tf32_hi(f[b][0][e]), h1 = tf32_hi(f[b][1][e]);
-            mma_tf32(c, pa[b], h0, h1);
-            mma_tf32(c, pa[b], tf32_rn(f[b][0][e] - h0), tf32_rn(f[b][1][e] - h1));
-          } else {
-            mma_tf32(c, pa[b], f[b][0][e], f[b][1][e]);
+          for (int i = 0; i < 2; ++i) {
+            const int row = k + 8 * b + 2 * t + i;
+            Word<TB_F32>::get(lds128(vt + row * C::RB + (((g + 8 * j) ^ (row & 7)) << 4)), f[b][i]);
           }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int b = 0; b < C::NT; ++b) {
+            const float h0 = tf32_hi(f[b][0][e]), h1 = tf32_hi(f[b][1][e]);
+            mma_tf32(o, pa[b], h0, h1);
+            mma_tf32(o, pa[b], tf32_rn(f[b][0][e] - h0), tf32_rn(f[b][1][e] - h1));
+          }
+          float(&r)[2] = s.acc[j * 4 + e];
+          r[0] = fmaf(r[0], alpha, o[0] + o[2]);
+          r[1] = fmaf(r[1], alpha, o[1] + o[3]);
         }
-        float(&o)[2] = s.acc[j * C::EPC + e];
-        o[0] = fmaf(o[0], alpha, c[0] + c[2]);
-        o[1] = fmaf(o[1], alpha, c[1] + c[3]);
+      }
+    } else {
+      uint32_t pa[C::QT][4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) p[b][i] *= C::PSCALE;
+#pragma unroll
+      for (int q = 0; q < C::QT; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) pa[q][2 * b + h] = pack_rest<CT>(p[b][0], p[b][1]);
+      const int row = k + (lane & 15);  // blocks: keys 0-7, 8-15 of word w, then of word w + 1
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const int w = 2 * j + (lane >> 4);
+        const uint4 v = ldmatrix_t(vt + row * C::RB + ((w ^ (row & 7)) << 4));
+        float o[2][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[0][i] = o[1][i] = 0.f;
+#pragma unroll
+        for (int q = 0; q < C::QT; ++q) {
+          mma_16<CT>(o[0], pa[q], v.x, v.y);
+          mma_16<CT>(o[1], pa[q], v.z, v.w);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float(&r)[2] = s.acc[2 * j + h];
+          r[0] = fmaf(r[0], alpha, o[h][0] + o[h][2]);
+          r[1] = fmaf(r[1], alpha, o[h][1] + o[h][3]);
+        }
       }
     }
   }
@@ -267,19 +426,25 @@ __device__ __forceinline__ void warp_tile(WarpState<D> &s, uint32_t stage, int n
 // Leaves the warp's (m, l, acc) in the merge buffer: acc[8 warps][8 rows][D],
 // then ml[8][8].
 template <class C, int D>
-__device__ __forceinline__ void leave(const WarpState<D> &s, float *merge) {
+__device__ __forceinline__ void leave(const WarpState<C, D> &s, float *merge) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float l = s.l;
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
   float *row = merge + (warp * 8 + g) * D;
-  // output column n of block (j, e) is element (n + 8 j) EPC + e; this thread holds n = 2 t, 2 t + 1
+  if constexpr (C::CT == TB_F32) {
 #pragma unroll
-  for (int j = 0; j < C::JV; ++j)
+    for (int j = 0; j < C::JV; ++j)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < C::EPC; ++e) row[(2 * t + i + 8 * j) * C::EPC + e] = s.acc[j * C::EPC + e][i];
+        for (int e = 0; e < C::EPC; ++e) row[(2 * t + i + 8 * j) * C::EPC + e] = s.acc[j * C::EPC + e][i];
+  } else {
+    constexpr float down = 1.f / C::PSCALE;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+      *reinterpret_cast<float2 *>(row + 8 * j + 2 * t) = make_float2(s.acc[j][0] * down, s.acc[j][1] * down);
+  }
   if (t == 0) reinterpret_cast<float2 *>(merge + kWarps * 8 * D)[warp * 8 + g] = make_float2(s.m, l);
 }
 
@@ -345,9 +510,9 @@ __device__ __forceinline__ void walk_on(Walk &w, const PagedSeqs &s, int items) 
   }
 }
 
-template <int CT, int D, int HW>
-__global__ void __launch_bounds__(kThreads) paged_decode_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
-  using C = Cfg<CT, D, HW>;
+template <int CT, int D, int HW, bool A32>
+__global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1024 ? 2 : 1) paged_decode_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
+  using C = Cfg<CT, D, HW, A32>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t warp_sum[kWarps];
   __shared__ Walk first;
@@ -416,14 +581,14 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const AttnArgs a
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
 
-  WarpState<D> s;
+  WarpState<C, D> s;
   int64_t item0 = u0 - cur.tile;  // first unit of the current item
   for (int64_t u = u0; u < u1; ++u) {
     const int kvh = cur.i / a.head_groups, hg = cur.i - kvh * a.head_groups;
     if (u == u0 || cur.tile == 0) {
       item0 = u - cur.tile;
       reset(s);
-      load_q<C>(s, a.q, hw, [&](int r) -> int64_t {
+      load_q(s, a.q, a.scale2, hw, [&](int r) -> int64_t {
         const int gi = hg * C::R + r;
         return gi < a.group ? (int64_t)cur.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
       });
@@ -431,11 +596,10 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const AttnArgs a
     cp_async_wait<kStages - 2>();
     __syncthreads();  // tile u is in shared memory, and tile u - 1 is no longer read
     issue(u + kStages - 1);
-    warp_tile<CT, C>(s, stages + (uint32_t)((u - u0) % kStages) * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw,
-                     a.scale2);
+    warp_tile(s, stages + (uint32_t)((u - u0) % kStages) * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw);
     if (cur.tile + 1 == cur.tiles || u + 1 == u1) {  // this CTA's part of the item is done
       const int64_t item1 = item0 + cur.tiles;
-      leave<C>(s, merge);
+      leave(s, merge);
       __syncthreads();
       constexpr int TPR = kThreads / C::R, N = D / TPR;
       const int row = tid / TPR, sub = tid % TPR;
@@ -492,9 +656,9 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const AttnArgs a
 
 // The prefix: item (split, row tile, key/value head), rows = the queries of all
 // sequences' heads of that key/value head, R of them per CTA.
-template <int CT, int D, int HW>
-__global__ void __launch_bounds__(kThreads) paged_prefix_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
-  using C = Cfg<CT, D, HW>;
+template <int CT, int D, int HW, bool A32>
+__global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1024 ? 2 : 1) paged_prefix_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
+  using C = Cfg<CT, D, HW, A32>;
   extern __shared__ __align__(128) unsigned char smem[];
   float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
   const uint32_t stages = smem_addr(smem);
@@ -511,9 +675,9 @@ __global__ void __launch_bounds__(kThreads) paged_prefix_kernel(const AttnArgs a
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue(t0 + i);
-  WarpState<D> s;
+  WarpState<C, D> s;
   reset(s);
-  load_q<C>(s, a.q, hw, [&](int r) -> int64_t {
+  load_q(s, a.q, a.scale2, hw, [&](int r) -> int64_t {
     const int row = rt * C::R + r;
     if (row >= a.prefix.rows) return -1;
     const int b = row / a.group;
@@ -523,10 +687,9 @@ __global__ void __launch_bounds__(kThreads) paged_prefix_kernel(const AttnArgs a
     cp_async_wait<kStages - 2>();
     __syncthreads();
     issue(t + kStages - 1);
-    warp_tile<CT, C>(s, stages + (uint32_t)((t - t0) % kStages) * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw,
-                     a.scale2);
+    warp_tile(s, stages + (uint32_t)((t - t0) % kStages) * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw);
   }
-  leave<C>(s, merge);
+  leave(s, merge);
   __syncthreads();
   constexpr int TPR = kThreads / C::R, N = D / TPR;
   const int r = tid / TPR, sub = tid % TPR, row = rt * C::R + r;
@@ -560,10 +723,10 @@ Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   return l;
 }
 
-template <int CT, int D, int HW>
+template <int CT, int D, int HW, bool A32>
 tb_status launch_decode(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
-  using C = Cfg<CT, D, HW>;
-  auto kern = paged_decode_kernel<CT, D, HW>;
+  using C = Cfg<CT, D, HW, A32>;
+  auto kern = paged_decode_kernel<CT, D, HW, A32>;
   TB_TRY(ensure_smem_for(kern, C::SMEM));
   const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kThreads, C::SMEM);
   a.max_ctas = std::min(ctas, kMaxCtas);
@@ -571,10 +734,10 @@ tb_status launch_decode(AttnArgs &a, const DeviceState *st, cudaStream_t s, cons
   return check_launch(who);
 }
 
-template <int CT, int D, int HW>
+template <int CT, int D, int HW, bool A32>
 tb_status launch_prefix(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
-  using C = Cfg<CT, D, HW>;
-  auto kern = paged_prefix_kernel<CT, D, HW>;
+  using C = Cfg<CT, D, HW, A32>;
+  auto kern = paged_prefix_kernel<CT, D, HW, A32>;
   TB_TRY(ensure_smem_for(kern, C::SMEM));
   const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kThreads, C::SMEM);
   const int row_tiles = (a.prefix.rows + C::R - 1) / C::R;
@@ -589,23 +752,23 @@ tb_status launch_prefix(AttnArgs &a, const DeviceState *st, cudaStream_t s, cons
   return check_launch(who);
 }
 
-template <int CT, int D>
+template <int CT, int D, bool A32>
 tb_status run(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
   if (a.prefix_len > 0) {
     switch (head_warps(a.prefix.rows)) {
-      case 1: TB_TRY((launch_prefix<CT, D, 1>(a, st, s, who))); break;
-      case 2: TB_TRY((launch_prefix<CT, D, 2>(a, st, s, who))); break;
-      case 4: TB_TRY((launch_prefix<CT, D, 4>(a, st, s, who))); break;
-      default: TB_TRY((launch_prefix<CT, D, 8>(a, st, s, who))); break;
+      case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, st, s, who))); break;
+      case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, st, s, who))); break;
+      case 4: TB_TRY((launch_prefix<CT, D, 4, A32>(a, st, s, who))); break;
+      default: TB_TRY((launch_prefix<CT, D, 8, A32>(a, st, s, who))); break;
     }
   }
   const int hw = head_warps(a.group);
   a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
   switch (hw) {
-    case 1: return launch_decode<CT, D, 1>(a, st, s, who);
-    case 2: return launch_decode<CT, D, 2>(a, st, s, who);
-    case 4: return launch_decode<CT, D, 4>(a, st, s, who);
-    default: return launch_decode<CT, D, 8>(a, st, s, who);
+    case 1: return launch_decode<CT, D, 1, A32>(a, st, s, who);
+    case 2: return launch_decode<CT, D, 2, A32>(a, st, s, who);
+    case 4: return launch_decode<CT, D, 4, A32>(a, st, s, who);
+    default: return launch_decode<CT, D, 8, A32>(a, st, s, who);
   }
 }
 
@@ -647,11 +810,13 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
   a.prefix.rows = (int)(B * a.group);
   a.prefix_table = prefix_table;
   a.prefix_len = (int)prefix_len;
-  switch (cache->dtype) {
-    case TB_F32: return D == 64 ? run<TB_F32, 64>(a, st, stream, who) : run<TB_F32, 128>(a, st, stream, who);
-    case TB_F16: return D == 64 ? run<TB_F16, 64>(a, st, stream, who) : run<TB_F16, 128>(a, st, stream, who);
-    default: return D == 64 ? run<TB_BF16, 64>(a, st, stream, who) : run<TB_BF16, 128>(a, st, stream, who);
-  }
+#define TB_RUN(CT, A32) return D == 64 ? run<CT, 64, A32>(a, st, stream, who) : run<CT, 128, A32>(a, st, stream, who)
+  if (act_dtype == TB_F16) TB_RUN(TB_F16, false);
+  if (act_dtype == TB_BF16) TB_RUN(TB_BF16, false);
+  if (cache->dtype == TB_F16) TB_RUN(TB_F16, true);
+  if (cache->dtype == TB_BF16) TB_RUN(TB_BF16, true);
+  TB_RUN(TB_F32, true);
+#undef TB_RUN
 }
 
 }  // namespace

@@ -1,6 +1,8 @@
 // tb_paged.cuh -- what the kernels over the paged key/value cache share.
 #pragma once
 
+#include <cuda.h>
+
 #include "tb_internal.cuh"
 
 namespace tb {
@@ -28,7 +30,7 @@ struct PagedSeqs {
 
 // Byte offset of a key/value head's row at slot t & mask of page `id`, or -1
 // where the page id lies outside the pool: the only way from a page table to
-// an address.
+// an address in this code (TMA checks its coordinates itself).
 __host__ __device__ inline int64_t row_offset(const PagedPools &p, int32_t id, int t, int64_t head) {
   if ((uint32_t)id >= p.n_pages) return -1;
   return id * p.page_stride + (t & p.mask) * p.token_stride + head * p.head_stride;
@@ -50,13 +52,21 @@ struct PrefixParts {
   int splits;  // 0: no prefix
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// The pools as 4-d tensors [page][token][head][head_dim] for TMA: a box is up
+// to `box_rows` tokens of one page and head, 128 bytes of each row, swizzled.
+struct PagedMaps {
+  CUtensorMap k, v;
+};
+// `rows` tokens per box at most; *box_rows gets the smaller of that and page_size.
+tb_status paged_maps(const tb_paged_cache *c, int rows, const char *who, PagedMaps *maps, int *box_rows);
+
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int head, int token, int page,
+                                        uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+          "r"(dst),
+      "l"(map), "r"(x), "r"(head), "r"(token), "r"(page), "r"(smem_addr(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ float ex2(float x) {

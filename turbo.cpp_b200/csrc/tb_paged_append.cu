@@ -36,7 +36,7 @@ tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_d
   const int64_t str[3] = {c->page_stride, c->token_stride, c->head_stride};
   for (int i = 0; i < 3; ++i) {
     if (ext[i] <= 1) continue;  // the stride of a single element is never used
-    if (str[i] < c->head_dim || str[i] > (int64_t(1) << 40) || str[i] * size % 16 != 0)
+    if (str[i] < c->head_dim || str[i] >= (int64_t(1) << 37) || str[i] * size % 16 != 0)
       return fail(TB_EINVAL, "%s: cache strides must cover head_dim and be multiples of 16 bytes", who);
   }
   if (c->n_pages > 0 && (!c->k || !c->v)) return fail(TB_EINVAL, "%s: null pool", who);
@@ -60,6 +60,42 @@ tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_d
   seqs->table_stride = b->table_stride;
   seqs->batch = (int)b->batch;
   seqs->max_len = (int)(b->max_pages * c->page_size);
+  return TB_OK;
+}
+
+tb_status paged_maps(const tb_paged_cache *c, int rows, const char *who, PagedMaps *maps, int *box_rows) {
+  typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {  // the driver's host-side encoder, looked up once per process
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!encode) return fail(TB_ECUDA, "%s: the driver has no cuTensorMapEncodeTiled", who);
+  const int size = dtype_size(c->dtype);
+  const CUtensorMapDataType dt = c->dtype == TB_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : c->dtype == TB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  *box_rows = c->page_size < rows ? c->page_size : rows;
+  const uint64_t row = (uint64_t)(c->head_dim * size);
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->kv_heads, (cuuint64_t)c->page_size,
+                              (cuuint64_t)c->n_pages};
+  // the stride of a single element is never used, but has to be a legal one
+  const cuuint64_t strides[3] = {c->kv_heads > 1 ? (cuuint64_t)(c->head_stride * size) : row,
+                                 c->page_size > 1 ? (cuuint64_t)(c->token_stride * size) : row,
+                                 c->n_pages > 1 ? (cuuint64_t)(c->page_stride * size) : row};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, (cuuint32_t)*box_rows, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 2; ++i) {
+    const CUresult r = encode(i ? &maps->v : &maps->k, dt, 4, i ? c->v : c->k, dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TB_ECUDA, "%s: cuTensorMapEncodeTiled: error %d", who, (int)r);
+  }
   return TB_OK;
 }
 

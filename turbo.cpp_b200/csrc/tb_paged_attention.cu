@@ -25,10 +25,10 @@
 // queries are exact in one part.  Products are summed inside the tensor core
 // over 16 keys and then added to fp32 registers.
 //
-// Layout.  A CTA of eight warps holds a tile of T keys and values in shared
-// memory (three tiles in flight by cp.async, 16-byte words swizzled by row so
-// that every 16-byte fragment load is free of bank conflicts).  HW warps take
-// eight query heads each, KW = 8 / HW take T / KW keys each; each warp keeps
+// Layout.  A ninth warp brings tiles of T keys and values into three stages of
+// shared memory by TMA, one box per page, 128 bytes of each row, swizzled so
+// that every 16-byte fragment load is free of bank conflicts.  Of the eight
+// other warps HW take eight query heads each, KW = 8 / HW take T / KW keys each; each warp keeps
 // its own (m, l, acc), joined once per item.  The order of head_dim inside the
 // dot product is chosen so that each thread's fragments are whole 16-byte words
 // of a key; 16-bit values are read transposed by ldmatrix.
@@ -49,8 +49,9 @@ namespace {
 
 constexpr int kMaxCtas = 320;                    // of a decode launch (counters and partial slots)
 constexpr int64_t kPrefixRows = 2 * 148 * 128;   // extra (row, split) pairs of prefix partials
-constexpr int kThreads = 256;
-constexpr int kWarps = 8;
+constexpr int kWarps = 8;             // computing warps
+constexpr int kThreads = kWarps * 32;  // their threads
+constexpr int kBlock = kThreads + 32;  // and one warp that loads
 constexpr int kStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -69,6 +70,7 @@ struct AttnArgs {
   PrefixParts prefix;
   const int32_t *prefix_table;  // prefix kernel
   int prefix_len;
+  int box_shift;  // a TMA box holds 1 << box_shift tokens
 };
 
 // x = hi + lo: hi the leading 11 bits (cut off, so that it neither overflows nor
@@ -104,6 +106,21 @@ __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same with nothing to add to.
+template <int CT>
+__device__ __forceinline__ void mma_16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (CT == TB_F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -111,6 +128,10 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+__device__ __forceinline__ void sts128_zero(uint32_t addr) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
 }
 
 // Four 8 x 8 blocks of 16-bit elements, transposed; lane i names row i % 8 of block i / 8.
@@ -140,6 +161,14 @@ __device__ __forceinline__ uint32_t pack_rest(float &x, float &y) {
   return u;
 }
 
+// What a CTA keeps in shared memory behind the stages and the merge buffer.
+struct Control {
+  uint64_t full[kStages], empty[kStages];
+  int64_t warp_sum[kWarps + 1];
+  int first[5];
+  int last;
+};
+
 // CT: cache type, D: head_dim, HW: warps across query heads, A32: fp32 activations.
 template <int CT_, int D, int HW, bool A32>
 struct Cfg {
@@ -158,7 +187,7 @@ struct Cfg {
   static constexpr int R = 8 * HW;                // rows (query heads) per item
   static constexpr int STAGE = 2 * T * RB;
   static constexpr int MERGE = kWarps * 8 * (D + 2) * 4;
-  static constexpr int SMEM = kStages * STAGE + MERGE;
+  static constexpr int SMEM = kStages * STAGE + MERGE + (int)sizeof(Control);
   static constexpr int JD = D / 4 / EPC;  // 16-byte words of a key per thread
   static constexpr int JV = D / 8 / EPC;  // 16-byte words of a value per thread and key
 };
@@ -173,31 +202,46 @@ struct WarpState {
   float m, l;
 };
 
-// Copies tile `tile` of a sequence's keys and values into a stage; rows at and
-// behind len (and rows of a page outside the pool) become zeros.
+__device__ __forceinline__ void computing_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+// Waits for a barrier's phase; once a wait has run out (bit 0 of the error
+// word is set then), later ones return at once, so that the kernel ends.
+__device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead) {
+  if (!dead && !mbar_wait_bounded(bar, phase, err)) dead = true;
+}
+
+// The loading warp: tile `tile` of a sequence's keys and values into a stage.
+// Boxes that begin at or behind len are left out; a page id outside the pool
+// is given to TMA as page -1, whose rows are zeros.
 template <class C>
-__device__ __forceinline__ void load_tile(uint32_t stage, const PagedPools &p, const int32_t *table, int len, int tile,
+__device__ __forceinline__ void load_tile(uint32_t stage, uint64_t *full, const CUtensorMap *km, const CUtensorMap *vm,
+                                          const PagedPools &p, int box_shift, const int32_t *table, int len, int tile,
                                           int kvh, uint32_t *err) {
-  constexpr int RPP = kThreads / C::CPR;  // rows per pass
-  const int c = threadIdx.x % C::CPR, r0 = threadIdx.x / C::CPR;
-#pragma unroll
-  for (int i = 0; i < C::T / RPP; ++i) {
-    const int r = r0 + i * RPP, t = tile * C::T + r;
-    int bytes = 0;
-    int64_t off = 0;
-    if (t < len) {
-      const int64_t row = row_offset(p, __ldg(table + (t >> p.shift)), t, kvh);
-      if (row >= 0) {
-        bytes = 16;
-        off = row + c * 16;
-      } else if (c == 0) {
-        atomicOr(err, ERR_INDEX);
-      }
+  const int lane = threadIdx.x & 31, box = 1 << box_shift;
+  const int boxes = (min(max(len - tile * C::T, 0), C::T) + box - 1) >> box_shift;
+  if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)((boxes << box_shift) * 2 * C::RB));
+  __syncwarp();
+  for (int i = lane; i < boxes; i += 32) {
+    const int t = tile * C::T + (i << box_shift);
+    int page = __ldg(table + (t >> p.shift));
+    if ((uint32_t)page >= p.n_pages) {
+      atomicOr(err, ERR_INDEX);
+      page = -1;
     }
-    const uint32_t dst = stage + r * C::RB + ((c ^ (r & 7)) << 4);
-    cp_async16(dst, p.k + off, bytes);
-    cp_async16(dst + C::T * C::RB, p.v + off, bytes);
+    const uint32_t dst = stage + (i << (box_shift + 7));
+#pragma unroll
+    for (int c = 0; c < C::RB / 128; ++c) {
+      const int x = c * (128 / Word<C::CT>::size);
+      tma_box(dst + c * C::T * 128, km, x, kvh, t & p.mask, page, full);
+      tma_box(dst + C::T * C::RB + c * C::T * 128, vm, x, kvh, t & p.mask, page, full);
+    }
   }
+}
+
+// Address of 16-byte word w of row `row` of a tile of keys or values.
+template <class C>
+__device__ __forceinline__ uint32_t word_at(uint32_t tile, int row, int w) {
+  return tile + (w >> 3) * (C::T * 128) + row * 128 + (((w ^ row) & 7) << 4);
 }
 
 // The queries of this warp's eight rows in parts.  row_at(r) gives the element
@@ -280,8 +324,17 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
   constexpr int CT = C::CT;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   constexpr int STEP = 8 * C::NT;
-  const int k0 = kw * C::KPW;
-  for (int k = k0; k < min(n, k0 + C::KPW); k += STEP) {
+  const int k0 = kw * C::KPW, k1 = min(n, k0 + C::KPW);
+  if (n < C::T && k1 > k0 && (k1 - k0) % STEP != 0) {
+    // The rows of the last step behind the sequence's end hold whatever their page held: 0 times that has to be 0.
+    // (Warps of other heads that share these keys write the same zeros before their own reads.)
+    const int rows = STEP - (k1 - k0) % STEP;
+    for (int i = lane; i < rows * C::CPR; i += 32)
+      sts128_zero(word_at<C>(stage + C::T * C::RB, k1 + i / C::CPR, i % C::CPR));
+    fence_proxy_async_smem();  // before TMA writes this stage again
+    __syncwarp();
+  }
+  for (int k = k0; k < k1; k += STEP) {
     // scores: thread holds keys k + 8 b + 2 t, + 1 of row g (c0, c1: first part of q; c2, c3: second)
     float c[C::NT][4];
 #pragma unroll
@@ -295,7 +348,7 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
 #pragma unroll
       for (int b = 0; b < C::NT; ++b) {
         const int row = k + 8 * b + g;
-        u[b] = lds128(stage + row * C::RB + ((w ^ (row & 7)) << 4));
+        u[b] = lds128(word_at<C>(stage, row, w));
       }
       if constexpr (CT == TB_F32) {
 #pragma unroll
@@ -371,7 +424,7 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int row = k + 8 * b + 2 * t + i;
-            Word<TB_F32>::get(lds128(vt + row * C::RB + (((g + 8 * j) ^ (row & 7)) << 4)), f[b][i]);
+            Word<TB_F32>::get(lds128(word_at<C>(vt, row, g + 8 * j)), f[b][i]);
           }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -403,12 +456,12 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
         const int w = 2 * j + (lane >> 4);
-        const uint4 v = ldmatrix_t(vt + row * C::RB + ((w ^ (row & 7)) << 4));
+        const uint4 v = ldmatrix_t(word_at<C>(vt, row, w));
         float o[2][4];
+        mma_16_first<CT>(o[0], pa[0], v.x, v.y);
+        mma_16_first<CT>(o[1], pa[0], v.z, v.w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[0][i] = o[1][i] = 0.f;
-#pragma unroll
-        for (int q = 0; q < C::QT; ++q) {
+        for (int q = 1; q < C::QT; ++q) {
           mma_16<CT>(o[0], pa[q], v.x, v.y);
           mma_16<CT>(o[1], pa[q], v.z, v.w);
         }
@@ -511,21 +564,26 @@ __device__ __forceinline__ void walk_on(Walk &w, const PagedSeqs &s, int items) 
 }
 
 template <int CT, int D, int HW, bool A32>
-__global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1024 ? 2 : 1) paged_decode_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
+__global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 1024 ? 2 : 1)
+    paged_decode_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
+                        uint32_t *__restrict__ err) {
   using C = Cfg<CT, D, HW, A32>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t warp_sum[kWarps];
-  __shared__ Walk first;
-  __shared__ int64_t total_s;
-  __shared__ int last_s;
+  extern __shared__ __align__(1024) unsigned char smem[];
   float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
+  Control &ctl = *reinterpret_cast<Control *>(smem + kStages * C::STAGE + C::MERGE);
   const uint32_t stages = smem_addr(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hw = warp % HW, kw = warp / HW;
   const int items = a.kv_heads * a.head_groups;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&ctl.full[i], 1);
+      mbar_init(&ctl.empty[i], kWarps);
+    }
+    fence_mbar_init();
+  }
 
   // ---- the units of all sequences, and this CTA's share
-  const int per = (a.seqs.batch + kThreads - 1) / kThreads;
+  const int per = (a.seqs.batch + kBlock - 1) / kBlock;
   const int b0 = min(a.seqs.batch, tid * per), b1 = min(a.seqs.batch, b0 + per);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
@@ -539,50 +597,52 @@ __global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1
     const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) warp_sum[warp] = incl;
+  if (lane == 31) ctl.warp_sum[warp] = incl;
   __syncthreads();
   int64_t before = incl - mine, total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
+  for (int w = 0; w <= kWarps; ++w) {
+    if (w < warp) before += ctl.warp_sum[w];
+    total += ctl.warp_sum[w];
   }
   const int64_t n_ctas = min((int64_t)a.max_ctas, total);
   if (blockIdx.x >= n_ctas) return;
   const int64_t u0 = blockIdx.x * total / n_ctas, u1 = (blockIdx.x + 1) * total / n_ctas;
   if (u0 >= before && u0 < before + mine) {
     int64_t u = u0 - before;
-    int b = b0;
-    Walk w;
-    for (;; ++b) {
-      w.len = seq_len(a.seqs, b);
-      w.tiles = tiles_of<C>(w.len);
-      const int64_t n = (int64_t)w.tiles * items;
-      if (u < n) break;
+    for (int b = b0;; ++b) {
+      const int len = seq_len(a.seqs, b), tiles = tiles_of<C>(len);
+      const int64_t n = (int64_t)tiles * items;
+      if (u < n) {
+        const int i = (int)(u / tiles);
+        ctl.first[0] = b, ctl.first[1] = i, ctl.first[2] = (int)(u - (int64_t)i * tiles);
+        ctl.first[3] = tiles, ctl.first[4] = len;
+        break;
+      }
       u -= n;
     }
-    w.b = b;
-    w.i = (int)(u / w.tiles);
-    w.tile = (int)(u - (int64_t)w.i * w.tiles);
-    first = w;
   }
   __syncthreads();
-  Walk load = first, cur = first;
+  Walk cur = {ctl.first[0], ctl.first[1], ctl.first[2], ctl.first[3], ctl.first[4]};
+  bool dead = false;
 
-  // ---- the pipeline: tiles ahead of the one in use
-  auto issue = [&](int64_t u) {
-    if (u < u1) {
-      load_tile<C>(stages + (uint32_t)((u - u0) % kStages) * C::STAGE, a.pools,
-                   a.seqs.table + (int64_t)load.b * a.seqs.table_stride, load.len, load.tile,
-                   load.i / a.head_groups, err);
-      walk_on<C>(load, a.seqs, items);
+  if (warp == kWarps) {  // ---- the loading warp
+    int stage = 0;
+    uint32_t phase = 1;  // the stages begin empty
+    for (int64_t u = u0; u < u1; ++u) {
+      wait_phase(&ctl.empty[stage], phase, err, dead);
+      load_tile<C>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift,
+                   a.seqs.table + (int64_t)cur.b * a.seqs.table_stride, cur.len, cur.tile, cur.i / a.head_groups, err);
+      walk_on<C>(cur, a.seqs, items);
+      if (++stage == kStages) stage = 0, phase ^= 1;
     }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
+    return;
+  }
 
+  const int hw = warp % HW, kw = warp / HW;
   WarpState<C, D> s;
   int64_t item0 = u0 - cur.tile;  // first unit of the current item
+  int stage = 0;
+  uint32_t phase = 0;
   for (int64_t u = u0; u < u1; ++u) {
     const int kvh = cur.i / a.head_groups, hg = cur.i - kvh * a.head_groups;
     if (u == u0 || cur.tile == 0) {
@@ -593,14 +653,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1
         return gi < a.group ? (int64_t)cur.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
       });
     }
-    cp_async_wait<kStages - 2>();
-    __syncthreads();  // tile u is in shared memory, and tile u - 1 is no longer read
-    issue(u + kStages - 1);
-    warp_tile(s, stages + (uint32_t)((u - u0) % kStages) * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw);
+    wait_phase(&ctl.full[stage], phase, err, dead);
+    warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.empty[stage]);
+    if (++stage == kStages) stage = 0, phase ^= 1;
     if (cur.tile + 1 == cur.tiles || u + 1 == u1) {  // this CTA's part of the item is done
       const int64_t item1 = item0 + cur.tiles;
       leave(s, merge);
-      __syncthreads();
+      computing_warps_sync();
       constexpr int TPR = kThreads / C::R, N = D / TPR;
       const int row = tid / TPR, sub = tid % TPR;
       const int gi = hg * C::R + row;
@@ -616,14 +677,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1
         for (int i = 0; i < N; ++i) __stcg(acc + i * TPR, j.acc[i]);
         if (sub == 0) __stcg(a.slot_ml + slot * C::R + row, make_float2(j.m, j.l));
         __threadfence();
-        __syncthreads();
+        computing_warps_sync();
         if (tid == 0) {
           const int before_me = atomicAdd(a.counters + c0, 1);
-          last_s = before_me == (int)(c1 - c0);
-          if (last_s) a.counters[c0] = 0;  // ready for the next launch
+          ctl.last = before_me == (int)(c1 - c0);
+          if (ctl.last) a.counters[c0] = 0;  // ready for the next launch
         }
-        __syncthreads();
-        finish = last_s != 0;
+        computing_warps_sync();
+        finish = ctl.last != 0;
         if (finish) {
           __threadfence();
           j = Join<N>();
@@ -648,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1
 #pragma unroll
         for (int i = 0; i < N; ++i) store_act1(a.out, at + i * TPR, a.q.dtype, none ? 0.f : __fdiv_rn(j.acc[i], j.l));
       }
-      // the merge buffer is written again only after the next tile's barrier
+      computing_warps_sync();  // the merge buffer has been read
     }
     walk_on<C>(cur, a.seqs, items);
   }
@@ -657,24 +718,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1
 // The prefix: item (split, row tile, key/value head), rows = the queries of all
 // sequences' heads of that key/value head, R of them per CTA.
 template <int CT, int D, int HW, bool A32>
-__global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1024 ? 2 : 1) paged_prefix_kernel(const AttnArgs a, uint32_t *__restrict__ err) {
+__global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 1024 ? 2 : 1)
+    paged_prefix_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
+                        uint32_t *__restrict__ err) {
   using C = Cfg<CT, D, HW, A32>;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
+  Control &ctl = *reinterpret_cast<Control *>(smem + kStages * C::STAGE + C::MERGE);
   const uint32_t stages = smem_addr(smem);
-  const int tid = threadIdx.x, warp = tid >> 5;
-  const int hw = warp % HW, kw = warp / HW;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&ctl.full[i], 1);
+      mbar_init(&ctl.empty[i], kWarps);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
   const int split = blockIdx.x, rt = blockIdx.y, kvh = blockIdx.z;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
   const int t0 = (int)((int64_t)split * tiles / a.prefix.splits);
   const int t1 = (int)((int64_t)(split + 1) * tiles / a.prefix.splits);
-  auto issue = [&](int t) {
-    if (t < t1)
-      load_tile<C>(stages + (uint32_t)((t - t0) % kStages) * C::STAGE, a.pools, a.prefix_table, a.prefix_len, t, kvh, err);
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(t0 + i);
+  bool dead = false;
+  if (warp == kWarps) {
+    int stage = 0;
+    uint32_t phase = 1;
+    for (int t = t0; t < t1; ++t) {
+      wait_phase(&ctl.empty[stage], phase, err, dead);
+      load_tile<C>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift,
+                   a.prefix_table, a.prefix_len, t, kvh, err);
+      if (++stage == kStages) stage = 0, phase ^= 1;
+    }
+    return;
+  }
+  const int hw = warp % HW, kw = warp / HW;
   WarpState<C, D> s;
   reset(s);
   load_q(s, a.q, a.scale2, hw, [&](int r) -> int64_t {
@@ -683,14 +760,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<CT, D, HW, A32>::SMEM <= 113 * 1
     const int b = row / a.group;
     return (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D;
   });
+  int stage = 0;
+  uint32_t phase = 0;
   for (int t = t0; t < t1; ++t) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    issue(t + kStages - 1);
-    warp_tile(s, stages + (uint32_t)((t - t0) % kStages) * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw);
+    wait_phase(&ctl.full[stage], phase, err, dead);
+    warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.empty[stage]);
+    if (++stage == kStages) stage = 0, phase ^= 1;
   }
   leave(s, merge);
-  __syncthreads();
+  computing_warps_sync();
   constexpr int TPR = kThreads / C::R, N = D / TPR;
   const int r = tid / TPR, sub = tid % TPR, row = rt * C::R + r;
   if (row >= a.prefix.rows) return;
@@ -723,23 +803,40 @@ Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   return l;
 }
 
+template <class C>
+tb_status tile_maps(AttnArgs &a, const tb_paged_cache *cache, const char *who, PagedMaps *maps) {
+  int rows;
+  tb_paged_cache c = *cache;
+  if (c.n_pages == 0) c.n_pages = 1, c.k = c.v = a.counters;  // an empty pool: every page id is outside it
+  TB_TRY(paged_maps(&c, C::T, who, maps, &rows));
+  a.box_shift = 0;
+  while ((1 << a.box_shift) < rows) ++a.box_shift;
+  return TB_OK;
+}
+
 template <int CT, int D, int HW, bool A32>
-tb_status launch_decode(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
+tb_status launch_decode(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
+                        const char *who) {
   using C = Cfg<CT, D, HW, A32>;
   auto kern = paged_decode_kernel<CT, D, HW, A32>;
   TB_TRY(ensure_smem_for(kern, C::SMEM));
-  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kThreads, C::SMEM);
+  PagedMaps maps;
+  TB_TRY(tile_maps<C>(a, cache, who, &maps));
+  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kBlock, C::SMEM);
   a.max_ctas = std::min(ctas, kMaxCtas);
-  kern<<<a.max_ctas, kThreads, C::SMEM, s>>>(a, st->err_word);
+  kern<<<a.max_ctas, kBlock, C::SMEM, s>>>(a, maps.k, maps.v, st->err_word);
   return check_launch(who);
 }
 
 template <int CT, int D, int HW, bool A32>
-tb_status launch_prefix(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
+tb_status launch_prefix(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
+                        const char *who) {
   using C = Cfg<CT, D, HW, A32>;
   auto kern = paged_prefix_kernel<CT, D, HW, A32>;
   TB_TRY(ensure_smem_for(kern, C::SMEM));
-  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kThreads, C::SMEM);
+  PagedMaps maps;
+  TB_TRY(tile_maps<C>(a, cache, who, &maps));
+  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kBlock, C::SMEM);
   const int row_tiles = (a.prefix.rows + C::R - 1) / C::R;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
@@ -748,27 +845,28 @@ tb_status launch_prefix(AttnArgs &a, const DeviceState *st, cudaStream_t s, cons
   splits = std::min(splits, 1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads));
   a.prefix.splits = (int)splits;
   if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
-  kern<<<dim3((unsigned)splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kThreads, C::SMEM, s>>>(a, st->err_word);
+  kern<<<dim3((unsigned)splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, C::SMEM, s>>>(a, maps.k, maps.v,
+                                                                                                      st->err_word);
   return check_launch(who);
 }
 
 template <int CT, int D, bool A32>
-tb_status run(AttnArgs &a, const DeviceState *st, cudaStream_t s, const char *who) {
+tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s, const char *who) {
   if (a.prefix_len > 0) {
     switch (head_warps(a.prefix.rows)) {
-      case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, st, s, who))); break;
-      case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, st, s, who))); break;
-      case 4: TB_TRY((launch_prefix<CT, D, 4, A32>(a, st, s, who))); break;
-      default: TB_TRY((launch_prefix<CT, D, 8, A32>(a, st, s, who))); break;
+      case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, cache, st, s, who))); break;
+      case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, cache, st, s, who))); break;
+      case 4: TB_TRY((launch_prefix<CT, D, 4, A32>(a, cache, st, s, who))); break;
+      default: TB_TRY((launch_prefix<CT, D, 8, A32>(a, cache, st, s, who))); break;
     }
   }
   const int hw = head_warps(a.group);
   a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
   switch (hw) {
-    case 1: return launch_decode<CT, D, 1, A32>(a, st, s, who);
-    case 2: return launch_decode<CT, D, 2, A32>(a, st, s, who);
-    case 4: return launch_decode<CT, D, 4, A32>(a, st, s, who);
-    default: return launch_decode<CT, D, 8, A32>(a, st, s, who);
+    case 1: return launch_decode<CT, D, 1, A32>(a, cache, st, s, who);
+    case 2: return launch_decode<CT, D, 2, A32>(a, cache, st, s, who);
+    case 4: return launch_decode<CT, D, 4, A32>(a, cache, st, s, who);
+    default: return launch_decode<CT, D, 8, A32>(a, cache, st, s, who);
   }
 }
 
@@ -810,7 +908,7 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
   a.prefix.rows = (int)(B * a.group);
   a.prefix_table = prefix_table;
   a.prefix_len = (int)prefix_len;
-#define TB_RUN(CT, A32) return D == 64 ? run<CT, 64, A32>(a, st, stream, who) : run<CT, 128, A32>(a, st, stream, who)
+#define TB_RUN(CT, A32) return D == 64 ? run<CT, 64, A32>(a, cache, st, stream, who) : run<CT, 128, A32>(a, cache, st, stream, who)
   if (act_dtype == TB_F16) TB_RUN(TB_F16, false);
   if (act_dtype == TB_BF16) TB_RUN(TB_BF16, false);
   if (cache->dtype == TB_F16) TB_RUN(TB_F16, true);

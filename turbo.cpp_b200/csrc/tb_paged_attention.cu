@@ -164,9 +164,9 @@ __device__ __forceinline__ uint32_t pack_rest(float &x, float &y) {
 // What a CTA keeps in shared memory behind the stages and the merge buffer.
 struct Control {
   uint64_t full[kStages], empty[kStages];
-  int64_t warp_sum[kWarps + 1];
+  int warp_sum[kWarps + 1];
   int first[5];
-  int last;
+  int last[2];
 };
 
 // CT: cache type, D: head_dim, HW: warps across query heads, A32: fp32 activations.
@@ -244,13 +244,12 @@ __device__ __forceinline__ uint32_t word_at(uint32_t tile, int row, int w) {
   return tile + (w >> 3) * (C::T * 128) + row * 128 + (((w ^ row) & 7) << 4);
 }
 
-// The queries of this warp's eight rows in parts.  row_at(r) gives the element
-// offset of row r of the item, or -1 where there is none.
-template <class C, int D, class RowAt>
-__device__ __forceinline__ void load_q(WarpState<C, D> &s, const ActRows &q, float scale2, int hw, RowAt row_at) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t at = row_at(hw * 8 + g);
-  float f[C::JD][C::EPC];
+// The queries of this warp's eight rows: row g at element offset `at` (-1:
+// none), as loaded (fetch_q, so that a next item's arrive during this one's
+// joins) and in parts (load_q).
+template <class C>
+__device__ __forceinline__ void fetch_q(float (&f)[C::JD][C::EPC], const ActRows &q, int64_t at) {
+  const int t = threadIdx.x & 3;
 #pragma unroll
   for (int j = 0; j < C::JD; ++j) {
     const int c = 8 * (j >> 1) + 2 * t + (j & 1);
@@ -258,6 +257,10 @@ __device__ __forceinline__ void load_q(WarpState<C, D> &s, const ActRows &q, flo
     for (int e = 0; e < C::EPC; ++e) f[j][e] = 0.f;
     if (at >= 0) load_act<C::EPC>(q.p, at + c * C::EPC, C::QR == 4 ? TB_F32 : C::CT, f[j]);
   }
+}
+
+template <class C, int D>
+__device__ __forceinline__ void load_q(WarpState<C, D> &s, float (&f)[C::JD][C::EPC], float scale2) {
   s.scale2 = scale2;
   if constexpr (C::CT == TB_F16 && C::QR == 4) {
     float mx = 0.f;
@@ -521,6 +524,28 @@ struct Join {
   }
 };
 
+// Adds `n` partial results in global memory (part p: ml(p), element i acc(p, i))
+// to a join, as many at a time as fit in 16 registers, so that their loads
+// overlap; in order.
+template <int N, class Ml, class Acc>
+__device__ __forceinline__ void join_parts(Join<N> &j, int n, Ml ml, Acc acc) {
+  constexpr int P = N >= 16 ? 1 : 16 / N;
+  for (int p0 = 0; p0 < n; p0 += P) {
+    float2 m[P];
+    float v[P][N];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const bool have = p0 + p < n;
+      m[p] = have ? __ldcg(ml(p0 + p)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[p][i] = have ? __ldcg(acc(p0 + p, i)) : 0.f;
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (p0 + p < n) j.add(m[p], [&](int i) { return v[p][i]; });
+  }
+}
+
 // The warps' results of row `row` of an item, joined; thread `sub` of TPR
 // takes elements sub + TPR i.
 template <class C, int D, int N>
@@ -582,39 +607,47 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     fence_mbar_init();
   }
 
-  // ---- the units of all sequences, and this CTA's share
+  // ---- the units of all sequences, and this CTA's share: with n CTAs, unit r of U goes to r / (U / n) or so, the
+  // first U % n CTAs taking one more (the host has made sure that U < 2^31)
   const int per = (a.seqs.batch + kBlock - 1) / kBlock;
   const int b0 = min(a.seqs.batch, tid * per), b1 = min(a.seqs.batch, b0 + per);
-  int64_t mine = 0;
+  int mine = 0;
   for (int b = b0; b < b1; ++b) {
     const int len = __ldg(a.seqs.lens + b);
     if (blockIdx.x == 0 && (len < 0 || len > a.seqs.max_len)) atomicOr(err, ERR_INDEX);
-    mine += (int64_t)tiles_of<C>(seq_len(a.seqs, b)) * items;
+    mine += tiles_of<C>(seq_len(a.seqs, b)) * items;
   }
-  int64_t incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) ctl.warp_sum[warp] = incl;
   __syncthreads();
-  int64_t before = incl - mine, total = 0;
+  int before = incl - mine, total = 0;
+#pragma unroll
   for (int w = 0; w <= kWarps; ++w) {
     if (w < warp) before += ctl.warp_sum[w];
     total += ctl.warp_sum[w];
   }
-  const int64_t n_ctas = min((int64_t)a.max_ctas, total);
-  if (blockIdx.x >= n_ctas) return;
-  const int64_t u0 = blockIdx.x * total / n_ctas, u1 = (blockIdx.x + 1) * total / n_ctas;
+  const int n_ctas = min(a.max_ctas, total), me = blockIdx.x;
+  if (me >= n_ctas) return;
+  const int share = total / n_ctas, more = total - share * n_ctas;
+  auto first_unit = [&](int c) { return c * share + min(c, more); };
+  auto owner = [&](int u) {
+    const int x = u - more * (share + 1);
+    return x < 0 ? u / (share + 1) : more + x / share;
+  };
+  const int u0 = first_unit(me), u1 = first_unit(me + 1);
   if (u0 >= before && u0 < before + mine) {
-    int64_t u = u0 - before;
+    int u = u0 - before;
     for (int b = b0;; ++b) {
       const int len = seq_len(a.seqs, b), tiles = tiles_of<C>(len);
-      const int64_t n = (int64_t)tiles * items;
+      const int n = tiles * items;
       if (u < n) {
-        const int i = (int)(u / tiles);
-        ctl.first[0] = b, ctl.first[1] = i, ctl.first[2] = (int)(u - (int64_t)i * tiles);
+        const int i = u / tiles;
+        ctl.first[0] = b, ctl.first[1] = i, ctl.first[2] = u - i * tiles;
         ctl.first[3] = tiles, ctl.first[4] = len;
         break;
       }
@@ -628,7 +661,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
   if (warp == kWarps) {  // ---- the loading warp
     int stage = 0;
     uint32_t phase = 1;  // the stages begin empty
-    for (int64_t u = u0; u < u1; ++u) {
+    for (int u = u0; u < u1; ++u) {
       wait_phase(&ctl.empty[stage], phase, err, dead);
       load_tile<C>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift,
                    a.seqs.table + (int64_t)cur.b * a.seqs.table_stride, cur.len, cur.tile, cur.i / a.head_groups, err);
@@ -638,80 +671,95 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     return;
   }
 
+  // ---- the computing warps
   const int hw = warp % HW, kw = warp / HW;
+  constexpr int TPR = kThreads / C::R, N = D / TPR;
+  const int row = tid / TPR, sub = tid % TPR;  // this thread's share of a join
+  auto q_at = [&](const Walk &w) -> int64_t {
+    const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + hw * 8 + (lane >> 2);
+    return gi < a.group ? (int64_t)w.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
+  };
+  // the output of item `w`: the join of its parts, behind those of the prefix
+  auto finish = [&](const Walk &w, Join<N> &j) {
+    const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + row;
+    if (gi >= a.group) return;
+    if (a.prefix.splits > 0) {
+      const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)w.b * a.group + gi) * a.prefix.splits;
+      join_parts(j, a.prefix.splits, [&](int p) { return a.prefix.ml + at + p; },
+                 [&](int p, int i) { return a.prefix.acc + (at + p) * D + sub + i * TPR; });
+    }
+    const bool none = w.len == 0 && a.prefix.splits == 0;
+    const int64_t at = (int64_t)w.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + sub;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      store_act1(a.out, at + i * TPR, A32 ? TB_F32 : CT, none ? 0.f : __fdiv_rn(j.acc[i], j.l));
+  };
   WarpState<C, D> s;
-  int64_t item0 = u0 - cur.tile;  // first unit of the current item
+  float qf[C::JD][C::EPC];
+  fetch_q<C>(qf, a.q, q_at(cur));
   int stage = 0;
   uint32_t phase = 0;
-  for (int64_t u = u0; u < u1; ++u) {
-    const int kvh = cur.i / a.head_groups, hg = cur.i - kvh * a.head_groups;
-    if (u == u0 || cur.tile == 0) {
-      item0 = u - cur.tile;
-      reset(s);
-      load_q(s, a.q, a.scale2, hw, [&](int r) -> int64_t {
-        const int gi = hg * C::R + r;
-        return gi < a.group ? (int64_t)cur.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
-      });
+  // the items that this CTA shares with others: its first, begun before u0, and its last, unfinished at u1
+  Walk cut[2];
+  int cut_unit[2] = {-1, -1};  // the item's first unit
+  for (int u = u0; u < u1;) {
+    const Walk item = cur;
+    const int item0 = u - cur.tile, end = min(u1, item0 + cur.tiles);
+    reset(s);
+    load_q(s, qf, a.scale2);
+    for (; u < end; ++u) {
+      wait_phase(&ctl.full[stage], phase, err, dead);
+      warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.empty[stage]);
+      if (++stage == kStages) stage = 0, phase ^= 1;
+      walk_on<C>(cur, a.seqs, items);
     }
-    wait_phase(&ctl.full[stage], phase, err, dead);
-    warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.empty[stage]);
-    if (++stage == kStages) stage = 0, phase ^= 1;
-    if (cur.tile + 1 == cur.tiles || u + 1 == u1) {  // this CTA's part of the item is done
-      const int64_t item1 = item0 + cur.tiles;
-      leave(s, merge);
-      computing_warps_sync();
-      constexpr int TPR = kThreads / C::R, N = D / TPR;
-      const int row = tid / TPR, sub = tid % TPR;
-      const int gi = hg * C::R + row;
-      Join<N> j;
-      join_warps<C, D>(j, merge, row, sub);
-      // the CTAs that share the item: owners of its first and last unit
-      const int64_t c0 = ((item0 + 1) * n_ctas - 1) / total, c1 = (item1 * n_ctas - 1) / total;
-      bool finish = true;
-      if (c0 != c1) {
-        const int64_t slot = 2 * blockIdx.x + (u0 >= item0 ? 0 : 1);
-        float *acc = a.slot_acc + (slot * C::R + row) * D + sub;
+    if (u < u1) fetch_q<C>(qf, a.q, q_at(cur));
+    leave(s, merge);
+    computing_warps_sync();
+    Join<N> j;
+    join_warps<C, D>(j, merge, row, sub);
+    if (item0 >= u0 && item0 + item.tiles <= u1) {
+      finish(item, j);
+    } else {
+      const int k = item0 < u0 ? 0 : 1;
+      const int64_t slot = 2 * me + k;
+      float *acc = a.slot_acc + (slot * C::R + row) * D + sub;
 #pragma unroll
-        for (int i = 0; i < N; ++i) __stcg(acc + i * TPR, j.acc[i]);
-        if (sub == 0) __stcg(a.slot_ml + slot * C::R + row, make_float2(j.m, j.l));
-        __threadfence();
-        computing_warps_sync();
-        if (tid == 0) {
-          const int before_me = atomicAdd(a.counters + c0, 1);
-          ctl.last = before_me == (int)(c1 - c0);
-          if (ctl.last) a.counters[c0] = 0;  // ready for the next launch
-        }
-        computing_warps_sync();
-        finish = ctl.last != 0;
-        if (finish) {
-          __threadfence();
-          j = Join<N>();
-          for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t cs = 2 * c + (c * total / n_ctas >= item0 ? 0 : 1);
-            const float *pa = a.slot_acc + (cs * C::R + row) * D + sub;
-            j.add(__ldcg(a.slot_ml + cs * C::R + row), [&](int i) { return __ldcg(pa + i * TPR); });
-          }
-        }
-      }
-      if (finish && gi < a.group) {
-        bool none = cur.len == 0;
-        if (a.prefix.splits > 0) {
-          none = false;
-          const int64_t pr = (int64_t)kvh * a.prefix.rows + (int64_t)cur.b * a.group + gi;
-          for (int p = 0; p < a.prefix.splits; ++p) {
-            const float *pa = a.prefix.acc + (pr * a.prefix.splits + p) * D + sub;
-            j.add(__ldcg(a.prefix.ml + pr * a.prefix.splits + p), [&](int i) { return __ldcg(pa + i * TPR); });
-          }
-        }
-        const int64_t at = (int64_t)cur.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + sub;
-#pragma unroll
-        for (int i = 0; i < N; ++i) store_act1(a.out, at + i * TPR, a.q.dtype, none ? 0.f : __fdiv_rn(j.acc[i], j.l));
-      }
-      computing_warps_sync();  // the merge buffer has been read
+      for (int i = 0; i < N; ++i) __stcg(acc + i * TPR, j.acc[i]);
+      if (sub == 0) __stcg(a.slot_ml + slot * C::R + row, make_float2(j.m, j.l));
+      cut[k] = item;
+      cut_unit[k] = item0;
     }
-    walk_on<C>(cur, a.seqs, items);
+    computing_warps_sync();  // the merge buffer has been read
+  }
+
+  // ---- the cut items: whoever of its CTAs comes last joins one
+  if (cut_unit[0] < 0 && cut_unit[1] < 0) return;
+  if (tid == 0) {
+    __threadfence();  // the whole CTA's partial results, seen by this thread at the barrier above
+    for (int k = 0; k < 2; ++k) {
+      ctl.last[k] = 0;
+      if (cut_unit[k] < 0) continue;
+      const int c0 = owner(cut_unit[k]), c1 = owner(cut_unit[k] + cut[k].tiles - 1);
+      if (atomicAdd(a.counters + c0, 1) == c1 - c0) {
+        ctl.last[k] = 1;
+        a.counters[c0] = 0;  // ready for the next launch
+      }
+    }
+    __threadfence();
+  }
+  computing_warps_sync();
+  for (int k = 0; k < 2; ++k) {
+    if (cut_unit[k] < 0 || !ctl.last[k]) continue;
+    const int c0 = owner(cut_unit[k]), c1 = owner(cut_unit[k] + cut[k].tiles - 1);
+    Join<N> j;
+    // CTA c's slot: its first item's where the item began before it
+    auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (cut_unit[k] < first_unit(c0 + p) ? 0 : 1)) * C::R + row; };
+    join_parts(j, c1 - c0 + 1, [&](int p) { return a.slot_ml + slot(p); },
+               [&](int p, int i) { return a.slot_acc + slot(p) * D + sub + i * TPR; });
+    finish(cut[k], j);
   }
 }
 
@@ -754,12 +802,13 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
   const int hw = warp % HW, kw = warp / HW;
   WarpState<C, D> s;
   reset(s);
-  load_q(s, a.q, a.scale2, hw, [&](int r) -> int64_t {
-    const int row = rt * C::R + r;
-    if (row >= a.prefix.rows) return -1;
-    const int b = row / a.group;
-    return (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D;
-  });
+  {
+    const int row = rt * C::R + hw * 8 + (lane >> 2), b = row / a.group;
+    float f[C::JD][C::EPC];
+    fetch_q<C>(f, a.q,
+               row < a.prefix.rows ? (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D : -1);
+    load_q(s, f, a.scale2);
+  }
   int stage = 0;
   uint32_t phase = 0;
   for (int t = t0; t < t1; ++t) {
@@ -881,6 +930,8 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
     return fail(TB_EINVAL, "%s: heads must be a positive multiple of kv_heads", who);
   if (B * heads > (1 << 24)) return fail(TB_EINVAL, "%s: more than 2^24 query rows", who);
   if (prefix_len < 0 || prefix_len > 0x7FFFFFFF - 65536) return fail(TB_EINVAL, "%s: bad prefix length", who);
+  if (B * heads * (a.seqs.max_len / 64 + 1) > 0x7FFFFFFF)  // units of work at most
+    return fail(TB_EINVAL, "%s: batch * heads * max_pages * page_size is too large (2^37)", who);
   if (B == 0) return TB_OK;
   if (!q || !out || !ws || (prefix_len > 0 && !prefix_table)) return fail(TB_EINVAL, "%s: null pointer", who);
   const int as = dtype_size(act_dtype);

@@ -9,10 +9,11 @@
 //
 // It moves every element once and computes next to nothing, so bytes bound it.
 // A thread takes eight elements of a head's first half and the eight they are
-// paired with (16- or 32-byte loads and stores); a warp takes 32 such pairs of
-// one token, so that the token's sequence, position and page are found once per
-// warp: a 32-way search of `starts` by ballot, then one table entry.  The data
-// loads do not depend on that chain and are issued before it.
+// paired with (16- or 32-byte loads and stores) for one to four heads of one
+// token, so that its cosines and sines are read once, and the token's sequence,
+// position and page are found once per warp: a 32-way search of `starts` by
+// ballot, then one table entry.  The data loads do not depend on that chain and
+// are issued before it.
 #include <algorithm>
 
 #include "tb_paged.cuh"
@@ -93,7 +94,7 @@ tb_status paged_maps(const tb_paged_cache *c, int rows, const char *who, PagedMa
   for (int i = 0; i < 2; ++i) {
     const CUresult r = encode(i ? &maps->v : &maps->k, dt, 4, i ? c->v : c->k, dims, strides, box, step,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(TB_ECUDA, "%s: cuTensorMapEncodeTiled: error %d", who, (int)r);
   }
   return TB_OK;
@@ -127,26 +128,47 @@ __device__ __forceinline__ void put8(void *p, const float (&f)[8]) {
   }
 }
 
-// ACT, CT: types of the activations and of the cache.
-template <int ACT, int CT>
+template <int ACT>
+__device__ __forceinline__ void words(const uint4 *w, float (&f)[8]) {
+  if constexpr (ACT == TB_F32) {
+    float lo[4], hi[4];
+    Word<TB_F32>::get(w[0], lo);
+    Word<TB_F32>::get(w[1], hi);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
+  } else {
+    Word<ACT>::get(w[0], f);
+  }
+}
+
+// ACT, CT: types of the activations and of the cache; U: groups of heads per
+// warp, of one token.
+template <int ACT, int CT, int U>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, uint32_t *__restrict__ err) {
   constexpr int AS = Word<ACT>::size, CS = Word<CT>::size;
+  constexpr int W = AS == 4 ? 2 : 1;  // 16-byte words of eight activations
   const int lane = threadIdx.x & 31;
   const int64_t warps = a.tokens * a.per_token;
   const int half = a.dim / 2;
+  // a group is 32 / per_head heads; this thread has the same elements of each
+  const int span = 32 / a.per_head, sub = lane / a.per_head, i = (lane - sub * a.per_head) * 8;
+  const int all = sub < span ? a.heads + 2 * a.kv_heads : 0;
   for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
     const int64_t t = w / a.per_token;
-    const int u = (int)(w - t * a.per_token) * 32 + lane;
-    const int head = u / a.per_head, i = (u - head * a.per_head) * 8;
-    // 0: query, 1: key, 2: value, 3: none
-    const int kind = head < a.heads ? 0 : head < a.heads + a.kv_heads ? 1 : head < a.heads + 2 * a.kv_heads ? 2 : 3;
-    const int h = kind == 0 ? head : kind == 1 ? head - a.heads : head - a.heads - a.kv_heads;
-    const ActRows &src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    float x0[8], x1[8];
-    if (kind < 3) {
-      const int64_t at = t * src.ld + (int64_t)h * a.dim + i;
-      load_act<8>(src.p, at, ACT, x0);
-      load_act<8>(src.p, at + half, ACT, x1);
+    const int head0 = (int)(w - t * a.per_token) * span * U + sub;
+    uint4 r0[U][W], r1[U][W];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int head = head0 + k * span;
+      if (head >= all) continue;
+      const ActRows &src = head < a.heads ? a.q : head < a.heads + a.kv_heads ? a.k : a.v;
+      const int h = head < a.heads ? head : head < a.heads + a.kv_heads ? head - a.heads : head - a.heads - a.kv_heads;
+      const char *at = static_cast<const char *>(src.p) + (t * src.ld + (int64_t)h * a.dim + i) * AS;
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        r0[k][e] = reinterpret_cast<const uint4 *>(at)[e];
+        r1[k][e] = reinterpret_cast<const uint4 *>(at + half * AS)[e];
+      }
     }
     // the token's sequence: the last b with starts[b] <= t
     int b = (int)t, pos;
@@ -176,33 +198,44 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
     int64_t row = -1;
     if (ok) {
       const int32_t id = __ldg(a.seqs.table + (int64_t)b * a.seqs.table_stride + (pos >> a.pools.shift));
-      row = row_offset(a.pools, id, pos, kind == 1 || kind == 2 ? h : 0);
+      row = row_offset(a.pools, id, pos, 0);
       ok = row >= 0;
     }
     if (!ok) {
       if (lane == 0) atomicOr(err, ERR_INDEX);
       continue;
     }
-    if (kind == 3) continue;
-    if (kind < 2 && a.cos_t) {
-      float c[8], s[8];
+    float c[8], sn[8];
+    if (a.cos_t && head0 < a.heads + a.kv_heads) {
       load_act<8>(a.cos_t, (int64_t)pos * half + i, TB_F32, c);
-      load_act<8>(a.sin_t, (int64_t)pos * half + i, TB_F32, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y0 = __fmaf_rn(x0[e], c[e], -__fmul_rn(x1[e], s[e]));
-        x1[e] = __fmaf_rn(x0[e], s[e], __fmul_rn(x1[e], c[e]));
-        x0[e] = y0;
-      }
+      load_act<8>(a.sin_t, (int64_t)pos * half + i, TB_F32, sn);
     }
-    if (kind == 0) {
-      char *d = static_cast<char *>(a.q_out) + (t * a.ldq_out + (int64_t)h * a.dim + i) * AS;
-      put8<ACT>(d, x0);
-      put8<ACT>(d + half * AS, x1);
-    } else {
-      char *d = const_cast<char *>(kind == 1 ? a.pools.k : a.pools.v) + row + i * CS;
-      put8<CT>(d, x0);
-      put8<CT>(d + half * CS, x1);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int head = head0 + k * span;
+      if (head >= all) continue;
+      float x0[8], x1[8];
+      words<ACT>(r0[k], x0);
+      words<ACT>(r1[k], x1);
+      if (a.cos_t && head < a.heads + a.kv_heads) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y0 = __fmaf_rn(x0[e], c[e], -__fmul_rn(x1[e], sn[e]));
+          x1[e] = __fmaf_rn(x0[e], sn[e], __fmul_rn(x1[e], c[e]));
+          x0[e] = y0;
+        }
+      }
+      if (head < a.heads) {
+        char *d = static_cast<char *>(a.q_out) + (t * a.ldq_out + (int64_t)head * a.dim + i) * AS;
+        put8<ACT>(d, x0);
+        put8<ACT>(d + half * AS, x1);
+      } else {
+        const bool key = head < a.heads + a.kv_heads;
+        const int h = head - a.heads - (key ? 0 : a.kv_heads);
+        char *d = const_cast<char *>(key ? a.pools.k : a.pools.v) + row + h * a.pools.head_stride + i * CS;
+        put8<CT>(d, x0);
+        put8<CT>(d + half * CS, x1);
+      }
     }
   }
 }
@@ -252,18 +285,27 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
   a.kv_heads = (int)KVH;
   a.dim = (int)D;
   a.per_head = (int)(D / 16);
-  a.per_token = (int)(((heads + 2 * KVH) * a.per_head + 31) / 32);
   a.starts = starts_dev;
   a.cos_t = cos_dev;
   a.sin_t = sin_dev;
   a.rope_max_seq = (int)rope_max_seq;
-  const int64_t threads = tokens * a.per_token * 32;
+  // Several groups per warp once that still fills the GPU: a token's lookups are shared and more loads are in flight.
+  const int span = 32 / a.per_head;
+  const int64_t groups = (heads + 2 * KVH + span - 1) / span;
+  const bool wide = tokens * groups >= (int64_t)st->sm_count * 64;
   cudaStream_t s = as_stream(stream);
-#define TB_APPEND(ACT, CT)                                                             \
+#define TB_APPEND_U(ACT, CT, U)                                                        \
   do {                                                                                 \
-    auto kern = paged_append_kernel<ACT, CT>;                                          \
+    auto kern = paged_append_kernel<ACT, CT, U>;                                       \
+    a.per_token = (int)((groups + U - 1) / U);                                         \
+    const int64_t threads = tokens * a.per_token * 32;                                 \
     kern<<<wave_grid(kern, 256, threads, st->sm_count), 256, 0, s>>>(a, st->err_word); \
     return check_launch("tb_rope_paged_append");                                       \
+  } while (0)
+#define TB_APPEND(ACT, CT)               \
+  do {                                   \
+    if (wide) TB_APPEND_U(ACT, CT, (ACT == TB_F32 ? 2 : 4)); \
+    TB_APPEND_U(ACT, CT, 1);             \
   } while (0)
   if (act_dtype == TB_F16) TB_APPEND(TB_F16, TB_F16);
   if (act_dtype == TB_BF16) TB_APPEND(TB_BF16, TB_BF16);
@@ -271,4 +313,5 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
   if (cache->dtype == TB_BF16) TB_APPEND(TB_F32, TB_BF16);
   TB_APPEND(TB_F32, TB_F32);
 #undef TB_APPEND
+#undef TB_APPEND_U
 }

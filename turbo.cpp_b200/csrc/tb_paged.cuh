@@ -69,6 +69,70 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, in
       : "memory");
 }
 
+// Waits for a barrier's phase; once a wait has run out (bit 0 of the error
+// word is set then), later ones return at once, so that the kernel ends.
+__device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead) {
+  if (!dead && !mbar_wait_bounded(bar, phase, err)) dead = true;
+}
+
+// One warp: tile `tile` (T keys or values of row size RB) of a sequence of len
+// tokens into shared memory, 128-byte columns T * 128 bytes apart.  Boxes that
+// begin at or behind len are left out; a page id outside the pool is given to
+// TMA as page -1, whose rows are zeros.  With two maps both tiles are fetched,
+// the second T * RB bytes behind the first.
+template <int T, int RB, int SIZE>
+__device__ __forceinline__ void load_rows(uint32_t dst0, uint64_t *full, const CUtensorMap *m0, const CUtensorMap *m1,
+                                          const PagedPools &p, int box_shift, const int32_t *table, int len, int tile,
+                                          int kvh, uint32_t *err) {
+  const int lane = threadIdx.x & 31, box = 1 << box_shift;
+  const int boxes = (min(max(len - tile * T, 0), T) + box - 1) >> box_shift;
+  if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)((boxes << box_shift) * (m1 ? 2 : 1) * RB));
+  __syncwarp();
+  for (int i = lane; i < boxes; i += 32) {
+    const int t = tile * T + (i << box_shift);
+    int page = __ldg(table + (t >> p.shift));
+    if ((uint32_t)page >= p.n_pages) {
+      atomicOr(err, ERR_INDEX);
+      page = -1;
+    }
+    const uint32_t dst = dst0 + (i << (box_shift + 7));
+#pragma unroll
+    for (int c = 0; c < RB / 128; ++c) {
+      tma_box(dst + c * T * 128, m0, c * (128 / SIZE), kvh, t & p.mask, page, full);
+      if (m1) tma_box(dst + T * RB + c * T * 128, m1, c * (128 / SIZE), kvh, t & p.mask, page, full);
+    }
+  }
+}
+
+// Two floats as one register of type CT, to nearest, and what is left of them.
+template <int CT>
+__device__ __forceinline__ uint32_t pack_rest(float &x, float &y) {
+  uint32_t u;
+  if constexpr (CT == TB_F16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    u = *reinterpret_cast<const uint32_t *>(&h);
+    const float2 f = __half22float2(h);
+    x -= f.x, y -= f.y;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    u = *reinterpret_cast<const uint32_t *>(&h);
+    x -= __uint_as_float(u << 16), y -= __uint_as_float(u & 0xFFFF0000u);
+  }
+  return u;
+}
+
+// The exponent e of the power of two that brings a maximum into [2^14, 2^15)
+// (0 for 0, inf and NaN), so that fp32 queries fit fp16 parts.
+__device__ __forceinline__ int fp16_exp(float mx) {
+  const int E = (int)(__float_as_uint(mx) >> 23);
+  return mx == 0.f || E == 255 ? 0 : min(max(141 - E, -126), 126);
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+__device__ __forceinline__ void sts128_zero(uint32_t addr) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -157,5 +221,31 @@ __device__ __forceinline__ void store_act1(void *p, int64_t i, int dtype, float 
   else if (dtype == TB_F16) static_cast<__half *>(p)[i] = __float2half_rn(x);
   else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
 }
+
+// What an attention launch is given (tb_paged_attention.cu).
+struct AttnArgs {
+  PagedPools pools;
+  PagedSeqs seqs;
+  ActRows q;
+  void *out;
+  int64_t ldo;
+  int kv_heads, group, head_groups;  // head_groups: items per (sequence, key/value head)
+  float scale2;                      // scale * log2(e)
+  int max_ctas;
+  int *counters;    // [kMaxCtas], zero between launches
+  float *slot_acc;  // [2 kMaxCtas][8 HW][D]
+  float2 *slot_ml;  // [2 kMaxCtas][8 HW]
+  PrefixParts prefix;
+  const int32_t *prefix_table;  // prefix kernels
+  int prefix_len;
+  int box_shift;  // a TMA box holds 1 << box_shift tokens
+};
+
+// Most splits of the prefix whose results the workspace holds.
+int max_prefix_splits(const AttnArgs &a);
+
+// The prefix on tcgen05 (tb_paged_prefix.cu), 16-bit caches; sets a.prefix.splits.
+tb_status launch_prefix_tc(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
+                           const char *who);
 
 }  // namespace tb

@@ -53,25 +53,8 @@ constexpr int kWarps = 8;             // computing warps
 constexpr int kThreads = kWarps * 32;  // their threads
 constexpr int kBlock = kThreads + 32;  // and one warp that loads
 constexpr int kStages = 3;
+constexpr int kTensorRows = 64;       // query rows of a key/value head from which the prefix runs on tcgen05
 constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttnArgs {
-  PagedPools pools;
-  PagedSeqs seqs;
-  ActRows q;
-  void *out;
-  int64_t ldo;
-  int kv_heads, group, head_groups;  // head_groups: items per (sequence, key/value head)
-  float scale2;                      // scale * log2(e)
-  int max_ctas;
-  int *counters;   // [kMaxCtas], zero between launches
-  float *slot_acc; // [2 kMaxCtas][8 HW][D]
-  float2 *slot_ml; // [2 kMaxCtas][8 HW]
-  PrefixParts prefix;
-  const int32_t *prefix_table;  // prefix kernel
-  int prefix_len;
-  int box_shift;  // a TMA box holds 1 << box_shift tokens
-};
 
 // x = hi + lo: hi the leading 11 bits (cut off, so that it neither overflows nor
 // differs from x in sign: an infinite sum keeps its sign), lo the rest to
@@ -130,10 +113,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ void sts128_zero(uint32_t addr) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
-}
-
 // Four 8 x 8 blocks of 16-bit elements, transposed; lane i names row i % 8 of block i / 8.
 __device__ __forceinline__ uint4 ldmatrix_t(uint32_t addr) {
   uint4 v;
@@ -142,23 +121,6 @@ __device__ __forceinline__ uint4 ldmatrix_t(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
-}
-
-// Two floats as one register of type CT, to nearest, and what is left of them.
-template <int CT>
-__device__ __forceinline__ uint32_t pack_rest(float &x, float &y) {
-  uint32_t u;
-  if constexpr (CT == TB_F16) {
-    const __half2 h = __floats2half2_rn(x, y);
-    u = *reinterpret_cast<const uint32_t *>(&h);
-    const float2 f = __half22float2(h);
-    x -= f.x, y -= f.y;
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    u = *reinterpret_cast<const uint32_t *>(&h);
-    x -= __uint_as_float(u << 16), y -= __uint_as_float(u & 0xFFFF0000u);
-  }
-  return u;
 }
 
 // What a CTA keeps in shared memory behind the stages and the merge buffer.
@@ -204,40 +166,6 @@ struct WarpState {
 
 __device__ __forceinline__ void computing_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
-// Waits for a barrier's phase; once a wait has run out (bit 0 of the error
-// word is set then), later ones return at once, so that the kernel ends.
-__device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead) {
-  if (!dead && !mbar_wait_bounded(bar, phase, err)) dead = true;
-}
-
-// The loading warp: tile `tile` of a sequence's keys and values into a stage.
-// Boxes that begin at or behind len are left out; a page id outside the pool
-// is given to TMA as page -1, whose rows are zeros.
-template <class C>
-__device__ __forceinline__ void load_tile(uint32_t stage, uint64_t *full, const CUtensorMap *km, const CUtensorMap *vm,
-                                          const PagedPools &p, int box_shift, const int32_t *table, int len, int tile,
-                                          int kvh, uint32_t *err) {
-  const int lane = threadIdx.x & 31, box = 1 << box_shift;
-  const int boxes = (min(max(len - tile * C::T, 0), C::T) + box - 1) >> box_shift;
-  if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)((boxes << box_shift) * 2 * C::RB));
-  __syncwarp();
-  for (int i = lane; i < boxes; i += 32) {
-    const int t = tile * C::T + (i << box_shift);
-    int page = __ldg(table + (t >> p.shift));
-    if ((uint32_t)page >= p.n_pages) {
-      atomicOr(err, ERR_INDEX);
-      page = -1;
-    }
-    const uint32_t dst = stage + (i << (box_shift + 7));
-#pragma unroll
-    for (int c = 0; c < C::RB / 128; ++c) {
-      const int x = c * (128 / Word<C::CT>::size);
-      tma_box(dst + c * C::T * 128, km, x, kvh, t & p.mask, page, full);
-      tma_box(dst + C::T * C::RB + c * C::T * 128, vm, x, kvh, t & p.mask, page, full);
-    }
-  }
-}
-
 // Address of 16-byte word w of row `row` of a tile of keys or values.
 template <class C>
 __device__ __forceinline__ uint32_t word_at(uint32_t tile, int row, int w) {
@@ -270,11 +198,9 @@ __device__ __forceinline__ void load_q(WarpState<C, D> &s, float (&f)[C::JD][C::
       for (int e = 0; e < C::EPC; ++e) mx = fmaxf(mx, fabsf(f[j][e]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // the power of two that brings the row's maximum into [2^14, 2^15); none for 0, inf, NaN
-    const int E = (int)(__float_as_uint(mx) >> 23);
-    const int e = mx == 0.f || E == 255 ? 0 : min(max(141 - E, -126), 126);
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    s.scale2 = scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
+    const int e = fp16_exp(mx);
+    const float up = pow2i(e);
+    s.scale2 = scale2 * pow2i(-e);
 #pragma unroll
     for (int j = 0; j < C::JD; ++j)
 #pragma unroll
@@ -663,8 +589,9 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     uint32_t phase = 1;  // the stages begin empty
     for (int u = u0; u < u1; ++u) {
       wait_phase(&ctl.empty[stage], phase, err, dead);
-      load_tile<C>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift,
-                   a.seqs.table + (int64_t)cur.b * a.seqs.table_stride, cur.len, cur.tile, cur.i / a.head_groups, err);
+      load_rows<C::T, C::RB, Word<CT>::size>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools,
+                                             a.box_shift, a.seqs.table + (int64_t)cur.b * a.seqs.table_stride, cur.len,
+                                             cur.tile, cur.i / a.head_groups, err);
       walk_on<C>(cur, a.seqs, items);
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
@@ -793,8 +720,8 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     uint32_t phase = 1;
     for (int t = t0; t < t1; ++t) {
       wait_phase(&ctl.empty[stage], phase, err, dead);
-      load_tile<C>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift,
-                   a.prefix_table, a.prefix_len, t, kvh, err);
+      load_rows<C::T, C::RB, Word<CT>::size>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools,
+                                             a.box_shift, a.prefix_table, a.prefix_len, t, kvh, err);
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
     return;
@@ -891,17 +818,18 @@ tb_status launch_prefix(AttnArgs &a, const tb_paged_cache *cache, const DeviceSt
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
   // one wave of CTAs, as far as the workspace holds its results
   int64_t splits = std::min<int64_t>(tiles, std::max<int64_t>(1, ctas / items));
-  splits = std::min(splits, 1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads));
-  a.prefix.splits = (int)splits;
+  a.prefix.splits = (int)std::min<int64_t>(splits, max_prefix_splits(a));
   if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
-  kern<<<dim3((unsigned)splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, C::SMEM, s>>>(a, maps.k, maps.v,
+  kern<<<dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, C::SMEM, s>>>(a, maps.k, maps.v,
                                                                                                       st->err_word);
   return check_launch(who);
 }
 
 template <int CT, int D, bool A32>
 tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s, const char *who) {
-  if (a.prefix_len > 0) {
+  if (CT != TB_F32 && a.prefix_len > 0 && a.prefix.rows >= kTensorRows) {
+    TB_TRY(launch_prefix_tc(a, cache, st, s, who));
+  } else if (a.prefix_len > 0) {
     switch (head_warps(a.prefix.rows)) {
       case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, cache, st, s, who))); break;
       case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, cache, st, s, who))); break;
@@ -969,6 +897,9 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
 }
 
 }  // namespace
+
+int max_prefix_splits(const AttnArgs &a) { return (int)(1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads)); }
+
 }  // namespace tb
 
 using namespace tb;

@@ -1,0 +1,440 @@
+// tb_paged_prefix.cu -- the common prefix of tb_paged_attention_shared on the
+// fifth-generation tensor cores (16-bit caches, many query rows).
+//
+// All sequences' query heads of one key/value head are the rows of a matrix
+// product against the prefix: S = Q K^T, P = exp2(scale S - m), O = P V, with
+// the running maximum m and sum l of each row; each CTA takes a share of the
+// keys and leaves (m, l, acc) per row, which the kernel of the sequences' own
+// keys joins.
+//
+// Accuracy: operands in parts as in tb_paged_attention.cu (a query in QT, a
+// probability in PT parts, one each with 16-bit activations, where a
+// probability is rounded to the cache's type as the output will be; fp16
+// probabilities are scaled by 2^15).  The parts are further MMAs into the same
+// accumulator.  O starts from zero for each tile and is added to fp32
+// registers (one FMA with the rescaling), so no long sum runs inside the
+// tensor core.
+//
+// Roles: two streams, each a warpgroup whose threads own one row each (TMEM
+// lane = row), and one warp issuing its MMAs; one warp loading.  While one
+// stream's exponentials run, the other's products do.  With more than 128 rows
+// the streams are two row tiles over the same keys (PAIR), which halves the
+// reads of K and V; else, or where two tiles' queries do not fit, they take
+// alternate key tiles of the same rows and join at the end.
+//   TMEM, per stream: S [KT columns] with P written over it, O [D columns].
+//   Chunk c of 32 keys is read from columns 32 c .. 32 c + 31 before its P is
+//   written: one part to 16 c, two parts to 32 c and 32 c + 16 (three parts,
+//   tiles of 64 keys: the third to 64 + 16 c).
+// The exponentials bound it (16 a cycle and SM: 1024 cycles for 128 x 128,
+// against 512 for the products at head_dim 64 and 1024 at 128).
+#include <algorithm>
+
+#include "tb_paged.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kBlock = 384;
+
+__device__ __forceinline__ void commit_to(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+// Waits for the loads; the registers are operands, so that no use of them moves ahead of it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory descriptor, 128-byte swizzle.  K-major (queries, keys): rows of
+// 128 bytes, groups of eight rows 1024 bytes apart.  MN-major (values): the same
+// bytes read as 64 columns of head_dim, groups of eight keys 1024 bytes apart,
+// the next 64 columns `lbo` bytes on.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// CT: cache type, D: head_dim, A32: fp32 activations.
+template <int CT_, int D, bool A32>
+struct TC {
+  static constexpr int CT = CT_;
+  static constexpr int QT = !A32 ? 1 : CT == TB_F16 ? 2 : 3;  // parts of a query and of a probability
+  static constexpr int KT = QT == 3 ? 64 : 128;               // keys per tile
+  static constexpr bool PAIR_FITS = QT * D <= 192;            // the queries of two row tiles in shared memory
+  static constexpr int RB = 2 * D, CB = D / 64;               // bytes and 128-byte columns of a row
+  static constexpr int QTILE = QT * CB * kRows * 128;
+  static constexpr int QBYTES = (PAIR_FITS ? 2 : 1) * QTILE;
+  static constexpr int HALF = KT * RB;  // a tile of keys, or of values
+  static constexpr int STAGES = (216 * 1024 - QBYTES) / (2 * HALF) < 4 ? (216 * 1024 - QBYTES) / (2 * HALF) : 4;
+  static constexpr float PEXP = CT == TB_F16 ? 15.f : 0.f;  // probabilities are scaled by 2^PEXP
+  static constexpr uint32_t F = CT == TB_BF16 ? 1u : 0u;
+  // D fp32, A and B of type F; N, M = 128; the second product's B is MN-major
+  static constexpr uint32_t IDESC_QK = (1u << 4) | (F << 7) | (F << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
+  static constexpr uint32_t IDESC_PV = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+  static constexpr int O = 128;  // column of a stream's O behind its S
+  static __device__ __forceinline__ int pcol(int part, int chunk) {
+    return QT == 1 ? 16 * chunk : part < 2 ? 32 * chunk + 16 * part : 64 + 16 * chunk;
+  }
+};
+
+struct PrefixControl {
+  uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+};
+
+template <class C>
+constexpr int prefix_smem() {
+  return C::QBYTES + C::STAGES * 2 * C::HALF + (int)sizeof(PrefixControl);
+}
+
+template <int CT, int D, bool A32>
+__global__ void __launch_bounds__(kBlock, 1)
+    paged_prefix_tc_kernel(const AttnArgs a, const int pair, const __grid_constant__ CUtensorMap km,
+                           const __grid_constant__ CUtensorMap vm, uint32_t *__restrict__ err) {
+  using C = TC<CT, D, A32>;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  PrefixControl &ctl = *reinterpret_cast<PrefixControl *>(smem + C::QBYTES + C::STAGES * 2 * C::HALF);
+  const uint32_t qs = smem_addr(smem), stages = qs + C::QBYTES;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.x, kvh = blockIdx.z;
+  const int all = (a.prefix_len + C::KT - 1) / C::KT;
+  const int t0 = (int)((int64_t)split * all / a.prefix.splits);
+  const int n = (int)((int64_t)(split + 1) * all / a.prefix.splits) - t0;  // tiles of this CTA
+  if (tid == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&ctl.kfull[i], 1);
+      mbar_init(&ctl.kempty[i], pair ? 2 : 1);
+      mbar_init(&ctl.vfull[i], 1);
+      mbar_init(&ctl.vempty[i], pair ? 2 : 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&ctl.s_full[w], 1);
+      mbar_init(&ctl.p_full[w], kRows);
+      mbar_init(&ctl.o_full[w], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 11) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&ctl.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // ---- queries: one thread per row of a stream
+  const int stream = warp >> 2, r = tid & 127;
+  const int row = (pair ? 2 * blockIdx.y + stream : blockIdx.y) * kRows + r;  // of all rows of the key/value head
+  float scale2 = fabsf(a.scale2);
+  if (stream < 2) {
+    const bool have = row < a.prefix.rows;
+    const int b = have ? row / a.group : 0;
+    const int64_t at = (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D;
+    const float sign = a.scale2 < 0.f ? -1.f : 1.f;  // a negative scale turns the queries round
+    float up = sign;
+    if (A32 && CT == TB_F16) {
+      float mx = 0.f;
+      for (int c = 0; have && c < D / 8; ++c) {
+        float f[8];
+        load_act<8>(a.q.p, at + 8 * c, TB_F32, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[e]));
+      }
+      const int e = fp16_exp(mx);
+      up *= pow2i(e);
+      scale2 *= pow2i(-e);
+    }
+    if (stream == 0 || pair) {
+#pragma unroll 2
+      for (int c = 0; c < D / 8; ++c) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 0.f;
+        if (have) load_act<8>(a.q.p, at + 8 * c, A32 ? TB_F32 : CT, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= up;
+#pragma unroll
+        for (int p = 0; p < C::QT; ++p) {
+          uint4 w;
+          w.x = pack_rest<CT>(f[0], f[1]);
+          w.y = pack_rest<CT>(f[2], f[3]);
+          w.z = pack_rest<CT>(f[4], f[5]);
+          w.w = pack_rest<CT>(f[6], f[7]);
+          const uint32_t to = qs + stream * C::QTILE + (p * C::CB + (c >> 3)) * kRows * 128 + r * 128 + (((c ^ r) & 7) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                       : "memory");
+        }
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = ctl.tmem;
+  bool dead = false;
+
+  // a stream's tiles: first, first + step, ... below n
+  const int step = pair ? 1 : 2;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 8) {  // ---- loading
+      for (int t = 0; t < n; ++t) {
+        const int s = t % C::STAGES;
+        const uint32_t ph = ((t / C::STAGES) & 1) ^ 1;
+        wait_phase(&ctl.kempty[s], ph, err, dead);
+        load_rows<C::KT, C::RB, 2>(stages + s * 2 * C::HALF, &ctl.kfull[s], &km, nullptr, a.pools, a.box_shift,
+                                   a.prefix_table, a.prefix_len, t0 + t, kvh, err);
+        wait_phase(&ctl.vempty[s], ph, err, dead);
+        load_rows<C::KT, C::RB, 2>(stages + s * 2 * C::HALF + C::HALF, &ctl.vfull[s], &vm, nullptr, a.pools,
+                                   a.box_shift, a.prefix_table, a.prefix_len, t0 + t, kvh, err);
+      }
+    } else if (warp < 11) {  // ---- products of stream w
+      const int w = warp - 9;
+      const uint32_t ts = tmem + w * 256, q = qs + (pair ? w * C::QTILE : 0);
+      uint32_t ph = 0;
+      for (int t = pair ? 0 : w; t < n; t += step, ph ^= 1) {
+        const int s = t % C::STAGES;
+        const uint32_t full = (t / C::STAGES) & 1;
+        const uint32_t k = stages + s * 2 * C::HALF, v = k + C::HALF;
+        const int keys = min(C::KT, a.prefix_len - (t0 + t) * C::KT);
+        wait_phase(&ctl.kfull[s], full, err, dead);
+        fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int p = 0; p < C::QT; ++p)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+              mma_ss(ts, desc(q + (p * C::CB + i / 4) * kRows * 128 + (i % 4) * 32, 16),
+                     desc(k + (i / 4) * C::KT * 128 + (i % 4) * 32, 16), C::IDESC_QK, p + i > 0);
+          commit_to(&ctl.s_full[w]);
+          commit_to(&ctl.kempty[s]);
+        }
+        __syncwarp();
+        wait_phase(&ctl.vfull[s], full, err, dead);
+        const int steps = (keys + 15) / 16;
+        if (keys < steps * 16) {
+          // the rows of the last step behind the prefix hold whatever their page held: 0 times that has to be 0
+          for (int i = lane; i < (steps * 16 - keys) * (C::RB / 16); i += 32) {
+            const int vr = keys + i / (C::RB / 16), c = i % (C::RB / 16);
+            sts128_zero(v + (c >> 3) * C::KT * 128 + vr * 128 + (((c ^ vr) & 7) << 4));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        wait_phase(&ctl.p_full[w], ph, err, dead);
+        fence_after();
+        if (lane == 0) {
+          for (int i = 0; i < steps; ++i)
+#pragma unroll
+            for (int p = 0; p < C::QT; ++p)
+              mma_ts(ts + C::O, ts + C::pcol(p, i / 2) + 8 * (i % 2), desc(v + i * 2048, C::KT * 128), C::IDESC_PV,
+                     p + i > 0);
+          commit_to(&ctl.vempty[s]);
+          if (t + step >= n) commit_to(&ctl.o_full[w]);
+        }
+        __syncwarp();
+      }
+    }
+  } else {  // ---- the exponentials of stream `stream`
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const uint32_t ts = tmem + stream * 256 + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
+    float acc[D], m = -INFINITY, l = 0.f, alpha = 1.f;
+#pragma unroll
+    for (int i = 0; i < D; ++i) acc[i] = 0.f;
+    // adds a finished tile's O to the running sum
+    auto take_o = [&]() {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(ts + C::O + 32 * c, o);
+        tmem_wait_ld(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(acc[32 * c + i], alpha, __uint_as_float(o[i]));
+      }
+    };
+    uint32_t ph = 0;
+    const int first = pair ? 0 : stream;
+    for (int t = first; t < n; t += step, ph ^= 1) {
+      wait_phase(&ctl.s_full[stream], ph, err, dead);  // this S, and with it the products before it: the last O
+      fence_after();
+      const int keys = a.prefix_len - (t0 + t) * C::KT;  // at most KT of them in this tile
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < C::KT / 32; ++c) {
+        uint32_t u[32];
+        tmem_ld32(ts + 32 * c, u);
+        tmem_wait_ld(u);
+        if (keys < C::KT) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= keys) u[i] = 0xFF800000u;  // -inf
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(u[i]));
+      }
+      if (t > first) take_o();
+      const float mn = fmaxf(m, mx * scale2);
+      const float ms = mn == -INFINITY ? 0.f : mn;
+      alpha = ex2(m - ms);
+      m = mn;
+      const float shift = C::PEXP - ms;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < C::KT / 32; ++c) {
+        uint32_t u[32];
+        tmem_ld32(ts + 32 * c, u);
+        tmem_wait_ld(u);
+        if (keys < C::KT) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= keys) u[i] = 0xFF800000u;
+        }
+        float p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          p[i] = ex2(fmaf(__uint_as_float(u[i]), scale2, shift));
+          sum += p[i];
+        }
+#pragma unroll
+        for (int k = 0; k < C::QT; ++k) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pack_rest<CT>(p[2 * i], p[2 * i + 1]);
+          tmem_st16(ts + C::pcol(k, c), w);
+        }
+      }
+      l = fmaf(l, alpha, sum);
+      tmem_wait_st();
+      fence_before();
+      mbar_arrive(&ctl.p_full[stream]);
+    }
+    if (first < n) {
+      wait_phase(&ctl.o_full[stream], 0, err, dead);
+      fence_after();
+      take_o();
+    }
+    const float down = CT == TB_F16 ? 1.f / 32768.f : 1.f;
+    l *= down;
+#pragma unroll
+    for (int i = 0; i < D; ++i) acc[i] *= down;
+    if (!pair) {
+      // both streams are done with the stages once both have their last O: the second leaves its results there
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      float *left = reinterpret_cast<float *>(smem + C::QBYTES);  // [D + 2][128]
+      if (stream == 1) {
+        left[D * kRows + r] = m;
+        left[(D + 1) * kRows + r] = l;
+#pragma unroll
+        for (int i = 0; i < D; ++i) left[i * kRows + r] = acc[i];
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (stream == 0) {
+        const float m1 = left[D * kRows + r];
+        const float mn = fmaxf(m, m1), ms = mn == -INFINITY ? 0.f : mn;
+        const float w0 = ex2(m - ms), w1 = ex2(m1 - ms);
+        m = mn;
+        l = l * w0 + left[(D + 1) * kRows + r] * w1;
+#pragma unroll
+        for (int i = 0; i < D; ++i) acc[i] = fmaf(acc[i], w0, left[i * kRows + r] * w1);
+      }
+    }
+    if (row < a.prefix.rows && (pair || stream == 0)) {
+      const int64_t at = ((int64_t)kvh * a.prefix.rows + row) * a.prefix.splits + split;
+      a.prefix.ml[at] = make_float2(m, l);
+      float4 *to = reinterpret_cast<float4 *>(a.prefix.acc + at * D);
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) to[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 11)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <int CT, int D, bool A32>
+tb_status launch(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s, const char *who) {
+  using C = TC<CT, D, A32>;
+  auto kern = paged_prefix_tc_kernel<CT, D, A32>;
+  constexpr int smem = prefix_smem<C>();
+  static_assert(smem <= 227 * 1024 && C::STAGES >= 2 && C::STAGES * 2 * C::HALF >= (D + 2) * kRows * 4, "");
+  TB_TRY(ensure_smem_for(kern, smem));
+  PagedMaps maps;
+  int box;
+  tb_paged_cache c = *cache;
+  if (c.n_pages == 0) c.n_pages = 1, c.k = c.v = a.counters;  // an empty pool: every page id is outside it
+  TB_TRY(paged_maps(&c, C::KT, who, &maps, &box));
+  a.box_shift = 0;
+  while ((1 << a.box_shift) < box) ++a.box_shift;
+  const int pair = C::PAIR_FITS && a.prefix.rows > kRows;
+  const int rows = pair ? 2 * kRows : kRows;
+  const int row_tiles = (a.prefix.rows + rows - 1) / rows;
+  const int tiles = (a.prefix_len + C::KT - 1) / C::KT;
+  const int64_t items = (int64_t)row_tiles * a.kv_heads;
+  const int64_t splits = std::min<int64_t>(tiles, std::max<int64_t>(1, st->sm_count / items));
+  a.prefix.splits = (int)std::min<int64_t>(splits, max_prefix_splits(a));
+  if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
+  kern<<<dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, smem, s>>>(
+      a, pair, maps.k, maps.v, st->err_word);
+  return check_launch(who);
+}
+
+}  // namespace
+
+tb_status launch_prefix_tc(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
+                           const char *who) {
+  const bool wide = cache->head_dim == 128, a32 = a.q.dtype == TB_F32;
+#define TB_PREFIX(CT, A32) \
+  return wide ? launch<CT, 128, A32>(a, cache, st, s, who) : launch<CT, 64, A32>(a, cache, st, s, who)
+  if (cache->dtype == TB_F16) {
+    if (a32) TB_PREFIX(TB_F16, true);
+    TB_PREFIX(TB_F16, false);
+  }
+  if (a32) TB_PREFIX(TB_BF16, true);
+  TB_PREFIX(TB_BF16, false);
+#undef TB_PREFIX
+}
+
+}  // namespace tb

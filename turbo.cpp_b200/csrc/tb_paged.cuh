@@ -42,14 +42,16 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_dtype, const char *who,
                      PagedPools *pools, PagedSeqs *seqs);
 
-// One row-tile's share of the prefix: unnormalised outputs acc[D] with their
-// running maximum m (of scale * log2(e) * q.k) and sum l, per row and split.
-// Row r of key/value head h, split s: acc at ((h * rows + r) * splits + s) * D.
+// Behind a prefix each query row has several partial results: one per split of
+// the prefix and a last one of the sequence's own keys.  Unnormalised outputs
+// acc[D] with their running maximum m (of scale * log2(e) * q.k) and sum l; row
+// r of key/value head h, part p: acc at ((h * rows + r) * parts + p) * D.
 struct PrefixParts {
   float *acc;
   float2 *ml;
   int rows;    // batch * group
   int splits;  // 0: no prefix
+  int parts;   // splits + 1
 };
 
 // The pools as 4-d tensors [page][token][head][head_dim] for TMA: a box is up
@@ -241,8 +243,27 @@ struct AttnArgs {
   int box_shift;  // a TMA box holds 1 << box_shift tokens
 };
 
-// Most splits of the prefix whose results the workspace holds.
-int max_prefix_splits(const AttnArgs &a);
+// Sets the prefix's splits: `want`, at least 1, as far as the workspace holds their results.
+void set_prefix_splits(AttnArgs &a, int64_t want);
+
+// A launch that may begin while the kernel before it ends; the kernel waits
+// (griddepcontrol.wait) before it reads what that one wrote.
+template <typename F, typename... A>
+tb_status launch_pdl(F *kern, dim3 grid, int threads, size_t smem, cudaStream_t s, const char *who, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) return fail(TB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
+  return check_launch(who);
+}
 
 // The prefix on tcgen05 (tb_paged_prefix.cu), 16-bit caches; sets a.prefix.splits.
 tb_status launch_prefix_tc(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,

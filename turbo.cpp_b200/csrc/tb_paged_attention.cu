@@ -39,7 +39,9 @@
 // lengths, so uneven batches and single long sequences fill the GPU alike and a
 // captured launch follows the lengths.  An item cut by a CTA boundary leaves
 // partial results in the workspace; the last of its CTAs to finish (a counter
-// per first CTA, reset by that CTA) joins them.
+// per first CTA, reset by that CTA) joins them.  Behind a prefix there are three
+// kernels: the prefix's (here, or tb_paged_prefix.cu for many rows), this one
+// for the sequences' own keys, and one that joins the parts of each row.
 #include <algorithm>
 
 #include "tb_paged.cuh"
@@ -533,6 +535,11 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     fence_mbar_init();
   }
 
+  // Behind a prefix the kernel before this one is the prefix's, whose results this one does not read and which began
+  // after everything earlier had ended: it is waited for only at the end, so that this kernel's end implies it.
+  pdl_launch_dependents();
+  if (a.prefix.splits == 0) pdl_wait();
+
   // ---- the units of all sequences, and this CTA's share: with n CTAs, unit r of U goes to r / (U / n) or so, the
   // first U % n CTAs taking one more (the host has made sure that U < 2^31)
   const int per = (a.seqs.batch + kBlock - 1) / kBlock;
@@ -558,7 +565,10 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     total += ctl.warp_sum[w];
   }
   const int n_ctas = min(a.max_ctas, total), me = blockIdx.x;
-  if (me >= n_ctas) return;
+  if (me >= n_ctas) {
+    pdl_wait();
+    return;
+  }
   const int share = total / n_ctas, more = total - share * n_ctas;
   auto first_unit = [&](int c) { return c * share + min(c, more); };
   auto owner = [&](int u) {
@@ -595,6 +605,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
       walk_on<C>(cur, a.seqs, items);
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
+    pdl_wait();
     return;
   }
 
@@ -606,16 +617,18 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + hw * 8 + (lane >> 2);
     return gi < a.group ? (int64_t)w.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
   };
-  // the output of item `w`: the join of its parts, behind those of the prefix
-  auto finish = [&](const Walk &w, Join<N> &j) {
+  // item `w` is complete: its output, or behind a prefix its part of it
+  auto finish = [&](const Walk &w, const Join<N> &j) {
     const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + row;
     if (gi >= a.group) return;
     if (a.prefix.splits > 0) {
-      const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)w.b * a.group + gi) * a.prefix.splits;
-      join_parts(j, a.prefix.splits, [&](int p) { return a.prefix.ml + at + p; },
-                 [&](int p, int i) { return a.prefix.acc + (at + p) * D + sub + i * TPR; });
+      const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)w.b * a.group + gi) * a.prefix.parts + a.prefix.splits;
+#pragma unroll
+      for (int i = 0; i < N; ++i) a.prefix.acc[at * D + sub + i * TPR] = j.acc[i];
+      if (sub == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
+      return;
     }
-    const bool none = w.len == 0 && a.prefix.splits == 0;
+    const bool none = w.len == 0;
     const int64_t at = (int64_t)w.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + sub;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -663,7 +676,10 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
   }
 
   // ---- the cut items: whoever of its CTAs comes last joins one
-  if (cut_unit[0] < 0 && cut_unit[1] < 0) return;
+  if (cut_unit[0] < 0 && cut_unit[1] < 0) {
+    pdl_wait();
+    return;
+  }
   if (tid == 0) {
     __threadfence();  // the whole CTA's partial results, seen by this thread at the barrier above
     for (int k = 0; k < 2; ++k) {
@@ -688,6 +704,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
                [&](int p, int i) { return a.slot_acc + slot(p) * D + sub + i * TPR; });
     finish(cut[k], j);
   }
+  pdl_wait();
 }
 
 // The prefix: item (split, row tile, key/value head), rows = the queries of all
@@ -710,6 +727,8 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     fence_mbar_init();
   }
   __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();  // only now: the next kernel relies on everything before this one having ended
   const int split = blockIdx.x, rt = blockIdx.y, kvh = blockIdx.z;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
   const int t0 = (int)((int64_t)split * tiles / a.prefix.splits);
@@ -752,10 +771,47 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
   if (row >= a.prefix.rows) return;
   Join<N> j;
   join_warps<C, D>(j, merge, r, sub);
-  const int64_t at = ((int64_t)kvh * a.prefix.rows + row) * a.prefix.splits + split;
+  const int64_t at = ((int64_t)kvh * a.prefix.rows + row) * a.prefix.parts + split;
 #pragma unroll
   for (int i = 0; i < N; ++i) a.prefix.acc[at * D + sub + i * TPR] = j.acc[i];
   if (sub == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
+}
+
+// The outputs behind a prefix: a warp per row joins its parts in order.
+template <int D>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const AttnArgs a, int heads) {
+  constexpr int E = D / 32, P = 8;  // elements per lane; parts loaded at once
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // b * heads + h
+  if (row >= (int64_t)a.seqs.batch * heads) return;
+  const int b = (int)(row / heads), h = (int)(row - (int64_t)b * heads), kvh = h / a.group;
+  const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)b * a.group + h - kvh * a.group) * a.prefix.parts;
+  Join<E> j;
+  for (int p0 = 0; p0 < a.prefix.parts; p0 += P) {
+    float2 ml[P];
+    float v[P][E];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const bool have = p0 + p < a.prefix.parts;
+      ml[p] = have ? __ldcg(a.prefix.ml + at + p0 + p) : make_float2(-INFINITY, 0.f);
+      const float *acc = a.prefix.acc + (at + p0 + p) * D + lane * E;
+      if constexpr (E == 2) {
+        const float2 x = have ? __ldcg(reinterpret_cast<const float2 *>(acc)) : make_float2(0.f, 0.f);
+        v[p][0] = x.x, v[p][1] = x.y;
+      } else {
+        const float4 x = have ? __ldcg(reinterpret_cast<const float4 *>(acc)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[p][0] = x.x, v[p][1] = x.y, v[p][2] = x.z, v[p][3] = x.w;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (p0 + p < a.prefix.parts) j.add(ml[p], [&](int i) { return v[p][i]; });
+  }
+  const int64_t to = (int64_t)b * a.ldo + (int64_t)h * D + lane * E;
+#pragma unroll
+  for (int i = 0; i < E; ++i) store_act1(a.out, to + i, a.q.dtype, __fdiv_rn(j.acc[i], j.l));
 }
 
 // Warps across query heads: the fewest that take the rows in one item, so that
@@ -769,7 +825,7 @@ struct Layout {
 };
 Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   const size_t slots = 2 * kMaxCtas * 8 * (size_t)head_warps(heads / kv_heads);
-  const size_t rows = (size_t)(batch * heads + kPrefixRows);
+  const size_t rows = (size_t)(2 * batch * heads + kPrefixRows);
   Layout l;
   l.slot_acc = up256(kMaxCtas * sizeof(int));
   l.slot_ml = l.slot_acc + up256(slots * D * sizeof(float));
@@ -800,8 +856,7 @@ tb_status launch_decode(AttnArgs &a, const tb_paged_cache *cache, const DeviceSt
   TB_TRY(tile_maps<C>(a, cache, who, &maps));
   const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kBlock, C::SMEM);
   a.max_ctas = std::min(ctas, kMaxCtas);
-  kern<<<a.max_ctas, kBlock, C::SMEM, s>>>(a, maps.k, maps.v, st->err_word);
-  return check_launch(who);
+  return launch_pdl(kern, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a, maps.k, maps.v, st->err_word);
 }
 
 template <int CT, int D, int HW, bool A32>
@@ -816,13 +871,11 @@ tb_status launch_prefix(AttnArgs &a, const tb_paged_cache *cache, const DeviceSt
   const int row_tiles = (a.prefix.rows + C::R - 1) / C::R;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
-  // one wave of CTAs, as far as the workspace holds its results
-  int64_t splits = std::min<int64_t>(tiles, std::max<int64_t>(1, ctas / items));
-  a.prefix.splits = (int)std::min<int64_t>(splits, max_prefix_splits(a));
+  // one wave of CTAs
+  set_prefix_splits(a, std::min<int64_t>(tiles, ctas / items));
   if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
-  kern<<<dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, C::SMEM, s>>>(a, maps.k, maps.v,
-                                                                                                      st->err_word);
-  return check_launch(who);
+  return launch_pdl(kern, dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, C::SMEM, s,
+                    who, a, maps.k, maps.v, st->err_word);
 }
 
 template <int CT, int D, bool A32>
@@ -840,11 +893,15 @@ tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, c
   const int hw = head_warps(a.group);
   a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
   switch (hw) {
-    case 1: return launch_decode<CT, D, 1, A32>(a, cache, st, s, who);
-    case 2: return launch_decode<CT, D, 2, A32>(a, cache, st, s, who);
-    case 4: return launch_decode<CT, D, 4, A32>(a, cache, st, s, who);
-    default: return launch_decode<CT, D, 8, A32>(a, cache, st, s, who);
+    case 1: TB_TRY((launch_decode<CT, D, 1, A32>(a, cache, st, s, who))); break;
+    case 2: TB_TRY((launch_decode<CT, D, 2, A32>(a, cache, st, s, who))); break;
+    case 4: TB_TRY((launch_decode<CT, D, 4, A32>(a, cache, st, s, who))); break;
+    default: TB_TRY((launch_decode<CT, D, 8, A32>(a, cache, st, s, who))); break;
   }
+  if (a.prefix.splits == 0) return TB_OK;
+  const int heads = a.kv_heads * a.group;
+  return launch_pdl(paged_combine_kernel<D>, dim3((unsigned)(((int64_t)a.seqs.batch * heads + 7) / 8)), 256, 0, s, who,
+                    a, heads);
 }
 
 tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, const int32_t *prefix_table,
@@ -898,7 +955,11 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
 
 }  // namespace
 
-int max_prefix_splits(const AttnArgs &a) { return (int)(1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads)); }
+void set_prefix_splits(AttnArgs &a, int64_t want) {
+  const int64_t most = 1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads);
+  a.prefix.splits = (int)std::min(std::max<int64_t>(want, 1), most);
+  a.prefix.parts = a.prefix.splits + 1;
+}
 
 }  // namespace tb
 

@@ -124,6 +124,7 @@ struct PrefixControl {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
   uint64_t s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
+  float down[2 * kRows];  // fp32 queries of an fp16 cache: 2^-e of each row
 };
 
 template <class C>
@@ -163,48 +164,50 @@ __global__ void __launch_bounds__(kBlock, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // ---- queries: one thread per row of a stream
+  pdl_wait();
+  pdl_launch_dependents();  // only now: the next kernel relies on everything before this one having ended
+  // ---- queries: D / 8 lanes per row, eight elements each
   const int stream = warp >> 2, r = tid & 127;
-  const int row = (pair ? 2 * blockIdx.y + stream : blockIdx.y) * kRows + r;  // of all rows of the key/value head
-  float scale2 = fabsf(a.scale2);
-  if (stream < 2) {
-    const bool have = row < a.prefix.rows;
-    const int b = have ? row / a.group : 0;
-    const int64_t at = (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D;
+  const int row0 = blockIdx.y * (pair ? 2 * kRows : kRows);  // of all rows of the key/value head
+  {
+    constexpr int L = D / 8;
+    const int c = tid % L;
     const float sign = a.scale2 < 0.f ? -1.f : 1.f;  // a negative scale turns the queries round
-    float up = sign;
-    if (A32 && CT == TB_F16) {
-      float mx = 0.f;
-      for (int c = 0; have && c < D / 8; ++c) {
-        float f[8];
-        load_act<8>(a.q.p, at + 8 * c, TB_F32, f);
+#pragma unroll 4
+    for (int i = tid / L; i < (pair ? 2 * kRows : kRows); i += kBlock / L) {
+      const int row = row0 + i;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+      if (row < a.prefix.rows) {
+        const int b = row / a.group;
+        load_act<8>(a.q.p, (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D + 8 * c,
+                    A32 ? TB_F32 : CT, f);
+      }
+      float up = sign;
+      if constexpr (A32 && CT == TB_F16) {
+        float mx = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[e]));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const int e = fp16_exp(mx);
+        up *= pow2i(e);
+        if (c == 0) ctl.down[i] = pow2i(-e);
       }
-      const int e = fp16_exp(mx);
-      up *= pow2i(e);
-      scale2 *= pow2i(-e);
-    }
-    if (stream == 0 || pair) {
-#pragma unroll 2
-      for (int c = 0; c < D / 8; ++c) {
-        float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = 0.f;
-        if (have) load_act<8>(a.q.p, at + 8 * c, A32 ? TB_F32 : CT, f);
+      for (int e = 0; e < 8; ++e) f[e] *= up;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= up;
-#pragma unroll
-        for (int p = 0; p < C::QT; ++p) {
-          uint4 w;
-          w.x = pack_rest<CT>(f[0], f[1]);
-          w.y = pack_rest<CT>(f[2], f[3]);
-          w.z = pack_rest<CT>(f[4], f[5]);
-          w.w = pack_rest<CT>(f[6], f[7]);
-          const uint32_t to = qs + stream * C::QTILE + (p * C::CB + (c >> 3)) * kRows * 128 + r * 128 + (((c ^ r) & 7) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                       : "memory");
-        }
+      for (int p = 0; p < C::QT; ++p) {
+        uint4 w;
+        w.x = pack_rest<CT>(f[0], f[1]);
+        w.y = pack_rest<CT>(f[2], f[3]);
+        w.z = pack_rest<CT>(f[4], f[5]);
+        w.w = pack_rest<CT>(f[6], f[7]);
+        const uint32_t to = qs + (i / kRows) * C::QTILE + (p * C::CB + (c >> 3)) * kRows * 128 + (i % kRows) * 128 +
+                            (((c ^ i) & 7) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                     : "memory");
       }
     }
   }
@@ -280,18 +283,33 @@ __global__ void __launch_bounds__(kBlock, 1)
   } else {  // ---- the exponentials of stream `stream`
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const uint32_t ts = tmem + stream * 256 + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
-    float acc[D], m = -INFINITY, l = 0.f, alpha = 1.f;
+    float scale2 = fabsf(a.scale2);
+    if (A32 && CT == TB_F16) scale2 *= ctl.down[(pair ? stream * kRows : 0) + r];
+    uint64_t acc[D / 2];  // pairs of columns
+    float m = -INFINITY, l = 0.f, alpha = 1.f;
 #pragma unroll
-    for (int i = 0; i < D; ++i) acc[i] = 0.f;
+    for (int i = 0; i < D / 2; ++i) acc[i] = 0ull;
     // adds a finished tile's O to the running sum
     auto take_o = [&]() {
+      const uint64_t al = pack2(alpha, alpha);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(ts + C::O + 32 * c, o);
         tmem_wait_ld(o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(acc[32 * c + i], alpha, __uint_as_float(o[i]));
+        for (int i = 0; i < 16; ++i)
+          acc[16 * c + i] = fma2(acc[16 * c + i], al, pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
+      }
+    };
+    // 32 scores of the row; those behind the prefix's end are -inf
+    auto scores = [&](uint32_t (&u)[32], int c, int keys) {
+      tmem_ld32(ts + 32 * c, u);
+      tmem_wait_ld(u);
+      if (keys < C::KT) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (32 * c + i >= keys) u[i] = 0xFF800000u;
       }
     };
     uint32_t ph = 0;
@@ -299,43 +317,34 @@ __global__ void __launch_bounds__(kBlock, 1)
     for (int t = first; t < n; t += step, ph ^= 1) {
       wait_phase(&ctl.s_full[stream], ph, err, dead);  // this S, and with it the products before it: the last O
       fence_after();
-      const int keys = a.prefix_len - (t0 + t) * C::KT;  // at most KT of them in this tile
-      float mx = -INFINITY;
+      const int keys = a.prefix_len - (t0 + t) * C::KT;  // KT or more except in the last tile
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < C::KT / 32; ++c) {
         uint32_t u[32];
-        tmem_ld32(ts + 32 * c, u);
-        tmem_wait_ld(u);
-        if (keys < C::KT) {
+        scores(u, c, keys);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i >= keys) u[i] = 0xFF800000u;  // -inf
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(u[i]));
+        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[i]));
       }
       if (t > first) take_o();
-      const float mn = fmaxf(m, mx * scale2);
+      const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2);
       const float ms = mn == -INFINITY ? 0.f : mn;
       alpha = ex2(m - ms);
       m = mn;
-      const float shift = C::PEXP - ms;
-      float sum = 0.f;
+      const uint64_t scale = pack2(scale2, scale2), shift = pack2(C::PEXP - ms, C::PEXP - ms);
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < C::KT / 32; ++c) {
         uint32_t u[32];
-        tmem_ld32(ts + 32 * c, u);
-        tmem_wait_ld(u);
-        if (keys < C::KT) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i >= keys) u[i] = 0xFF800000u;
-        }
+        scores(u, c, keys);
         float p[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          p[i] = ex2(fmaf(__uint_as_float(u[i]), scale2, shift));
-          sum += p[i];
+        for (int i = 0; i < 16; ++i) {
+          const uint64_t x = fma2(pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), scale, shift);
+          unpack2(x, p[2 * i], p[2 * i + 1]);
+          p[2 * i] = ex2(p[2 * i]);
+          p[2 * i + 1] = ex2(p[2 * i + 1]);
+          sum[i & 1] = add2(sum[i & 1], pack2(p[2 * i], p[2 * i + 1]));
         }
 #pragma unroll
         for (int k = 0; k < C::QT; ++k) {
@@ -345,7 +354,9 @@ __global__ void __launch_bounds__(kBlock, 1)
           tmem_st16(ts + C::pcol(k, c), w);
         }
       }
-      l = fmaf(l, alpha, sum);
+      float s0, s1;
+      unpack2(add2(sum[0], sum[1]), s0, s1);
+      l = fmaf(l, alpha, s0 + s1);
       tmem_wait_st();
       fence_before();
       mbar_arrive(&ctl.p_full[stream]);
@@ -355,10 +366,15 @@ __global__ void __launch_bounds__(kBlock, 1)
       fence_after();
       take_o();
     }
-    const float down = CT == TB_F16 ? 1.f / 32768.f : 1.f;
+    constexpr float down = CT == TB_F16 ? 1.f / 32768.f : 1.f;
+    float out[D];
     l *= down;
 #pragma unroll
-    for (int i = 0; i < D; ++i) acc[i] *= down;
+    for (int i = 0; i < D / 2; ++i) {
+      unpack2(acc[i], out[2 * i], out[2 * i + 1]);
+      out[2 * i] *= down;
+      out[2 * i + 1] *= down;
+    }
     if (!pair) {
       // both streams are done with the stages once both have their last O: the second leaves its results there
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         left[D * kRows + r] = m;
         left[(D + 1) * kRows + r] = l;
 #pragma unroll
-        for (int i = 0; i < D; ++i) left[i * kRows + r] = acc[i];
+        for (int i = 0; i < D; ++i) left[i * kRows + r] = out[i];
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (stream == 0) {
@@ -377,15 +393,33 @@ __global__ void __launch_bounds__(kBlock, 1)
         m = mn;
         l = l * w0 + left[(D + 1) * kRows + r] * w1;
 #pragma unroll
-        for (int i = 0; i < D; ++i) acc[i] = fmaf(acc[i], w0, left[i * kRows + r] * w1);
+        for (int i = 0; i < D; ++i) out[i] = fmaf(out[i], w0, left[i * kRows + r] * w1);
       }
     }
-    if (row < a.prefix.rows && (pair || stream == 0)) {
-      const int64_t at = ((int64_t)kvh * a.prefix.rows + row) * a.prefix.splits + split;
-      a.prefix.ml[at] = make_float2(m, l);
-      float4 *to = reinterpret_cast<float4 *>(a.prefix.acc + at * D);
+    // results through shared memory, so that rows leave whole: the stream's queries are no longer read (its last O is
+    // here), and half of the columns take at most their room
+    if (pair || stream == 0) {
+      constexpr int H = D / 2;  // columns at a time
+      static_assert(kRows * H * 4 <= C::QTILE, "");
+      const int row = row0 + (pair ? stream * kRows : 0);
+      if (row + r < a.prefix.rows)
+        a.prefix.ml[((int64_t)kvh * a.prefix.rows + row + r) * a.prefix.parts + split] = make_float2(m, l);
+      float4 *buf = reinterpret_cast<float4 *>(smem + (pair ? stream * C::QTILE : 0));
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) to[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < H / 4; ++i)
+          buf[r * (H / 4) + (i ^ (r & 7))] = make_float4(out[h * H + 4 * i], out[h * H + 4 * i + 1],
+                                                         out[h * H + 4 * i + 2], out[h * H + 4 * i + 3]);
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
+        for (int i = r; i < kRows * H / 4; i += kRows) {
+          const int x = i / (H / 4), c = i % (H / 4);
+          if (row + x < a.prefix.rows)
+            reinterpret_cast<float4 *>(a.prefix.acc + (((int64_t)kvh * a.prefix.rows + row + x) * a.prefix.parts + split) * D +
+                                       h * H)[c] = buf[x * (H / 4) + (c ^ (x & 7))];
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
+      }
     }
   }
   fence_before();
@@ -413,12 +447,10 @@ tb_status launch(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st
   const int row_tiles = (a.prefix.rows + rows - 1) / rows;
   const int tiles = (a.prefix_len + C::KT - 1) / C::KT;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
-  const int64_t splits = std::min<int64_t>(tiles, std::max<int64_t>(1, st->sm_count / items));
-  a.prefix.splits = (int)std::min<int64_t>(splits, max_prefix_splits(a));
+  set_prefix_splits(a, std::min<int64_t>(tiles, st->sm_count / items));
   if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
-  kern<<<dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, smem, s>>>(
-      a, pair, maps.k, maps.v, st->err_word);
-  return check_launch(who);
+  return launch_pdl(kern, dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, smem, s,
+                    who, a, pair, maps.k, maps.v, st->err_word);
 }
 
 }  // namespace

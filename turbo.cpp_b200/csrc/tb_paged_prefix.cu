@@ -11,9 +11,12 @@
 // probability in PT parts, one each with 16-bit activations, where a
 // probability is rounded to the cache's type as the output will be; fp16
 // probabilities are scaled by 2^15).  The parts are further MMAs into the same
-// accumulator.  O starts from zero for each tile and is added to fp32
-// registers (one FMA with the rescaling), so no long sum runs inside the
-// tensor core.
+// accumulator.  With fp32 activations O starts from zero for each tile and is
+// added to fp32 registers (one FMA with the rescaling), so no long sum runs
+// inside the tensor core, whose accumulator cuts off rather than rounds (2^-24 a
+// step: some 1e-5 over a share of the keys).  With 16-bit activations, whose
+// outputs are rounded to 2^-9 or 2^-12, O stays in tensor memory for the whole
+// share and is rescaled only where a row's maximum has grown by 2^8.
 //
 // Roles: two streams, each a warpgroup whose threads own one row each (TMEM
 // lane = row), and one warp issuing its MMAs; one warp loading.  While one
@@ -69,9 +72,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-// Waits for the loads; the registers are operands, so that no use of them moves ahead of it.
-__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// After the wait: the registers become operands, so that no use of them moves ahead of it.
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
+  asm volatile(""
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
                  "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
@@ -102,14 +116,17 @@ template <int CT_, int D, bool A32>
 struct TC {
   static constexpr int CT = CT_;
   static constexpr int QT = !A32 ? 1 : CT == TB_F16 ? 2 : 3;  // parts of a query and of a probability
-  static constexpr int KT = QT == 3 ? 64 : 128;               // keys per tile
+  static constexpr int KT = QT == 3 || QT * D == 256 ? 64 : 128;  // keys per tile: a row's scores, and with fp32
+                                                                  // activations its sums, are one thread's registers
+  static constexpr bool SUMS = A32;                           // O summed in registers, tile by tile
   static constexpr bool PAIR_FITS = QT * D <= 192;            // the queries of two row tiles in shared memory
   static constexpr int RB = 2 * D, CB = D / 64;               // bytes and 128-byte columns of a row
   static constexpr int QTILE = QT * CB * kRows * 128;
   static constexpr int QBYTES = (PAIR_FITS ? 2 : 1) * QTILE;
   static constexpr int HALF = KT * RB;  // a tile of keys, or of values
   static constexpr int STAGES = (216 * 1024 - QBYTES) / (2 * HALF) < 4 ? (216 * 1024 - QBYTES) / (2 * HALF) : 4;
-  static constexpr float PEXP = CT == TB_F16 ? 15.f : 0.f;  // probabilities are scaled by 2^PEXP
+  static constexpr float SLACK = SUMS ? 0.f : 8.f;  // log2 by which a row may exceed its reference maximum
+  static constexpr float PEXP = CT == TB_F16 ? 15.f - SLACK : 0.f;  // probabilities are scaled by 2^PEXP
   static constexpr uint32_t F = CT == TB_BF16 ? 1u : 0u;
   // D fp32, A and B of type F; N, M = 128; the second product's B is MN-major
   static constexpr uint32_t IDESC_QK = (1u << 4) | (F << 7) | (F << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
@@ -242,6 +259,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         const uint32_t full = (t / C::STAGES) & 1;
         const uint32_t k = stages + s * 2 * C::HALF, v = k + C::HALF;
         const int keys = min(C::KT, a.prefix_len - (t0 + t) * C::KT);
+        const bool later = t >= step;  // not the stream's first tile: O is added to, where it stays in TMEM
         wait_phase(&ctl.kfull[s], full, err, dead);
         fence_after();
         if (lane == 0) {
@@ -273,7 +291,7 @@ __global__ void __launch_bounds__(kBlock, 1)
 #pragma unroll
             for (int p = 0; p < C::QT; ++p)
               mma_ts(ts + C::O, ts + C::pcol(p, i / 2) + 8 * (i % 2), desc(v + i * 2048, C::KT * 128), C::IDESC_PV,
-                     p + i > 0);
+                     p + i > 0 || (!C::SUMS && later));
           commit_to(&ctl.vempty[s]);
           if (t + step >= n) commit_to(&ctl.o_full[w]);
         }
@@ -285,31 +303,40 @@ __global__ void __launch_bounds__(kBlock, 1)
     const uint32_t ts = tmem + stream * 256 + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
     float scale2 = fabsf(a.scale2);
     if (A32 && CT == TB_F16) scale2 *= ctl.down[(pair ? stream * kRows : 0) + r];
-    uint64_t acc[D / 2];  // pairs of columns
+    uint64_t acc[C::SUMS ? D / 2 : 1];  // pairs of columns
     float m = -INFINITY, l = 0.f, alpha = 1.f;
 #pragma unroll
-    for (int i = 0; i < D / 2; ++i) acc[i] = 0ull;
-    // adds a finished tile's O to the running sum
+    for (int i = 0; i < (C::SUMS ? D / 2 : 1); ++i) acc[i] = 0ull;
+    // SUMS: adds a finished tile's O to the running sum
     auto take_o = [&]() {
       const uint64_t al = pack2(alpha, alpha);
 #pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t o[2][32];
+        tmem_ld32(ts + C::O + 64 * c, o[0]);
+        tmem_ld32(ts + C::O + 64 * c + 32, o[1]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          loaded(o[h]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            uint64_t &x = acc[C::SUMS ? 32 * c + 16 * h + i : 0];
+            x = fma2(x, al, pack2(__uint_as_float(o[h][2 * i]), __uint_as_float(o[h][2 * i + 1])));
+          }
+        }
+      }
+    };
+    // not SUMS: O times this row's factor, in place (the products before are done, the next wait for P)
+    auto scale_o = [&](float f) {
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(ts + C::O + 32 * c, o);
-        tmem_wait_ld(o);
+        tmem_wait_ld();
+        loaded(o);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          acc[16 * c + i] = fma2(acc[16 * c + i], al, pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
-      }
-    };
-    // 32 scores of the row; those behind the prefix's end are -inf
-    auto scores = [&](uint32_t (&u)[32], int c, int keys) {
-      tmem_ld32(ts + 32 * c, u);
-      tmem_wait_ld(u);
-      if (keys < C::KT) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (32 * c + i >= keys) u[i] = 0xFF800000u;
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st32(ts + C::O + 32 * c, o);
       }
     };
     uint32_t ph = 0;
@@ -317,30 +344,53 @@ __global__ void __launch_bounds__(kBlock, 1)
     for (int t = first; t < n; t += step, ph ^= 1) {
       wait_phase(&ctl.s_full[stream], ph, err, dead);  // this S, and with it the products before it: the last O
       fence_after();
+      if (C::SUMS && t > first) take_o();
+      uint32_t u[C::KT / 32][32];  // the row's scores, then its probabilities
+#pragma unroll
+      for (int c = 0; c < C::KT / 32; ++c) tmem_ld32(ts + 32 * c, u[c]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < C::KT / 32; ++c) loaded(u[c]);
       const int keys = a.prefix_len - (t0 + t) * C::KT;  // KT or more except in the last tile
+      if (keys < C::KT) {
+#pragma unroll
+        for (int c = 0; c < C::KT / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= keys) u[c][i] = 0xFF800000u;  // -inf
+      }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < C::KT / 32; ++c) {
-        uint32_t u[32];
-        scores(u, c, keys);
+      for (int c = 0; c < C::KT / 32; ++c)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[i]));
+        for (int i = 0; i < 32; i += 2)
+          mx[(i >> 1) & 3] = fmaxf(mx[(i >> 1) & 3], fmaxf(__uint_as_float(u[c][i]), __uint_as_float(u[c][i + 1])));
+      const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2);
+      if constexpr (C::SUMS) {
+        alpha = ex2(m - (top == -INFINITY ? 0.f : top));
+        l *= alpha;
+        m = top;
+      } else if (t == first) {
+        m = top;
+      } else {
+        // the reference maximum follows only where a row has outgrown it by 2^SLACK; its O and l are then scaled down
+        const bool grown = top > m + C::SLACK;
+        if (__any_sync(0xffffffffu, grown)) {
+          const float f = grown ? ex2(m - top) : 1.f;
+          scale_o(f);
+          l *= f;
+          if (grown) m = top;
+        }
       }
-      if (t > first) take_o();
-      const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2);
-      const float ms = mn == -INFINITY ? 0.f : mn;
-      alpha = ex2(m - ms);
-      m = mn;
+      const float ms = m == -INFINITY ? 0.f : m;
       const uint64_t scale = pack2(scale2, scale2), shift = pack2(C::PEXP - ms, C::PEXP - ms);
       uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < C::KT / 32; ++c) {
-        uint32_t u[32];
-        scores(u, c, keys);
         float p[32];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint64_t x = fma2(pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), scale, shift);
+          const uint64_t x = fma2(pack2(__uint_as_float(u[c][2 * i]), __uint_as_float(u[c][2 * i + 1])), scale, shift);
           unpack2(x, p[2 * i], p[2 * i + 1]);
           p[2 * i] = ex2(p[2 * i]);
           p[2 * i + 1] = ex2(p[2 * i + 1]);
@@ -356,25 +406,37 @@ __global__ void __launch_bounds__(kBlock, 1)
       }
       float s0, s1;
       unpack2(add2(sum[0], sum[1]), s0, s1);
-      l = fmaf(l, alpha, s0 + s1);
+      l += s0 + s1;
       tmem_wait_st();
       fence_before();
       mbar_arrive(&ctl.p_full[stream]);
     }
+    float out[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i) out[i] = 0.f;
     if (first < n) {
       wait_phase(&ctl.o_full[stream], 0, err, dead);
       fence_after();
-      take_o();
+      if constexpr (C::SUMS) {
+        take_o();
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) unpack2(acc[i], out[2 * i], out[2 * i + 1]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(ts + C::O + 32 * c, o);
+          tmem_wait_ld();
+          loaded(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) out[32 * c + i] = __uint_as_float(o[i]);
+        }
+      }
     }
-    constexpr float down = CT == TB_F16 ? 1.f / 32768.f : 1.f;
-    float out[D];
+    const float down = ex2(-C::PEXP);
     l *= down;
 #pragma unroll
-    for (int i = 0; i < D / 2; ++i) {
-      unpack2(acc[i], out[2 * i], out[2 * i + 1]);
-      out[2 * i] *= down;
-      out[2 * i + 1] *= down;
-    }
+    for (int i = 0; i < D; ++i) out[i] *= down;
     if (!pair) {
       // both streams are done with the stages once both have their last O: the second leaves its results there
       asm volatile("bar.sync 1, 256;" ::: "memory");

@@ -102,6 +102,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Shared-memory descriptor, 128-byte swizzle.  K-major (queries, keys): rows of
 // 128 bytes, groups of eight rows 1024 bytes apart.  MN-major (values): the same
 // bytes read as 64 columns of head_dim, groups of eight keys 1024 bytes apart,
@@ -139,7 +145,7 @@ struct TC {
 
 struct PrefixControl {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2];
   uint32_t tmem;
   float down[2 * kRows];  // fp32 queries of an fp16 cache: 2^-e of each row
 };
@@ -171,7 +177,8 @@ __global__ void __launch_bounds__(kBlock, 1)
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&ctl.s_full[w], 1);
-      mbar_init(&ctl.p_full[w], kRows);
+      mbar_init(&ctl.p_full[w][0], kRows);
+      mbar_init(&ctl.p_full[w][1], kRows);
       mbar_init(&ctl.o_full[w], 1);
     }
     fence_mbar_init();
@@ -181,25 +188,48 @@ __global__ void __launch_bounds__(kBlock, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  fence_before();
+  __syncthreads();
+  fence_after();
   pdl_wait();
   pdl_launch_dependents();  // only now: the next kernel relies on everything before this one having ended
-  // ---- queries: D / 8 lanes per row, eight elements each
   const int stream = warp >> 2, r = tid & 127;
   const int row0 = blockIdx.y * (pair ? 2 * kRows : kRows);  // of all rows of the key/value head
-  {
-    constexpr int L = D / 8;
-    const int c = tid % L;
-    const float sign = a.scale2 < 0.f ? -1.f : 1.f;  // a negative scale turns the queries round
-#pragma unroll 4
-    for (int i = tid / L; i < (pair ? 2 * kRows : kRows); i += kBlock / L) {
-      const int row = row0 + i;
-      float f[8];
+  // ---- queries (all warps but the loading one): D / 8 lanes per row, eight elements each
+  if (warp != 8) {
+    constexpr int L = D / 8, PER = (kBlock - 32) / L;  // rows at a time
+    constexpr int N = 2 * kRows / PER + 1, W = A32 ? 2 : 1;
+    static_assert(PER % (32 / L) == 0, "a warp's rows end together");
+    const int at = tid < 256 ? tid : tid - 32, c = at % L;
+    const int rows = pair ? 2 * kRows : kRows;
+    uint4 raw[N][W];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = 0.f;
-      if (row < a.prefix.rows) {
+    for (int k = 0; k < N; ++k) {
+      const int i = at / L + k * PER, row = row0 + i;
+#pragma unroll
+      for (int e = 0; e < W; ++e) raw[k][e] = make_uint4(0, 0, 0, 0);
+      if (i < rows && row < a.prefix.rows) {
         const int b = row / a.group;
-        load_act<8>(a.q.p, (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D + 8 * c,
-                    A32 ? TB_F32 : CT, f);
+        const int64_t from = (int64_t)b * a.q.ld + (int64_t)(kvh * a.group + row - b * a.group) * D + 8 * c;
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          raw[k][e] = reinterpret_cast<const uint4 *>(static_cast<const char *>(a.q.p) + from * (A32 ? 4 : 2))[e];
+      }
+    }
+    const float sign = a.scale2 < 0.f ? -1.f : 1.f;  // a negative scale turns the queries round
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = at / L + k * PER;
+      if (i >= rows) break;
+      float f[8];
+      if constexpr (A32) {
+        float lo[4], hi[4];
+        Word<TB_F32>::get(raw[k][0], lo);
+        Word<TB_F32>::get(raw[k][W - 1], hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
+      } else {
+        Word<CT>::get(raw[k][0], f);
       }
       float up = sign;
       if constexpr (A32 && CT == TB_F16) {
@@ -227,11 +257,9 @@ __global__ void __launch_bounds__(kBlock, 1)
                      : "memory");
       }
     }
+    fence_proxy_async_smem();
+    asm volatile("bar.sync 4, %0;" ::"n"(kBlock - 32) : "memory");
   }
-  fence_proxy_async_smem();
-  fence_before();
-  __syncthreads();
-  fence_after();
   const uint32_t tmem = ctl.tmem;
   bool dead = false;
 
@@ -284,14 +312,20 @@ __global__ void __launch_bounds__(kBlock, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        wait_phase(&ctl.p_full[w], ph, err, dead);
-        fence_after();
-        if (lane == 0) {
-          for (int i = 0; i < steps; ++i)
+        // P arrives in two halves, so that the first one's products run during the second's exponentials
+        for (int h = 0; h < 2; ++h) {
+          wait_phase(&ctl.p_full[w][h], ph, err, dead);
+          fence_after();
+          if (lane == 0) {
+            for (int i = h * (C::KT / 32); i < min(steps, (h + 1) * (C::KT / 32)); ++i)
 #pragma unroll
-            for (int p = 0; p < C::QT; ++p)
-              mma_ts(ts + C::O, ts + C::pcol(p, i / 2) + 8 * (i % 2), desc(v + i * 2048, C::KT * 128), C::IDESC_PV,
-                     p + i > 0 || (!C::SUMS && later));
+              for (int p = 0; p < C::QT; ++p)
+                mma_ts(ts + C::O, ts + C::pcol(p, i / 2) + 8 * (i % 2), desc(v + i * 2048, C::KT * 128), C::IDESC_PV,
+                       p + i > 0 || (!C::SUMS && later));
+          }
+          __syncwarp();
+        }
+        if (lane == 0) {
           commit_to(&ctl.vempty[s]);
           if (t + step >= n) commit_to(&ctl.o_full[w]);
         }
@@ -311,19 +345,15 @@ __global__ void __launch_bounds__(kBlock, 1)
     auto take_o = [&]() {
       const uint64_t al = pack2(alpha, alpha);
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t o[2][32];
-        tmem_ld32(ts + C::O + 64 * c, o[0]);
-        tmem_ld32(ts + C::O + 64 * c + 32, o[1]);
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(ts + C::O + 32 * c, o);
         tmem_wait_ld();
+        loaded(o);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          loaded(o[h]);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            uint64_t &x = acc[C::SUMS ? 32 * c + 16 * h + i : 0];
-            x = fma2(x, al, pack2(__uint_as_float(o[h][2 * i]), __uint_as_float(o[h][2 * i + 1])));
-          }
+        for (int i = 0; i < 16; ++i) {
+          uint64_t &x = acc[C::SUMS ? 16 * c + i : 0];
+          x = fma2(x, al, pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
         }
       }
     };
@@ -364,7 +394,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       for (int c = 0; c < C::KT / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 32; i += 2)
-          mx[(i >> 1) & 3] = fmaxf(mx[(i >> 1) & 3], fmaxf(__uint_as_float(u[c][i]), __uint_as_float(u[c][i + 1])));
+          mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(u[c][i]), __uint_as_float(u[c][i + 1]));
       const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2);
       if constexpr (C::SUMS) {
         alpha = ex2(m - (top == -INFINITY ? 0.f : top));
@@ -403,13 +433,15 @@ __global__ void __launch_bounds__(kBlock, 1)
           for (int i = 0; i < 16; ++i) w[i] = pack_rest<CT>(p[2 * i], p[2 * i + 1]);
           tmem_st16(ts + C::pcol(k, c), w);
         }
+        if (c == C::KT / 64 - 1 || c == C::KT / 32 - 1) {
+          tmem_wait_st();
+          fence_before();
+          mbar_arrive(&ctl.p_full[stream][c == C::KT / 32 - 1]);
+        }
       }
       float s0, s1;
       unpack2(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
-      tmem_wait_st();
-      fence_before();
-      mbar_arrive(&ctl.p_full[stream]);
     }
     float out[D];
 #pragma unroll

@@ -71,28 +71,44 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, in
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // Waits for a barrier's phase; once a wait has run out (bit 0 of the error
 // word is set then), later ones return at once, so that the kernel ends.
 __device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead) {
   if (!dead && !mbar_wait_bounded(bar, phase, err)) dead = true;
 }
 
-// One warp: tile `tile` (T keys or values of row size RB) of a sequence of len
-// tokens into shared memory, 128-byte columns T * 128 bytes apart.  Boxes that
-// begin at or behind len are left out; a page id outside the pool is given to
-// TMA as page -1, whose rows are zeros.  With two maps both tiles are fetched,
-// the second T * RB bytes behind the first.
+// A tile of T keys or values of a sequence of len tokens, in boxes of one page.
+struct TileBoxes {
+  int n, first;  // boxes that begin before len; page id of this lane's first one
+};
+template <int T>
+__device__ __forceinline__ TileBoxes tile_boxes(const PagedPools &p, int box_shift, const int32_t *table, int len,
+                                                int tile) {
+  const int lane = threadIdx.x & 31;
+  TileBoxes b;
+  b.n = (min(max(len - tile * T, 0), T) + (1 << box_shift) - 1) >> box_shift;
+  b.first = lane < b.n ? __ldg(table + ((tile * T + (lane << box_shift)) >> p.shift)) : 0;
+  return b;
+}
+
+// One warp: the tile's rows (RB bytes each) into shared memory, 128-byte
+// columns T * 128 bytes apart.  A page id outside the pool is given to TMA as
+// page -1, whose rows are zeros.  With two maps both tiles are fetched, the
+// second T * RB bytes behind the first.
 template <int T, int RB, int SIZE>
 __device__ __forceinline__ void load_rows(uint32_t dst0, uint64_t *full, const CUtensorMap *m0, const CUtensorMap *m1,
-                                          const PagedPools &p, int box_shift, const int32_t *table, int len, int tile,
-                                          int kvh, uint32_t *err) {
-  const int lane = threadIdx.x & 31, box = 1 << box_shift;
-  const int boxes = (min(max(len - tile * T, 0), T) + box - 1) >> box_shift;
-  if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)((boxes << box_shift) * (m1 ? 2 : 1) * RB));
+                                          const PagedPools &p, int box_shift, const int32_t *table, TileBoxes b,
+                                          int tile, int kvh, uint32_t *err) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)((b.n << box_shift) * (m1 ? 2 : 1) * RB));
   __syncwarp();
-  for (int i = lane; i < boxes; i += 32) {
+  for (int i = lane; i < b.n; i += 32) {
     const int t = tile * T + (i << box_shift);
-    int page = __ldg(table + (t >> p.shift));
+    int page = i == lane ? b.first : __ldg(table + (t >> p.shift));
     if ((uint32_t)page >= p.n_pages) {
       atomicOr(err, ERR_INDEX);
       page = -1;

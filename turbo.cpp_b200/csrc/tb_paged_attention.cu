@@ -25,10 +25,10 @@
 // queries are exact in one part.  Products are summed inside the tensor core
 // over 16 keys and then added to fp32 registers.
 //
-// Layout.  A ninth warp brings tiles of T keys and values into three stages of
-// shared memory by TMA, one box per page, 128 bytes of each row, swizzled so
-// that every 16-byte fragment load is free of bank conflicts.  Of the eight
-// other warps HW take eight query heads each, KW = 8 / HW take T / KW keys each; each warp keeps
+// Layout.  Each CTA's fifth warp brings tiles of T keys and values into three or
+// four stages of shared memory by TMA, one box per page, 128 bytes of each row,
+// swizzled so that every 16-byte fragment load is free of bank conflicts.  Of
+// the four other warps HW take eight query heads each, KW = 4 / HW take T / KW keys each; each warp keeps
 // its own (m, l, acc), joined once per item.  The order of head_dim inside the
 // dot product is chosen so that each thread's fragments are whole 16-byte words
 // of a key; 16-bit values are read transposed by ldmatrix.
@@ -49,12 +49,11 @@
 namespace tb {
 namespace {
 
-constexpr int kMaxCtas = 320;                    // of a decode launch (counters and partial slots)
+constexpr int kMaxCtas = 448;                    // of a decode launch (counters and partial slots)
 constexpr int64_t kPrefixRows = 2 * 148 * 128;   // extra (row, split) pairs of prefix partials
-constexpr int kWarps = 8;             // computing warps
+constexpr int kWarps = 4;              // computing warps
 constexpr int kThreads = kWarps * 32;  // their threads
 constexpr int kBlock = kThreads + 32;  // and one warp that loads
-constexpr int kStages = 3;
 constexpr int kTensorRows = 64;       // query rows of a key/value head from which the prefix runs on tcgen05
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -126,10 +125,15 @@ __device__ __forceinline__ uint4 ldmatrix_t(uint32_t addr) {
 }
 
 // What a CTA keeps in shared memory behind the stages and the merge buffer.
+struct Walk {  // where a CTA stands in the list of all units: tile `tile` of item (b, i)
+  int b, i, tile, tiles, len;
+};
+constexpr int kMaxStages = 4;
 struct Control {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  Walk at[kMaxStages];  // what each stage holds
+  Walk first;
   int warp_sum[kWarps + 1];
-  int first[5];
   int last[2];
 };
 
@@ -144,14 +148,16 @@ struct Cfg {
   static constexpr int EPC = Word<CT>::n;         // elements per 16-byte word
   static constexpr int RB = D * Word<CT>::size;   // bytes per row
   static constexpr int CPR = RB / 16;             // words per row
-  static constexpr int T = RB > 256 ? 64 : 128;   // keys per tile
+  static constexpr int T = RB > 256 ? 32 : 64;    // keys per tile
   static constexpr int KW = kWarps / HW;          // warps across keys
   static constexpr int KPW = T / KW;              // keys per warp and tile
   static constexpr int NT = KPW >= 16 ? 2 : 1;    // 8-key blocks per step
   static constexpr int R = 8 * HW;                // rows (query heads) per item
   static constexpr int STAGE = 2 * T * RB;
+  static constexpr int STAGES = RB > 128 ? 3 : 4;
+  static constexpr int CTAS = RB > 128 ? 2 : 3;   // per SM: 192 KB of tiles in either case
   static constexpr int MERGE = kWarps * 8 * (D + 2) * 4;
-  static constexpr int SMEM = kStages * STAGE + MERGE + (int)sizeof(Control);
+  static constexpr int SMEM = STAGES * STAGE + MERGE + (int)sizeof(Control);
   static constexpr int JD = D / 4 / EPC;  // 16-byte words of a key per thread
   static constexpr int JV = D / 8 / EPC;  // 16-byte words of a value per thread and key
 };
@@ -165,6 +171,12 @@ struct WarpState {
   float acc[D / 8][2];
   float m, l;
 };
+
+__device__ __forceinline__ int atom_add_acq_rel(int *p, int v) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
 
 __device__ __forceinline__ void computing_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
@@ -407,8 +419,8 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
   }
 }
 
-// Leaves the warp's (m, l, acc) in the merge buffer: acc[8 warps][8 rows][D],
-// then ml[8][8].
+// Leaves the warp's (m, l, acc) in the merge buffer: acc[kWarps][8 rows][D],
+// then ml[kWarps][8].
 template <class C, int D>
 __device__ __forceinline__ void leave(const WarpState<C, D> &s, float *merge) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -452,28 +464,6 @@ struct Join {
   }
 };
 
-// Adds `n` partial results in global memory (part p: ml(p), element i acc(p, i))
-// to a join, as many at a time as fit in 16 registers, so that their loads
-// overlap; in order.
-template <int N, class Ml, class Acc>
-__device__ __forceinline__ void join_parts(Join<N> &j, int n, Ml ml, Acc acc) {
-  constexpr int P = N >= 16 ? 1 : 16 / N;
-  for (int p0 = 0; p0 < n; p0 += P) {
-    float2 m[P];
-    float v[P][N];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const bool have = p0 + p < n;
-      m[p] = have ? __ldcg(ml(p0 + p)) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[p][i] = have ? __ldcg(acc(p0 + p, i)) : 0.f;
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (p0 + p < n) j.add(m[p], [&](int i) { return v[p][i]; });
-  }
-}
-
 // The warps' results of row `row` of an item, joined; thread `sub` of TPR
 // takes elements sub + TPR i.
 template <class C, int D, int N>
@@ -489,11 +479,6 @@ __device__ __forceinline__ void join_warps(Join<N> &j, const float *merge, int r
   }
 }
 
-// Where a CTA stands in the list of all units: item (b, i) and a tile of it.
-struct Walk {
-  int b, i, tile, tiles, len;
-};
-
 template <class C>
 __device__ __forceinline__ int tiles_of(int len) {
   return max(1, (len + C::T - 1) / C::T);
@@ -504,35 +489,27 @@ __device__ __forceinline__ int seq_len(const PagedSeqs &s, int b) {
   return len < 0 || len > s.max_len ? 0 : len;
 }
 
-template <class C>
-__device__ __forceinline__ void walk_on(Walk &w, const PagedSeqs &s, int items) {
-  if (++w.tile < w.tiles) return;
-  w.tile = 0;
-  if (++w.i < items) return;
-  w.i = 0;
-  if (++w.b < s.batch) {
-    w.len = seq_len(s, w.b);
-    w.tiles = tiles_of<C>(w.len);
-  }
-}
-
 template <int CT, int D, int HW, bool A32>
-__global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 1024 ? 2 : 1)
+__global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     paged_decode_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                         uint32_t *__restrict__ err) {
   using C = Cfg<CT, D, HW, A32>;
   extern __shared__ __align__(1024) unsigned char smem[];
-  float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
-  Control &ctl = *reinterpret_cast<Control *>(smem + kStages * C::STAGE + C::MERGE);
+  float *merge = reinterpret_cast<float *>(smem + C::STAGES * C::STAGE);
+  Control &ctl = *reinterpret_cast<Control *>(smem + C::STAGES * C::STAGE + C::MERGE);
   const uint32_t stages = smem_addr(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int items = a.kv_heads * a.head_groups;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], kWarps);
     }
     fence_mbar_init();
+  }
+  if (tid == kThreads) {
+    prefetch_map(&km);
+    prefetch_map(&vm);
   }
 
   // Behind a prefix the kernel before this one is the prefix's, whose results this one does not read and which began
@@ -583,27 +560,36 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
       const int n = tiles * items;
       if (u < n) {
         const int i = u / tiles;
-        ctl.first[0] = b, ctl.first[1] = i, ctl.first[2] = u - i * tiles;
-        ctl.first[3] = tiles, ctl.first[4] = len;
+        ctl.first = {b, i, u - i * tiles, tiles, len};
         break;
       }
       u -= n;
     }
   }
   __syncthreads();
-  Walk cur = {ctl.first[0], ctl.first[1], ctl.first[2], ctl.first[3], ctl.first[4]};
+  Walk cur = ctl.first;
   bool dead = false;
 
   if (warp == kWarps) {  // ---- the loading warp
     int stage = 0;
     uint32_t phase = 1;  // the stages begin empty
+    int next_len = cur.b + 1 < a.seqs.batch ? seq_len(a.seqs, cur.b + 1) : 0;
     for (int u = u0; u < u1; ++u) {
+      const int32_t *table = a.seqs.table + (int64_t)cur.b * a.seqs.table_stride;
+      const TileBoxes box = tile_boxes<C::T>(a.pools, a.box_shift, table, cur.len, cur.tile);  // before the wait
       wait_phase(&ctl.empty[stage], phase, err, dead);
+      if (lane == 0) ctl.at[stage] = cur;
       load_rows<C::T, C::RB, Word<CT>::size>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools,
-                                             a.box_shift, a.seqs.table + (int64_t)cur.b * a.seqs.table_stride, cur.len,
-                                             cur.tile, cur.i / a.head_groups, err);
-      walk_on<C>(cur, a.seqs, items);
-      if (++stage == kStages) stage = 0, phase ^= 1;
+                                             a.box_shift, table, box, cur.tile, cur.i / a.head_groups, err);
+      if (++stage == C::STAGES) stage = 0, phase ^= 1;
+      if (++cur.tile < cur.tiles) continue;
+      cur.tile = 0;
+      if (++cur.i < items) continue;
+      cur.i = 0;
+      ++cur.b;
+      cur.len = next_len;
+      cur.tiles = tiles_of<C>(next_len);
+      if (cur.b + 1 < a.seqs.batch) next_len = seq_len(a.seqs, cur.b + 1);
     }
     pdl_wait();
     return;
@@ -617,22 +603,22 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + hw * 8 + (lane >> 2);
     return gi < a.group ? (int64_t)w.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
   };
-  // item `w` is complete: its output, or behind a prefix its part of it
-  auto finish = [&](const Walk &w, const Join<N> &j) {
-    const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + row;
+  // results of a row of item `w`, elements e, e + step, ...: its output, or behind a prefix its part of it
+  auto put = [&](const Walk &w, int gi, int e, int step, float2 ml, const auto &o) {
+    constexpr int n = sizeof(o) / sizeof(float);
+    const int kvh = w.i / a.head_groups;
     if (gi >= a.group) return;
     if (a.prefix.splits > 0) {
       const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)w.b * a.group + gi) * a.prefix.parts + a.prefix.splits;
 #pragma unroll
-      for (int i = 0; i < N; ++i) a.prefix.acc[at * D + sub + i * TPR] = j.acc[i];
-      if (sub == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
+      for (int i = 0; i < n; ++i) a.prefix.acc[at * D + e + i * step] = o[i];
+      if (e == 0) a.prefix.ml[at] = ml;
       return;
     }
-    const bool none = w.len == 0;
-    const int64_t at = (int64_t)w.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + sub;
+    const int64_t at = (int64_t)w.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + e;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      store_act1(a.out, at + i * TPR, A32 ? TB_F32 : CT, none ? 0.f : __fdiv_rn(j.acc[i], j.l));
+    for (int i = 0; i < n; ++i)
+      store_act1(a.out, at + i * step, A32 ? TB_F32 : CT, w.len == 0 ? 0.f : __fdiv_rn(o[i], ml.y));
   };
   WarpState<C, D> s;
   float qf[C::JD][C::EPC];
@@ -644,24 +630,27 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
   int cut_unit[2] = {-1, -1};  // the item's first unit
   for (int u = u0; u < u1;) {
     const Walk item = cur;
-    const int item0 = u - cur.tile, end = min(u1, item0 + cur.tiles);
+    const int item0 = u - item.tile, end = min(u1, item0 + item.tiles);
     reset(s);
     load_q(s, qf, a.scale2);
     for (; u < end; ++u) {
       wait_phase(&ctl.full[stage], phase, err, dead);
-      warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, cur.len - cur.tile * C::T), kw);
+      warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, item.len - (u - item0) * C::T), kw);
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.empty[stage]);
-      if (++stage == kStages) stage = 0, phase ^= 1;
-      walk_on<C>(cur, a.seqs, items);
+      if (++stage == C::STAGES) stage = 0, phase ^= 1;
     }
-    if (u < u1) fetch_q<C>(qf, a.q, q_at(cur));
+    if (u < u1) {  // the next item's queries arrive during this one's joins
+      wait_phase(&ctl.full[stage], phase, err, dead);
+      cur = ctl.at[stage];
+      fetch_q<C>(qf, a.q, q_at(cur));
+    }
     leave(s, merge);
     computing_warps_sync();
     Join<N> j;
     join_warps<C, D>(j, merge, row, sub);
     if (item0 >= u0 && item0 + item.tiles <= u1) {
-      finish(item, j);
+      put(item, (item.i % a.head_groups) * C::R + row, sub, TPR, make_float2(j.m, j.l), j.acc);
     } else {
       const int k = item0 < u0 ? 0 : 1;
       const int64_t slot = 2 * me + k;
@@ -680,29 +669,47 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     pdl_wait();
     return;
   }
-  if (tid == 0) {
-    __threadfence();  // the whole CTA's partial results, seen by this thread at the barrier above
-    for (int k = 0; k < 2; ++k) {
-      ctl.last[k] = 0;
-      if (cut_unit[k] < 0) continue;
-      const int c0 = owner(cut_unit[k]), c1 = owner(cut_unit[k] + cut[k].tiles - 1);
-      if (atomicAdd(a.counters + c0, 1) == c1 - c0) {
-        ctl.last[k] = 1;
+  if (tid < 2) {  // (the barrier above ordered the CTA's partial results before this)
+    const int unit = tid ? cut_unit[1] : cut_unit[0], tiles = tid ? cut[1].tiles : cut[0].tiles;
+    int last = 0;
+    if (unit >= 0) {
+      const int c0 = owner(unit), parts = owner(unit + tiles - 1) - c0 + 1;
+      if (atom_add_acq_rel(a.counters + c0, 1) == parts - 1) {
         a.counters[c0] = 0;  // ready for the next launch
+        last = parts;
       }
     }
-    __threadfence();
+    ctl.last[tid] = last;
   }
   computing_warps_sync();
+#pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (cut_unit[k] < 0 || !ctl.last[k]) continue;
-    const int c0 = owner(cut_unit[k]), c1 = owner(cut_unit[k] + cut[k].tiles - 1);
-    Join<N> j;
+    const int parts = ctl.last[k];  // 0: not the last
+    if (parts == 0) continue;
+    const int c0 = owner(cut_unit[k]);
     // CTA c's slot: its first item's where the item began before it
-    auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (cut_unit[k] < first_unit(c0 + p) ? 0 : 1)) * C::R + row; };
-    join_parts(j, c1 - c0 + 1, [&](int p) { return a.slot_ml + slot(p); },
-               [&](int p, int i) { return a.slot_acc + slot(p) * D + sub + i * TPR; });
-    finish(cut[k], j);
+    auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (cut_unit[k] < first_unit(c0 + p) ? 0 : 1)) * C::R; };
+    const int hg = cut[k].i % a.head_groups, rows = min(C::R, a.group - hg * C::R);
+    // four elements of a row per thread; eight parts' loads at a time, joined in their order
+    for (int x = tid; x < rows * (D / 4); x += kThreads) {
+      const int r = x / (D / 4), e = x % (D / 4) * 4;
+      Join<4> j;
+      for (int p0 = 0; p0 < parts; p0 += 8) {
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          if (p0 + p >= parts) continue;
+          const int64_t at = slot(p0 + p) + r;
+          ml[p] = __ldcg(a.slot_ml + at);
+          v[p] = __ldcg(reinterpret_cast<const float4 *>(a.slot_acc + at * D + e));
+        }
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p0 + p < parts) j.add(ml[p], [&](int i) { return i == 0 ? v[p].x : i == 1 ? v[p].y : i == 2 ? v[p].z : v[p].w; });
+      }
+      put(cut[k], hg * C::R + r, e, 1, make_float2(j.m, j.l), j.acc);
+    }
   }
   pdl_wait();
 }
@@ -710,17 +717,17 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
 // The prefix: item (split, row tile, key/value head), rows = the queries of all
 // sequences' heads of that key/value head, R of them per CTA.
 template <int CT, int D, int HW, bool A32>
-__global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 1024 ? 2 : 1)
+__global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     paged_prefix_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                         uint32_t *__restrict__ err) {
   using C = Cfg<CT, D, HW, A32>;
   extern __shared__ __align__(1024) unsigned char smem[];
-  float *merge = reinterpret_cast<float *>(smem + kStages * C::STAGE);
-  Control &ctl = *reinterpret_cast<Control *>(smem + kStages * C::STAGE + C::MERGE);
+  float *merge = reinterpret_cast<float *>(smem + C::STAGES * C::STAGE);
+  Control &ctl = *reinterpret_cast<Control *>(smem + C::STAGES * C::STAGE + C::MERGE);
   const uint32_t stages = smem_addr(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], kWarps);
     }
@@ -739,9 +746,10 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     uint32_t phase = 1;
     for (int t = t0; t < t1; ++t) {
       wait_phase(&ctl.empty[stage], phase, err, dead);
-      load_rows<C::T, C::RB, Word<CT>::size>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools,
-                                             a.box_shift, a.prefix_table, a.prefix_len, t, kvh, err);
-      if (++stage == kStages) stage = 0, phase ^= 1;
+      load_rows<C::T, C::RB, Word<CT>::size>(
+          stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift, a.prefix_table,
+          tile_boxes<C::T>(a.pools, a.box_shift, a.prefix_table, a.prefix_len, t), t, kvh, err);
+      if (++stage == C::STAGES) stage = 0, phase ^= 1;
     }
     return;
   }
@@ -762,7 +770,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::SMEM <= 114 * 102
     warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw);
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.empty[stage]);
-    if (++stage == kStages) stage = 0, phase ^= 1;
+    if (++stage == C::STAGES) stage = 0, phase ^= 1;
   }
   leave(s, merge);
   computing_warps_sync();
@@ -816,7 +824,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const AttnArgs a, in
 
 // Warps across query heads: the fewest that take the rows in one item, so that
 // as many warps as possible split the keys (up to 8 rows 1, 16: 2, 32: 4).
-int head_warps(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8; }
+int head_warps(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -886,8 +894,7 @@ tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, c
     switch (head_warps(a.prefix.rows)) {
       case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, cache, st, s, who))); break;
       case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, cache, st, s, who))); break;
-      case 4: TB_TRY((launch_prefix<CT, D, 4, A32>(a, cache, st, s, who))); break;
-      default: TB_TRY((launch_prefix<CT, D, 8, A32>(a, cache, st, s, who))); break;
+      default: TB_TRY((launch_prefix<CT, D, 4, A32>(a, cache, st, s, who))); break;
     }
   }
   const int hw = head_warps(a.group);
@@ -895,8 +902,7 @@ tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, c
   switch (hw) {
     case 1: TB_TRY((launch_decode<CT, D, 1, A32>(a, cache, st, s, who))); break;
     case 2: TB_TRY((launch_decode<CT, D, 2, A32>(a, cache, st, s, who))); break;
-    case 4: TB_TRY((launch_decode<CT, D, 4, A32>(a, cache, st, s, who))); break;
-    default: TB_TRY((launch_decode<CT, D, 8, A32>(a, cache, st, s, who))); break;
+    default: TB_TRY((launch_decode<CT, D, 4, A32>(a, cache, st, s, who))); break;
   }
   if (a.prefix.splits == 0) return TB_OK;
   const int heads = a.kv_heads * a.group;

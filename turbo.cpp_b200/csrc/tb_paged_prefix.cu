@@ -183,6 +183,10 @@ __global__ void __launch_bounds__(kBlock, 1)
     }
     fence_mbar_init();
   }
+  if (tid == 256) {
+    prefetch_map(&km);
+    prefetch_map(&vm);
+  }
   if (warp == 11) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&ctl.tmem))
                  : "memory");
@@ -271,12 +275,13 @@ __global__ void __launch_bounds__(kBlock, 1)
       for (int t = 0; t < n; ++t) {
         const int s = t % C::STAGES;
         const uint32_t ph = ((t / C::STAGES) & 1) ^ 1;
+        const TileBoxes box = tile_boxes<C::KT>(a.pools, a.box_shift, a.prefix_table, a.prefix_len, t0 + t);
         wait_phase(&ctl.kempty[s], ph, err, dead);
         load_rows<C::KT, C::RB, 2>(stages + s * 2 * C::HALF, &ctl.kfull[s], &km, nullptr, a.pools, a.box_shift,
-                                   a.prefix_table, a.prefix_len, t0 + t, kvh, err);
+                                   a.prefix_table, box, t0 + t, kvh, err);
         wait_phase(&ctl.vempty[s], ph, err, dead);
         load_rows<C::KT, C::RB, 2>(stages + s * 2 * C::HALF + C::HALF, &ctl.vfull[s], &vm, nullptr, a.pools,
-                                   a.box_shift, a.prefix_table, a.prefix_len, t0 + t, kvh, err);
+                                   a.box_shift, a.prefix_table, box, t0 + t, kvh, err);
       }
     } else if (warp < 11) {  // ---- products of stream w
       const int w = warp - 9;

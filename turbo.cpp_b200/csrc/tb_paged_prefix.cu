@@ -19,17 +19,20 @@
 // share and is rescaled only where a row's maximum has grown by 2^8.
 //
 // Roles: two streams, each a warpgroup whose threads own one row each (TMEM
-// lane = row), and one warp issuing its MMAs; one warp loading.  While one
-// stream's exponentials run, the other's products do.  With more than 128 rows
-// the streams are two row tiles over the same keys (PAIR), which halves the
-// reads of K and V; else, or where two tiles' queries do not fit, they take
-// alternate key tiles of the same rows and join at the end.
-//   TMEM, per stream: S [KT columns] with P written over it, O [D columns].
-//   Chunk c of 32 keys is read from columns 32 c .. 32 c + 31 before its P is
-//   written: one part to 16 c, two parts to 32 c and 32 c + 16 (three parts,
-//   tiles of 64 keys: the third to 64 + 16 c).
-// The exponentials bound it (16 a cycle and SM: 1024 cycles for 128 x 128,
-// against 512 for the products at head_dim 64 and 1024 at 128).
+// lane = row), and one warp issuing its MMAs; one warp loading.  A stream's
+// scores have two buffers: while the exponentials of one run, the products fill
+// the other.  With more than 128 rows the streams are two row tiles over the
+// same keys (PAIR), which halves the reads of K and V; else, or where two
+// tiles' queries do not fit, they take alternate key tiles of the same rows and
+// join at the end.
+//   TMEM, per stream: S [64 columns, twice] with P written over it, O [D
+//   columns].  Chunk c of 32 keys is read before its P is written: one part to
+//   columns 16 c, two parts to 32 c and 32 c + 16, a third to 64 + 16 c (three
+//   parts at head_dim 128 leave room for one buffer only).
+// Bounds for 64 keys and two row tiles (cycles per SM): exponentials 1024 on the
+// special function units, less what the FMA units take; products 320 at
+// head_dim 64 and 640 at 128 per row tile (Q is read from shared memory at 128
+// bytes a cycle, 1.5 times the tensor cores' own time for S).
 #include <algorithm>
 
 #include "tb_paged.cuh"
@@ -46,6 +49,13 @@ __device__ __forceinline__ void commit_to(uint64_t *bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// One thread of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -108,6 +118,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// 2^x of a pair on the FMA units, so that they share the exponentials with the
+// special function units (a quarter of the FMA rate): x = n + f, n the nearest
+// integer (added to 1.5 2^23, whose low bits then hold it), |f| <= 1/2, 2^f a
+// polynomial, n added to the exponent.  The polynomials are minimax in the
+// relative error (Remez exchange): degree 3 is off by 7.5e-5, far below the
+// rounding of a probability to 16 bits, degree 5 by 7.5e-8 (2e-7 evaluated in
+// fp32).  Below -126 the result is 2^-126.
+template <int DEG>
+__device__ __forceinline__ void exp2_pair(uint64_t x, float &lo, float &hi) {
+  float a, b;
+  unpack2(x, a, b);
+  x = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2(x, pack2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), x);
+  auto c = [](float v) { return pack2(v, v); };
+  uint64_t p;
+  if constexpr (DEG == 3) {
+    p = fma2(c(0.05517166853f), f, c(0.24261112511f));
+    p = fma2(p, f, c(0.69326096773f));
+    p = fma2(p, f, c(0.99992805719f));
+  } else {
+    p = fma2(c(0.00132764725f), f, c(0.00967554096f));
+    p = fma2(p, f, c(0.05550713092f));
+    p = fma2(p, f, c(0.2402212024f));
+    p = fma2(p, f, c(0.69314694404f));
+    p = fma2(p, f, c(1.00000011921f));
+  }
+  float n0, n1, p0, p1;
+  unpack2(t, n0, n1);
+  unpack2(p, p0, p1);
+  lo = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+  hi = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+}
+
 // Shared-memory descriptor, 128-byte swizzle.  K-major (queries, keys): rows of
 // 128 bytes, groups of eight rows 1024 bytes apart.  MN-major (values): the same
 // bytes read as 64 columns of head_dim, groups of eight keys 1024 bytes apart,
@@ -122,8 +166,8 @@ template <int CT_, int D, bool A32>
 struct TC {
   static constexpr int CT = CT_;
   static constexpr int QT = !A32 ? 1 : CT == TB_F16 ? 2 : 3;  // parts of a query and of a probability
-  static constexpr int KT = QT == 3 || QT * D == 256 ? 64 : 128;  // keys per tile: a row's scores, and with fp32
-                                                                  // activations its sums, are one thread's registers
+  static constexpr int KT = 64;                               // keys per tile
+  static constexpr int NB = QT == 3 && D == 128 ? 1 : 2;      // buffers of S
   static constexpr bool SUMS = A32;                           // O summed in registers, tile by tile
   static constexpr bool PAIR_FITS = QT * D <= 192;            // the queries of two row tiles in shared memory
   static constexpr int RB = 2 * D, CB = D / 64;               // bytes and 128-byte columns of a row
@@ -131,13 +175,16 @@ struct TC {
   static constexpr int QBYTES = (PAIR_FITS ? 2 : 1) * QTILE;
   static constexpr int HALF = KT * RB;  // a tile of keys, or of values
   static constexpr int STAGES = (216 * 1024 - QBYTES) / (2 * HALF) < 4 ? (216 * 1024 - QBYTES) / (2 * HALF) : 4;
+  static constexpr int FMA_EIGHTHS = A32 ? 2 : 2;  // of the exponentials, on the FMA units
   static constexpr float SLACK = SUMS ? 0.f : 8.f;  // log2 by which a row may exceed its reference maximum
   static constexpr float PEXP = CT == TB_F16 ? 15.f - SLACK : 0.f;  // probabilities are scaled by 2^PEXP
   static constexpr uint32_t F = CT == TB_BF16 ? 1u : 0u;
   // D fp32, A and B of type F; N, M = 128; the second product's B is MN-major
   static constexpr uint32_t IDESC_QK = (1u << 4) | (F << 7) | (F << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
   static constexpr uint32_t IDESC_PV = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-  static constexpr int O = 128;  // column of a stream's O behind its S
+  static constexpr int BUF = QT == 3 ? 96 : 64;              // columns of a buffer of S and P
+  static constexpr int O = QT == 3 && D == 64 ? 192 : 128;  // column of a stream's O
+  static_assert(NB * BUF <= O && O + D <= 256, "");
   static __device__ __forceinline__ int pcol(int part, int chunk) {
     return QT == 1 ? 16 * chunk : part < 2 ? 32 * chunk + 16 * part : 64 + 16 * chunk;
   }
@@ -145,7 +192,7 @@ struct TC {
 
 struct PrefixControl {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t s_full[2], p_full[2][2], o_full[2];
+  uint64_t s_full[2][2], p_full[2], o_full[2];
   uint32_t tmem;
   float down[2 * kRows];  // fp32 queries of an fp16 cache: 2^-e of each row
 };
@@ -163,7 +210,9 @@ __global__ void __launch_bounds__(kBlock, 1)
   extern __shared__ __align__(1024) unsigned char smem[];
   PrefixControl &ctl = *reinterpret_cast<PrefixControl *>(smem + C::QBYTES + C::STAGES * 2 * C::HALF);
   const uint32_t qs = smem_addr(smem), stages = qs + C::QBYTES;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (the warp's number by a shuffle: known to be the same in all lanes, what follows from it stays in uniform registers,
+  // which the tensor core's operands come from)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int split = blockIdx.x, kvh = blockIdx.z;
   const int all = (a.prefix_len + C::KT - 1) / C::KT;
   const int t0 = (int)((int64_t)split * all / a.prefix.splits);
@@ -176,9 +225,9 @@ __global__ void __launch_bounds__(kBlock, 1)
       mbar_init(&ctl.vempty[i], pair ? 2 : 1);
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&ctl.s_full[w], 1);
-      mbar_init(&ctl.p_full[w][0], kRows);
-      mbar_init(&ctl.p_full[w][1], kRows);
+      mbar_init(&ctl.s_full[w][0], 1);
+      mbar_init(&ctl.s_full[w][1], 1);
+      mbar_init(&ctl.p_full[w], kRows);
       mbar_init(&ctl.o_full[w], 1);
     }
     fence_mbar_init();
@@ -267,7 +316,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   const uint32_t tmem = ctl.tmem;
   bool dead = false;
 
-  // a stream's tiles: first, first + step, ... below n
+  // tile j of a stream w is tile first + j * step of the CTA's n
   const int step = pair ? 1 : 2;
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -284,30 +333,33 @@ __global__ void __launch_bounds__(kBlock, 1)
                                    a.box_shift, a.prefix_table, box, t0 + t, kvh, err);
       }
     } else if (warp < 11) {  // ---- products of stream w
-      const int w = warp - 9;
+      const int w = warp - 9, first = pair ? 0 : w, mine = (n - first + step - 1) / step;
       const uint32_t ts = tmem + w * 256, q = qs + (pair ? w * C::QTILE : 0);
-      uint32_t ph = 0;
-      for (int t = pair ? 0 : w; t < n; t += step, ph ^= 1) {
-        const int s = t % C::STAGES;
-        const uint32_t full = (t / C::STAGES) & 1;
-        const uint32_t k = stages + s * 2 * C::HALF, v = k + C::HALF;
-        const int keys = min(C::KT, a.prefix_len - (t0 + t) * C::KT);
-        const bool later = t >= step;  // not the stream's first tile: O is added to, where it stays in TMEM
-        wait_phase(&ctl.kfull[s], full, err, dead);
+      const uint64_t qd = desc(q, 16);
+      auto scores = [&](int j) {
+        const int t = first + j * step, s = t % C::STAGES;
+        const uint32_t k = stages + s * 2 * C::HALF, to = ts + (j % C::NB) * C::BUF;
+        const uint64_t kd = desc(k, 16);  // 16 elements further: 32 bytes, 2 in the descriptor's address field
+        wait_phase(&ctl.kfull[s], (t / C::STAGES) & 1, err, dead);
         fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
 #pragma unroll
           for (int p = 0; p < C::QT; ++p)
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
-              mma_ss(ts, desc(q + (p * C::CB + i / 4) * kRows * 128 + (i % 4) * 32, 16),
-                     desc(k + (i / 4) * C::KT * 128 + (i % 4) * 32, 16), C::IDESC_QK, p + i > 0);
-          commit_to(&ctl.s_full[w]);
+              mma_ss(to, qd + ((p * C::CB + i / 4) * kRows * 8 + (i % 4) * 2), kd + ((i / 4) * C::KT * 8 + (i % 4) * 2),
+                     C::IDESC_QK, p + i > 0);
+          commit_to(&ctl.s_full[w][j % C::NB]);
           commit_to(&ctl.kempty[s]);
         }
         __syncwarp();
-        wait_phase(&ctl.vfull[s], full, err, dead);
-        const int steps = (keys + 15) / 16;
+      };
+      for (int j = 0; j < min(C::NB, mine); ++j) scores(j);
+      for (int j = 0; j < mine; ++j) {
+        const int t = first + j * step, s = t % C::STAGES;
+        const uint32_t v = stages + s * 2 * C::HALF + C::HALF, p0 = ts + (j % C::NB) * C::BUF;
+        const int keys = min(C::KT, a.prefix_len - (t0 + t) * C::KT), steps = (keys + 15) / 16;
+        wait_phase(&ctl.vfull[s], (t / C::STAGES) & 1, err, dead);
         if (keys < steps * 16) {
           // the rows of the last step behind the prefix hold whatever their page held: 0 times that has to be 0
           for (int i = lane; i < (steps * 16 - keys) * (C::RB / 16); i += 32) {
@@ -317,24 +369,24 @@ __global__ void __launch_bounds__(kBlock, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        // P arrives in two halves, so that the first one's products run during the second's exponentials
-        for (int h = 0; h < 2; ++h) {
-          wait_phase(&ctl.p_full[w][h], ph, err, dead);
-          fence_after();
-          if (lane == 0) {
-            for (int i = h * (C::KT / 32); i < min(steps, (h + 1) * (C::KT / 32)); ++i)
+        wait_phase(&ctl.p_full[w], j & 1, err, dead);
+        fence_after();
+        const uint64_t vd = desc(v, C::KT * 128);  // 16 keys further: 2048 bytes
+        if (elect_one()) {
 #pragma unroll
-              for (int p = 0; p < C::QT; ++p)
-                mma_ts(ts + C::O, ts + C::pcol(p, i / 2) + 8 * (i % 2), desc(v + i * 2048, C::KT * 128), C::IDESC_PV,
-                       p + i > 0 || (!C::SUMS && later));
+          for (int i = 0; i < C::KT / 16; ++i) {
+            if (i >= steps) break;
+#pragma unroll
+            for (int p = 0; p < C::QT; ++p)
+              mma_ts(ts + C::O, p0 + C::pcol(p, i / 2) + 8 * (i % 2), vd + i * 128, C::IDESC_PV,
+                     p + i > 0 || (!C::SUMS && j > 0));
           }
-          __syncwarp();
-        }
-        if (lane == 0) {
           commit_to(&ctl.vempty[s]);
-          if (t + step >= n) commit_to(&ctl.o_full[w]);
+          commit_to(&ctl.o_full[w]);
         }
         __syncwarp();
+        // into the buffer whose P the products just issued read: the tensor core takes them in order
+        if (j + C::NB < mine) scores(j + C::NB);
       }
     }
   } else {  // ---- the exponentials of stream `stream`
@@ -343,12 +395,12 @@ __global__ void __launch_bounds__(kBlock, 1)
     float scale2 = fabsf(a.scale2);
     if (A32 && CT == TB_F16) scale2 *= ctl.down[(pair ? stream * kRows : 0) + r];
     uint64_t acc[C::SUMS ? D / 2 : 1];  // pairs of columns
-    float m = -INFINITY, l = 0.f, alpha = 1.f;
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < (C::SUMS ? D / 2 : 1); ++i) acc[i] = 0ull;
     // SUMS: adds a finished tile's O to the running sum
-    auto take_o = [&]() {
-      const uint64_t al = pack2(alpha, alpha);
+    auto take_o = [&](float f) {
+      const uint64_t al = pack2(f, f);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -374,19 +426,19 @@ __global__ void __launch_bounds__(kBlock, 1)
         tmem_st32(ts + C::O + 32 * c, o);
       }
     };
-    uint32_t ph = 0;
-    const int first = pair ? 0 : stream;
-    for (int t = first; t < n; t += step, ph ^= 1) {
-      wait_phase(&ctl.s_full[stream], ph, err, dead);  // this S, and with it the products before it: the last O
+    const int first = pair ? 0 : stream, mine = (n - first + step - 1) / step;
+    float before = 1.f;  // SUMS: the factor that the sums before the last tile's O still need
+    for (int j = 0; j < mine; ++j) {
+      const uint32_t sp = ts + (j % C::NB) * C::BUF;
+      wait_phase(&ctl.s_full[stream][j % C::NB], (j / C::NB) & 1, err, dead);
       fence_after();
-      if (C::SUMS && t > first) take_o();
-      uint32_t u[C::KT / 32][32];  // the row's scores, then its probabilities
+      uint32_t u[C::KT / 32][32];  // the row's scores
 #pragma unroll
-      for (int c = 0; c < C::KT / 32; ++c) tmem_ld32(ts + 32 * c, u[c]);
+      for (int c = 0; c < C::KT / 32; ++c) tmem_ld32(sp + 32 * c, u[c]);
       tmem_wait_ld();
 #pragma unroll
       for (int c = 0; c < C::KT / 32; ++c) loaded(u[c]);
-      const int keys = a.prefix_len - (t0 + t) * C::KT;  // KT or more except in the last tile
+      const int keys = a.prefix_len - (t0 + first + j * step) * C::KT;  // KT or more except in the last tile
       if (keys < C::KT) {
 #pragma unroll
         for (int c = 0; c < C::KT / 32; ++c)
@@ -401,17 +453,20 @@ __global__ void __launch_bounds__(kBlock, 1)
         for (int i = 0; i < 32; i += 2)
           mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(u[c][i]), __uint_as_float(u[c][i + 1]));
       const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2);
+      float alpha = 1.f;
       if constexpr (C::SUMS) {
         alpha = ex2(m - (top == -INFINITY ? 0.f : top));
         l *= alpha;
         m = top;
-      } else if (t == first) {
+      } else if (j == 0) {
         m = top;
       } else {
         // the reference maximum follows only where a row has outgrown it by 2^SLACK; its O and l are then scaled down
         const bool grown = top > m + C::SLACK;
         if (__any_sync(0xffffffffu, grown)) {
           const float f = grown ? ex2(m - top) : 1.f;
+          wait_phase(&ctl.o_full[stream], (j - 1) & 1, err, dead);
+          fence_after();
           scale_o(f);
           l *= f;
           if (grown) m = top;
@@ -426,9 +481,13 @@ __global__ void __launch_bounds__(kBlock, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint64_t x = fma2(pack2(__uint_as_float(u[c][2 * i]), __uint_as_float(u[c][2 * i + 1])), scale, shift);
-          unpack2(x, p[2 * i], p[2 * i + 1]);
-          p[2 * i] = ex2(p[2 * i]);
-          p[2 * i + 1] = ex2(p[2 * i + 1]);
+          if (i * C::FMA_EIGHTHS % 8 < C::FMA_EIGHTHS) {
+            exp2_pair<A32 ? 5 : 3>(x, p[2 * i], p[2 * i + 1]);
+          } else {
+            unpack2(x, p[2 * i], p[2 * i + 1]);
+            p[2 * i] = ex2(p[2 * i]);
+            p[2 * i + 1] = ex2(p[2 * i + 1]);
+          }
           sum[i & 1] = add2(sum[i & 1], pack2(p[2 * i], p[2 * i + 1]));
         }
 #pragma unroll
@@ -436,26 +495,30 @@ __global__ void __launch_bounds__(kBlock, 1)
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) w[i] = pack_rest<CT>(p[2 * i], p[2 * i + 1]);
-          tmem_st16(ts + C::pcol(k, c), w);
-        }
-        if (c == C::KT / 64 - 1 || c == C::KT / 32 - 1) {
-          tmem_wait_st();
-          fence_before();
-          mbar_arrive(&ctl.p_full[stream][c == C::KT / 32 - 1]);
+          tmem_st16(sp + C::pcol(k, c), w);
         }
       }
       float s0, s1;
       unpack2(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
+      if (C::SUMS && j > 0) {  // the last tile's O, before the next products overwrite it
+        wait_phase(&ctl.o_full[stream], (j - 1) & 1, err, dead);
+        fence_after();
+        take_o(before);
+      }
+      before = alpha;
+      tmem_wait_st();
+      fence_before();
+      mbar_arrive(&ctl.p_full[stream]);
     }
     float out[D];
 #pragma unroll
     for (int i = 0; i < D; ++i) out[i] = 0.f;
-    if (first < n) {
-      wait_phase(&ctl.o_full[stream], 0, err, dead);
+    if (mine > 0) {
+      wait_phase(&ctl.o_full[stream], (mine - 1) & 1, err, dead);
       fence_after();
       if constexpr (C::SUMS) {
-        take_o();
+        take_o(before);
 #pragma unroll
         for (int i = 0; i < D / 2; ++i) unpack2(acc[i], out[2 * i], out[2 * i + 1]);
       } else {

@@ -460,6 +460,15 @@ SHARED = [
     ("bf16", "bf16", 4, 8, 128, 64, "head", [1, 2, 300] * 11, 9000),
     ("f32", "f16", 2, 1, 128, 32, "head", [3] * 300, 515),
     ("f32", "f32", 1, 1, 64, 16, "token", [2], 50000),
+    # many key tiles per CTA, one row tile and two, every number of operand parts
+    ("bf16", "bf16", 4, 8, 64, 64, "head", [b % 3 for b in range(17)], 30011),
+    ("bf16", "bf16", 4, 8, 128, 64, "head", [b % 3 for b in range(33)], 20003),
+    ("f16", "f16", 4, 8, 128, 16, "token", [b % 3 for b in range(64)], 20000),
+    ("f16", "f16", 8, 8, 64, 16, "token", [b % 3 for b in range(40)], 20001),
+    ("f32", "f16", 4, 8, 64, 16, "token", [b % 3 for b in range(20)], 15000),
+    ("f32", "f16", 4, 8, 128, 16, "token", [b % 3 for b in range(40)], 15000),
+    ("f32", "bf16", 4, 8, 64, 16, "token", [b % 3 for b in range(70)], 15000),
+    ("f32", "bf16", 4, 8, 128, 16, "token", [b % 3 for b in range(20)], 15000),
 ]
 
 

@@ -52,6 +52,7 @@ struct PrefixParts {
   int rows;    // batch * group
   int splits;  // 0: no prefix
   int parts;   // splits + 1
+  int join_here;  // the kernel of the sequences' own keys joins the parts
 };
 
 // The pools as 4-d tensors [page][token][head][head_dim] for TMA: a box is up
@@ -281,8 +282,8 @@ tb_status launch_pdl(F *kern, dim3 grid, int threads, size_t smem, cudaStream_t 
   return check_launch(who);
 }
 
-// The prefix on tcgen05 (tb_paged_prefix.cu), 16-bit caches; sets a.prefix.splits.
-tb_status launch_prefix_tc(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
-                           const char *who);
+// The prefix on tcgen05 (tb_paged_prefix.cu), 16-bit caches; sets a.prefix.splits.  The maps' boxes are those of 64 keys.
+tb_status launch_prefix_tc(AttnArgs &a, const PagedMaps &maps, int cache_dtype, int head_dim, const DeviceState *st,
+                           cudaStream_t s, const char *who);
 
 }  // namespace tb

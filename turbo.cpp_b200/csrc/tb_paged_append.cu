@@ -15,6 +15,7 @@
 // ballot, then one table entry.  The data loads do not depend on that chain and
 // are issued before it.
 #include <algorithm>
+#include <atomic>
 
 #include "tb_paged.cuh"
 
@@ -240,6 +241,18 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
   }
 }
 
+// wave_grid for CTAs of 256 threads, the CTAs per SM found once per kernel and device.
+template <auto KERN>
+int wave_grid_of(int64_t threads, const DeviceState *st) {
+  static std::atomic<int> known[64];
+  int n = known[st->device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = resident_ctas(reinterpret_cast<const void *>(KERN), 256, 0);
+    known[st->device].store(n, std::memory_order_relaxed);
+  }
+  return (int)std::min<int64_t>((threads + 255) / 256, (int64_t)st->sm_count * n);
+}
+
 }  // namespace
 }  // namespace tb
 
@@ -296,10 +309,10 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
   cudaStream_t s = as_stream(stream);
 #define TB_APPEND_U(ACT, CT, U)                                                        \
   do {                                                                                 \
-    auto kern = paged_append_kernel<ACT, CT, U>;                                       \
     a.per_token = (int)((groups + U - 1) / U);                                         \
     const int64_t threads = tokens * a.per_token * 32;                                 \
-    kern<<<wave_grid(kern, 256, threads, st->sm_count), 256, 0, s>>>(a, st->err_word); \
+    paged_append_kernel<ACT, CT, U>                                                    \
+        <<<wave_grid_of<paged_append_kernel<ACT, CT, U>>(threads, st), 256, 0, s>>>(a, st->err_word); \
     return check_launch("tb_rope_paged_append");                                       \
   } while (0)
 #define TB_APPEND(ACT, CT)               \

@@ -41,8 +41,10 @@
 // partial results in the workspace; the last of its CTAs to finish (a counter
 // per first CTA, reset by that CTA) joins them.  Behind a prefix there are three
 // kernels: the prefix's (here, or tb_paged_prefix.cu for many rows), this one
-// for the sequences' own keys, and one that joins the parts of each row.
+// for the sequences' own keys, and one that joins the parts of each row; where
+// every item has a CTA of its own this one joins them itself.
 #include <algorithm>
+#include <atomic>
 
 #include "tb_paged.cuh"
 
@@ -54,6 +56,7 @@ constexpr int64_t kPrefixRows = 2 * 148 * 128;   // extra (row, split) pairs of 
 constexpr int kWarps = 4;              // computing warps
 constexpr int kThreads = kWarps * 32;  // their threads
 constexpr int kBlock = kThreads + 32;  // and one warp that loads
+constexpr int kJoinSplits = 16;       // splits of a prefix up to which the decode kernel may join them
 constexpr int kTensorRows = 64;       // query rows of a key/value head from which the prefix runs on tcgen05
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -489,7 +492,9 @@ __device__ __forceinline__ int seq_len(const PagedSeqs &s, int b) {
   return len < 0 || len > s.max_len ? 0 : len;
 }
 
-template <int CT, int D, int HW, bool A32>
+// JOIN: it joins a prefix's parts itself (a variant, since the code for it costs the others registers: 128 ragged
+// sequences 356 us with it, 322 without).
+template <int CT, int D, int HW, bool A32, bool JOIN>
 __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     paged_decode_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                         uint32_t *__restrict__ err) {
@@ -603,22 +608,42 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     const int kvh = w.i / a.head_groups, gi = (w.i - kvh * a.head_groups) * C::R + hw * 8 + (lane >> 2);
     return gi < a.group ? (int64_t)w.b * a.q.ld + (int64_t)(kvh * a.group + gi) * D : -1;
   };
-  // results of a row of item `w`, elements e, e + step, ...: its output, or behind a prefix its part of it
-  auto put = [&](const Walk &w, int gi, int e, int step, float2 ml, const auto &o) {
-    constexpr int n = sizeof(o) / sizeof(float);
+  // results of a row of item `w`, elements e, e + step, ...: its output, joined with the prefix's parts first, or its
+  // part of it
+  auto put = [&](const Walk &w, int gi, int e, int step, auto &j) {
+    constexpr int n = sizeof(j.acc) / sizeof(float);
     const int kvh = w.i / a.head_groups;
+    if constexpr (JOIN) pdl_wait();
     if (gi >= a.group) return;
-    if (a.prefix.splits > 0) {
-      const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)w.b * a.group + gi) * a.prefix.parts + a.prefix.splits;
+    const int64_t at_parts = ((int64_t)kvh * a.prefix.rows + (int64_t)w.b * a.group + gi) * a.prefix.parts;
+    if constexpr (JOIN) {
+      constexpr int P = n >= 16 ? 2 : 32 / n;
+      for (int p0 = 0; p0 < a.prefix.splits; p0 += P) {
+        float2 ml[P];
+        float v[P][n];
 #pragma unroll
-      for (int i = 0; i < n; ++i) a.prefix.acc[at * D + e + i * step] = o[i];
-      if (e == 0) a.prefix.ml[at] = ml;
+        for (int p = 0; p < P; ++p) {
+          if (p0 + p >= a.prefix.splits) continue;
+          ml[p] = __ldcg(a.prefix.ml + at_parts + p0 + p);
+#pragma unroll
+          for (int i = 0; i < n; ++i) v[p][i] = __ldcg(a.prefix.acc + (at_parts + p0 + p) * D + e + i * step);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          if (p0 + p < a.prefix.splits) j.add(ml[p], [&](int i) { return v[p][i]; });
+      }
+    } else if (a.prefix.splits > 0) {
+      const int64_t at = at_parts + a.prefix.splits;
+#pragma unroll
+      for (int i = 0; i < n; ++i) a.prefix.acc[at * D + e + i * step] = j.acc[i];
+      if (e == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
       return;
     }
+    const bool none = w.len == 0 && a.prefix.splits == 0;
     const int64_t at = (int64_t)w.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + e;
 #pragma unroll
     for (int i = 0; i < n; ++i)
-      store_act1(a.out, at + i * step, A32 ? TB_F32 : CT, w.len == 0 ? 0.f : __fdiv_rn(o[i], ml.y));
+      store_act1(a.out, at + i * step, A32 ? TB_F32 : CT, none ? 0.f : __fdiv_rn(j.acc[i], j.l));
   };
   WarpState<C, D> s;
   float qf[C::JD][C::EPC];
@@ -650,7 +675,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     Join<N> j;
     join_warps<C, D>(j, merge, row, sub);
     if (item0 >= u0 && item0 + item.tiles <= u1) {
-      put(item, (item.i % a.head_groups) * C::R + row, sub, TPR, make_float2(j.m, j.l), j.acc);
+      put(item, (item.i % a.head_groups) * C::R + row, sub, TPR, j);
     } else {
       const int k = item0 < u0 ? 0 : 1;
       const int64_t slot = 2 * me + k;
@@ -708,7 +733,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
         for (int p = 0; p < 8; ++p)
           if (p0 + p < parts) j.add(ml[p], [&](int i) { return i == 0 ? v[p].x : i == 1 ? v[p].y : i == 2 ? v[p].z : v[p].w; });
       }
-      put(cut[k], hg * C::R + r, e, 1, make_float2(j.m, j.l), j.acc);
+      put(cut[k], hg * C::R + r, e, 1, j);
     }
   }
   pdl_wait();
@@ -843,39 +868,42 @@ Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   return l;
 }
 
-template <class C>
-tb_status tile_maps(AttnArgs &a, const tb_paged_cache *cache, const char *who, PagedMaps *maps) {
-  int rows;
-  tb_paged_cache c = *cache;
-  if (c.n_pages == 0) c.n_pages = 1, c.k = c.v = a.counters;  // an empty pool: every page id is outside it
-  TB_TRY(paged_maps(&c, C::T, who, maps, &rows));
-  a.box_shift = 0;
-  while ((1 << a.box_shift) < rows) ++a.box_shift;
+// CTAs of a kernel in one wave of the current device, its shared memory limit raised; found once per device.
+template <class C, auto KERN>
+tb_status wave_of(const DeviceState *st, int *ctas) {
+  static std::atomic<int> known[64];
+  int n = known[st->device].load(std::memory_order_acquire);
+  if (n == 0) {
+    TB_TRY(ensure_smem_for(KERN, C::SMEM));
+    n = st->sm_count * resident_ctas(reinterpret_cast<const void *>(KERN), kBlock, C::SMEM);
+    known[st->device].store(n, std::memory_order_release);
+  }
+  *ctas = n;
   return TB_OK;
 }
 
 template <int CT, int D, int HW, bool A32>
-tb_status launch_decode(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
-                        const char *who) {
+tb_status launch_decode(AttnArgs &a, const PagedMaps &maps, const DeviceState *st, cudaStream_t s, const char *who) {
   using C = Cfg<CT, D, HW, A32>;
-  auto kern = paged_decode_kernel<CT, D, HW, A32>;
-  TB_TRY(ensure_smem_for(kern, C::SMEM));
-  PagedMaps maps;
-  TB_TRY(tile_maps<C>(a, cache, who, &maps));
-  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kBlock, C::SMEM);
+  int ctas;
+  TB_TRY((wave_of<C, paged_decode_kernel<CT, D, HW, A32, false>>(st, &ctas)));
   a.max_ctas = std::min(ctas, kMaxCtas);
-  return launch_pdl(kern, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a, maps.k, maps.v, st->err_word);
+  a.prefix.join_here = a.prefix.splits > 0 && a.prefix.splits <= kJoinSplits && (int64_t)a.seqs.batch * a.kv_heads * a.head_groups <= a.max_ctas;
+  if (a.prefix.join_here) {
+    TB_TRY((wave_of<C, paged_decode_kernel<CT, D, HW, A32, true>>(st, &ctas)));
+    a.max_ctas = std::min(ctas, kMaxCtas);
+    return launch_pdl(paged_decode_kernel<CT, D, HW, A32, true>, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a,
+                      maps.k, maps.v, st->err_word);
+  }
+  return launch_pdl(paged_decode_kernel<CT, D, HW, A32, false>, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a, maps.k, maps.v, st->err_word);
 }
 
 template <int CT, int D, int HW, bool A32>
-tb_status launch_prefix(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
-                        const char *who) {
+tb_status launch_prefix(AttnArgs &a, const PagedMaps &maps, const DeviceState *st, cudaStream_t s, const char *who) {
   using C = Cfg<CT, D, HW, A32>;
-  auto kern = paged_prefix_kernel<CT, D, HW, A32>;
-  TB_TRY(ensure_smem_for(kern, C::SMEM));
-  PagedMaps maps;
-  TB_TRY(tile_maps<C>(a, cache, who, &maps));
-  const int ctas = st->sm_count * resident_ctas(reinterpret_cast<const void *>(kern), kBlock, C::SMEM);
+  constexpr auto kern = paged_prefix_kernel<CT, D, HW, A32>;
+  int ctas;
+  TB_TRY((wave_of<C, paged_prefix_kernel<CT, D, HW, A32>>(st, &ctas)));
   const int row_tiles = (a.prefix.rows + C::R - 1) / C::R;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
@@ -888,23 +916,32 @@ tb_status launch_prefix(AttnArgs &a, const tb_paged_cache *cache, const DeviceSt
 
 template <int CT, int D, bool A32>
 tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s, const char *who) {
+  // every kernel here takes tiles of as many keys (one warp's 16 and more; 8 of 512 bytes)
+  constexpr int T = Cfg<CT, D, 1, A32>::T;
+  PagedMaps maps;
+  int box;
+  tb_paged_cache c = *cache;
+  if (c.n_pages == 0) c.n_pages = 1, c.k = c.v = a.counters;  // an empty pool: every page id is outside it
+  TB_TRY(paged_maps(&c, T, who, &maps, &box));
+  a.box_shift = 0;
+  while ((1 << a.box_shift) < box) ++a.box_shift;
   if (CT != TB_F32 && a.prefix_len > 0 && a.prefix.rows >= kTensorRows) {
-    TB_TRY(launch_prefix_tc(a, cache, st, s, who));
+    TB_TRY(launch_prefix_tc(a, maps, CT, D, st, s, who));
   } else if (a.prefix_len > 0) {
     switch (head_warps(a.prefix.rows)) {
-      case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, cache, st, s, who))); break;
-      case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, cache, st, s, who))); break;
-      default: TB_TRY((launch_prefix<CT, D, 4, A32>(a, cache, st, s, who))); break;
+      case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, maps, st, s, who))); break;
+      case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, maps, st, s, who))); break;
+      default: TB_TRY((launch_prefix<CT, D, 4, A32>(a, maps, st, s, who))); break;
     }
   }
   const int hw = head_warps(a.group);
   a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
   switch (hw) {
-    case 1: TB_TRY((launch_decode<CT, D, 1, A32>(a, cache, st, s, who))); break;
-    case 2: TB_TRY((launch_decode<CT, D, 2, A32>(a, cache, st, s, who))); break;
-    default: TB_TRY((launch_decode<CT, D, 4, A32>(a, cache, st, s, who))); break;
+    case 1: TB_TRY((launch_decode<CT, D, 1, A32>(a, maps, st, s, who))); break;
+    case 2: TB_TRY((launch_decode<CT, D, 2, A32>(a, maps, st, s, who))); break;
+    default: TB_TRY((launch_decode<CT, D, 4, A32>(a, maps, st, s, who))); break;
   }
-  if (a.prefix.splits == 0) return TB_OK;
+  if (a.prefix.splits == 0 || a.prefix.join_here) return TB_OK;
   const int heads = a.kv_heads * a.group;
   return launch_pdl(paged_combine_kernel<D>, dim3((unsigned)(((int64_t)a.seqs.batch * heads + 7) / 8)), 256, 0, s, who,
                     a, heads);

@@ -174,7 +174,7 @@ struct TC {
   static constexpr int QTILE = QT * CB * kRows * 128;
   static constexpr int QBYTES = (PAIR_FITS ? 2 : 1) * QTILE;
   static constexpr int HALF = KT * RB;  // a tile of keys, or of values
-  static constexpr int STAGES = (216 * 1024 - QBYTES) / (2 * HALF) < 4 ? (216 * 1024 - QBYTES) / (2 * HALF) : 4;
+  static constexpr int STAGES = 4;      // even, so that with alternate tiles a stage is always the same stream's
   static constexpr int FMA_EIGHTHS = A32 ? 2 : 2;  // of the exponentials, on the FMA units
   static constexpr float SLACK = SUMS ? 0.f : 8.f;  // log2 by which a row may exceed its reference maximum
   static constexpr float PEXP = CT == TB_F16 ? 15.f - SLACK : 0.f;  // probabilities are scaled by 2^PEXP
@@ -192,7 +192,9 @@ struct TC {
 
 struct PrefixControl {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t s_full[2][2], p_full[2], o_full[2];
+  // per stream and buffer of S (a barrier then never runs a whole phase ahead of a waiter that skips one: tile j's
+  // scores imply the products of tile j - NB)
+  uint64_t s_full[2][2], p_full[2][2], o_full[2][2];
   uint32_t tmem;
   float down[2 * kRows];  // fp32 queries of an fp16 cache: 2^-e of each row
 };
@@ -227,8 +229,10 @@ __global__ void __launch_bounds__(kBlock, 1)
     for (int w = 0; w < 2; ++w) {
       mbar_init(&ctl.s_full[w][0], 1);
       mbar_init(&ctl.s_full[w][1], 1);
-      mbar_init(&ctl.p_full[w], kRows);
-      mbar_init(&ctl.o_full[w], 1);
+      mbar_init(&ctl.p_full[w][0], kRows);
+      mbar_init(&ctl.p_full[w][1], kRows);
+      mbar_init(&ctl.o_full[w][0], 1);
+      mbar_init(&ctl.o_full[w][1], 1);
     }
     fence_mbar_init();
   }
@@ -369,7 +373,7 @@ __global__ void __launch_bounds__(kBlock, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        wait_phase(&ctl.p_full[w], j & 1, err, dead);
+        wait_phase(&ctl.p_full[w][j % C::NB], (j / C::NB) & 1, err, dead);
         fence_after();
         const uint64_t vd = desc(v, C::KT * 128);  // 16 keys further: 2048 bytes
         if (elect_one()) {
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kBlock, 1)
                      p + i > 0 || (!C::SUMS && j > 0));
           }
           commit_to(&ctl.vempty[s]);
-          commit_to(&ctl.o_full[w]);
+          commit_to(&ctl.o_full[w][j % C::NB]);
         }
         __syncwarp();
         // into the buffer whose P the products just issued read: the tensor core takes them in order
@@ -427,6 +431,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       }
     };
     const int first = pair ? 0 : stream, mine = (n - first + step - 1) / step;
+    auto wait_o = [&](int j) { wait_phase(&ctl.o_full[stream][j % C::NB], (j / C::NB) & 1, err, dead); };
     float before = 1.f;  // SUMS: the factor that the sums before the last tile's O still need
     for (int j = 0; j < mine; ++j) {
       const uint32_t sp = ts + (j % C::NB) * C::BUF;
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         const bool grown = top > m + C::SLACK;
         if (__any_sync(0xffffffffu, grown)) {
           const float f = grown ? ex2(m - top) : 1.f;
-          wait_phase(&ctl.o_full[stream], (j - 1) & 1, err, dead);
+          wait_o(j - 1);
           fence_after();
           scale_o(f);
           l *= f;
@@ -502,20 +507,20 @@ __global__ void __launch_bounds__(kBlock, 1)
       unpack2(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
       if (C::SUMS && j > 0) {  // the last tile's O, before the next products overwrite it
-        wait_phase(&ctl.o_full[stream], (j - 1) & 1, err, dead);
+        wait_o(j - 1);
         fence_after();
         take_o(before);
       }
       before = alpha;
       tmem_wait_st();
       fence_before();
-      mbar_arrive(&ctl.p_full[stream]);
+      mbar_arrive(&ctl.p_full[stream][j % C::NB]);
     }
     float out[D];
 #pragma unroll
     for (int i = 0; i < D; ++i) out[i] = 0.f;
     if (mine > 0) {
-      wait_phase(&ctl.o_full[stream], (mine - 1) & 1, err, dead);
+      wait_o(mine - 1);
       fence_after();
       if constexpr (C::SUMS) {
         take_o(before);
@@ -591,19 +596,12 @@ __global__ void __launch_bounds__(kBlock, 1)
 }
 
 template <int CT, int D, bool A32>
-tb_status launch(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s, const char *who) {
+tb_status launch(AttnArgs &a, const PagedMaps &maps, const DeviceState *st, cudaStream_t s, const char *who) {
   using C = TC<CT, D, A32>;
   auto kern = paged_prefix_tc_kernel<CT, D, A32>;
   constexpr int smem = prefix_smem<C>();
-  static_assert(smem <= 227 * 1024 && C::STAGES >= 2 && C::STAGES * 2 * C::HALF >= (D + 2) * kRows * 4, "");
+  static_assert(smem <= 227 * 1024 && C::STAGES * 2 * C::HALF >= (D + 2) * kRows * 4, "");
   TB_TRY(ensure_smem_for(kern, smem));
-  PagedMaps maps;
-  int box;
-  tb_paged_cache c = *cache;
-  if (c.n_pages == 0) c.n_pages = 1, c.k = c.v = a.counters;  // an empty pool: every page id is outside it
-  TB_TRY(paged_maps(&c, C::KT, who, &maps, &box));
-  a.box_shift = 0;
-  while ((1 << a.box_shift) < box) ++a.box_shift;
   const int pair = C::PAIR_FITS && a.prefix.rows > kRows;
   const int rows = pair ? 2 * kRows : kRows;
   const int row_tiles = (a.prefix.rows + rows - 1) / rows;
@@ -617,12 +615,12 @@ tb_status launch(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st
 
 }  // namespace
 
-tb_status launch_prefix_tc(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, cudaStream_t s,
-                           const char *who) {
-  const bool wide = cache->head_dim == 128, a32 = a.q.dtype == TB_F32;
+tb_status launch_prefix_tc(AttnArgs &a, const PagedMaps &maps, int cache_dtype, int head_dim, const DeviceState *st,
+                           cudaStream_t s, const char *who) {
+  const bool wide = head_dim == 128, a32 = a.q.dtype == TB_F32;
 #define TB_PREFIX(CT, A32) \
-  return wide ? launch<CT, 128, A32>(a, cache, st, s, who) : launch<CT, 64, A32>(a, cache, st, s, who)
-  if (cache->dtype == TB_F16) {
+  return wide ? launch<CT, 128, A32>(a, maps, st, s, who) : launch<CT, 64, A32>(a, maps, st, s, who)
+  if (cache_dtype == TB_F16) {
     if (a32) TB_PREFIX(TB_F16, true);
     TB_PREFIX(TB_F16, false);
   }

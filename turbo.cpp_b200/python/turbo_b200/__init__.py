@@ -170,25 +170,52 @@ def check(status, what=""):
         raise TbError(status, (what + ": " if what else "") + msg)
 
 
+_FN = {}
+
+
 def call(name, *args):
-    check(getattr(load(), name)(*args), name)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(load(), name)
+    status = fn(*args)
+    if status != OK:
+        check(status, name)
 
 
 # ---- torch helpers -----------------------------------------------------------
 
+_raw_stream = None
+
+
 def stream_handle(stream=None):
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    """The cudaStream_t of a torch stream, or of the current one."""
+    global _raw_stream
+    if stream is not None:
+        return ctypes.c_void_p(stream.cuda_stream)
+    if _raw_stream is None:
+        import torch
+        try:  # the handle alone: torch.cuda.current_stream() builds a Stream object around it (3 us)
+            get, device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+            torch.cuda.current_stream()  # initialises CUDA
+            get(device())
+            _raw_stream = lambda: get(device())
+        except AttributeError:
+            _raw_stream = lambda: torch.cuda.current_stream().cuda_stream
+    return ctypes.c_void_p(_raw_stream())
 
 
 def ptr(t):
     return ctypes.c_void_p(t.data_ptr())
 
 
+_DTYPES = {}
+
+
 def dtype_code(t):
-    import torch
-    return {torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.bfloat16: BF16}[t.dtype]
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.bfloat16: BF16})
+    return _DTYPES[t.dtype]
 
 
 def view(base, offset=None, shape=None, strides=None, dtype=None):

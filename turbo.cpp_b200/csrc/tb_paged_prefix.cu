@@ -30,7 +30,8 @@
 //   columns 16 c, two parts to 32 c and 32 c + 16, a third to 64 + 16 c (three
 //   parts at head_dim 128 leave room for one buffer only).
 // Bounds for 64 keys and two row tiles (cycles per SM): exponentials 1024 on the
-// special function units, less what the FMA units take; products 320 at
+// special function units (a polynomial on the FMA units for some of them gained
+// nothing: 0, 1/8 .. 4/8 of them measured 81, 80, 81, 83, 85 us); products 320 at
 // head_dim 64 and 640 at 128 per row tile (Q is read from shared memory at 128
 // bytes a cycle, 1.5 times the tensor cores' own time for S).
 #include <algorithm>
@@ -118,40 +119,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x of a pair on the FMA units, so that they share the exponentials with the
-// special function units (a quarter of the FMA rate): x = n + f, n the nearest
-// integer (added to 1.5 2^23, whose low bits then hold it), |f| <= 1/2, 2^f a
-// polynomial, n added to the exponent.  The polynomials are minimax in the
-// relative error (Remez exchange): degree 3 is off by 7.5e-5, far below the
-// rounding of a probability to 16 bits, degree 5 by 7.5e-8 (2e-7 evaluated in
-// fp32).  Below -126 the result is 2^-126.
-template <int DEG>
-__device__ __forceinline__ void exp2_pair(uint64_t x, float &lo, float &hi) {
-  float a, b;
-  unpack2(x, a, b);
-  x = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t t = add2(x, pack2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), x);
-  auto c = [](float v) { return pack2(v, v); };
-  uint64_t p;
-  if constexpr (DEG == 3) {
-    p = fma2(c(0.05517166853f), f, c(0.24261112511f));
-    p = fma2(p, f, c(0.69326096773f));
-    p = fma2(p, f, c(0.99992805719f));
-  } else {
-    p = fma2(c(0.00132764725f), f, c(0.00967554096f));
-    p = fma2(p, f, c(0.05550713092f));
-    p = fma2(p, f, c(0.2402212024f));
-    p = fma2(p, f, c(0.69314694404f));
-    p = fma2(p, f, c(1.00000011921f));
-  }
-  float n0, n1, p0, p1;
-  unpack2(t, n0, n1);
-  unpack2(p, p0, p1);
-  lo = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
-  hi = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
-}
-
 // Shared-memory descriptor, 128-byte swizzle.  K-major (queries, keys): rows of
 // 128 bytes, groups of eight rows 1024 bytes apart.  MN-major (values): the same
 // bytes read as 64 columns of head_dim, groups of eight keys 1024 bytes apart,
@@ -175,7 +142,6 @@ struct TC {
   static constexpr int QBYTES = (PAIR_FITS ? 2 : 1) * QTILE;
   static constexpr int HALF = KT * RB;  // a tile of keys, or of values
   static constexpr int STAGES = 4;      // even, so that with alternate tiles a stage is always the same stream's
-  static constexpr int FMA_EIGHTHS = A32 ? 2 : 2;  // of the exponentials, on the FMA units
   static constexpr float SLACK = SUMS ? 0.f : 8.f;  // log2 by which a row may exceed its reference maximum
   static constexpr float PEXP = CT == TB_F16 ? 15.f - SLACK : 0.f;  // probabilities are scaled by 2^PEXP
   static constexpr uint32_t F = CT == TB_BF16 ? 1u : 0u;
@@ -486,13 +452,9 @@ __global__ void __launch_bounds__(kBlock, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint64_t x = fma2(pack2(__uint_as_float(u[c][2 * i]), __uint_as_float(u[c][2 * i + 1])), scale, shift);
-          if (i * C::FMA_EIGHTHS % 8 < C::FMA_EIGHTHS) {
-            exp2_pair<A32 ? 5 : 3>(x, p[2 * i], p[2 * i + 1]);
-          } else {
-            unpack2(x, p[2 * i], p[2 * i + 1]);
-            p[2 * i] = ex2(p[2 * i]);
-            p[2 * i + 1] = ex2(p[2 * i + 1]);
-          }
+          unpack2(x, p[2 * i], p[2 * i + 1]);
+          p[2 * i] = ex2(p[2 * i]);
+          p[2 * i + 1] = ex2(p[2 * i + 1]);
           sum[i & 1] = add2(sum[i & 1], pack2(p[2 * i], p[2 * i + 1]));
         }
 #pragma unroll

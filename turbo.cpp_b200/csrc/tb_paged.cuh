@@ -53,6 +53,9 @@ struct PrefixParts {
   int splits;  // 0: no prefix
   int parts;   // splits + 1
   int join_here;  // the kernel of the sequences' own keys joins the parts
+  // else per item of that kernel: its first CTA's slot and how many CTAs share it (0: one, its part is the row's last)
+  int2 *own;
+  int slot_rows;  // rows of a slot
 };
 
 // The pools as 4-d tensors [page][token][head][head_dim] for TMA: a box is up

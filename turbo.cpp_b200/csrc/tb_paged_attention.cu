@@ -656,6 +656,9 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   for (int u = u0; u < u1;) {
     const Walk item = cur;
     const int item0 = u - item.tile, end = min(u1, item0 + item.tiles);
+    if (!JOIN && a.prefix.splits > 0 && tid == 0 && item0 >= u0)
+      a.prefix.own[(int64_t)item.b * items + item.i] =
+          make_int2(2 * me + 1, item0 + item.tiles <= u1 ? 0 : owner(item0 + item.tiles - 1) - me + 1);
     reset(s);
     load_q(s, qf, a.scale2);
     for (; u < end; ++u) {
@@ -689,8 +692,8 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     computing_warps_sync();  // the merge buffer has been read
   }
 
-  // ---- the cut items: whoever of its CTAs comes last joins one
-  if (cut_unit[0] < 0 && cut_unit[1] < 0) {
+  // ---- the cut items: whoever of its CTAs comes last joins one (behind a prefix the next kernel does, JOIN apart)
+  if ((cut_unit[0] < 0 && cut_unit[1] < 0) || (!JOIN && a.prefix.splits > 0)) {
     pdl_wait();
     return;
   }
@@ -810,7 +813,8 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   if (sub == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
 }
 
-// The outputs behind a prefix: a warp per row joins its parts in order.
+// The outputs behind a prefix: a warp per row joins the prefix's parts and then
+// its own keys', in order, eight parts' loads at a time.
 template <int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const AttnArgs a, int heads) {
   constexpr int E = D / 32, P = 8;  // elements per lane; parts loaded at once
@@ -819,29 +823,40 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const AttnArgs a, in
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // b * heads + h
   if (row >= (int64_t)a.seqs.batch * heads) return;
-  const int b = (int)(row / heads), h = (int)(row - (int64_t)b * heads), kvh = h / a.group;
-  const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)b * a.group + h - kvh * a.group) * a.prefix.parts;
+  const int b = (int)(row / heads), h = (int)(row - (int64_t)b * heads), kvh = h / a.group, gi = h - kvh * a.group;
+  const int hg = gi / a.prefix.slot_rows;
+  const int2 own = __ldcg(a.prefix.own + ((int64_t)b * a.kv_heads + kvh) * a.head_groups + hg);
   Join<E> j;
-  for (int p0 = 0; p0 < a.prefix.parts; p0 += P) {
-    float2 ml[P];
-    float v[P][E];
+  // parts 0 .. n - 1, part p at index at(p) of acc and ml
+  auto join = [&](const float *acc, const float2 *ml, int n, auto at) {
+    for (int p0 = 0; p0 < n; p0 += P) {
+      float2 m[P];
+      float v[P][E];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const bool have = p0 + p < a.prefix.parts;
-      ml[p] = have ? __ldcg(a.prefix.ml + at + p0 + p) : make_float2(-INFINITY, 0.f);
-      const float *acc = a.prefix.acc + (at + p0 + p) * D + lane * E;
-      if constexpr (E == 2) {
-        const float2 x = have ? __ldcg(reinterpret_cast<const float2 *>(acc)) : make_float2(0.f, 0.f);
-        v[p][0] = x.x, v[p][1] = x.y;
-      } else {
-        const float4 x = have ? __ldcg(reinterpret_cast<const float4 *>(acc)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[p][0] = x.x, v[p][1] = x.y, v[p][2] = x.z, v[p][3] = x.w;
+      for (int p = 0; p < P; ++p) {
+        if (p0 + p >= n) continue;
+        const int64_t i = at(p0 + p);
+        m[p] = __ldcg(ml + i);
+        const float *from = acc + i * D + lane * E;
+        if constexpr (E == 2) {
+          const float2 x = __ldcg(reinterpret_cast<const float2 *>(from));
+          v[p][0] = x.x, v[p][1] = x.y;
+        } else {
+          const float4 x = __ldcg(reinterpret_cast<const float4 *>(from));
+          v[p][0] = x.x, v[p][1] = x.y, v[p][2] = x.z, v[p][3] = x.w;
+        }
       }
-    }
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (p0 + p < a.prefix.parts) j.add(ml[p], [&](int i) { return v[p][i]; });
-  }
+      for (int p = 0; p < P; ++p)
+        if (p0 + p < n) j.add(m[p], [&](int i) { return v[p][i]; });
+    }
+  };
+  const int64_t at = ((int64_t)kvh * a.prefix.rows + (int64_t)b * a.group + gi) * a.prefix.parts;
+  join(a.prefix.acc, a.prefix.ml, a.prefix.splits + (own.y == 0), [&](int p) { return at + p; });
+  // CTA c's slot 2 c + 1 where the item begins in it, the others' slot 2 c
+  const int r = gi - hg * a.prefix.slot_rows;
+  join(a.slot_acc, a.slot_ml, own.y,
+       [&](int p) { return (int64_t)(own.x + (p ? 2 * p - 1 : 0)) * a.prefix.slot_rows + r; });
   const int64_t to = (int64_t)b * a.ldo + (int64_t)h * D + lane * E;
 #pragma unroll
   for (int i = 0; i < E; ++i) store_act1(a.out, to + i, a.q.dtype, __fdiv_rn(j.acc[i], j.l));
@@ -854,7 +869,7 @@ int head_warps(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
-  size_t slot_acc, slot_ml, prefix_acc, prefix_ml, bytes;
+  size_t slot_acc, slot_ml, prefix_acc, prefix_ml, own, bytes;
 };
 Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   const size_t slots = 2 * kMaxCtas * 8 * (size_t)head_warps(heads / kv_heads);
@@ -864,7 +879,8 @@ Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   l.slot_ml = l.slot_acc + up256(slots * D * sizeof(float));
   l.prefix_acc = l.slot_ml + up256(slots * sizeof(float2));
   l.prefix_ml = l.prefix_acc + up256(rows * D * sizeof(float));
-  l.bytes = l.prefix_ml + up256(rows * sizeof(float2));
+  l.own = l.prefix_ml + up256(rows * sizeof(float2));
+  l.bytes = l.own + up256((size_t)(batch * heads) * sizeof(int2));
   return l;
 }
 
@@ -936,6 +952,7 @@ tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, c
   }
   const int hw = head_warps(a.group);
   a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
+  a.prefix.slot_rows = 8 * hw;
   switch (hw) {
     case 1: TB_TRY((launch_decode<CT, D, 1, A32>(a, maps, st, s, who))); break;
     case 2: TB_TRY((launch_decode<CT, D, 2, A32>(a, maps, st, s, who))); break;
@@ -984,6 +1001,7 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
   a.slot_ml = reinterpret_cast<float2 *>(w + l.slot_ml);
   a.prefix.acc = reinterpret_cast<float *>(w + l.prefix_acc);
   a.prefix.ml = reinterpret_cast<float2 *>(w + l.prefix_ml);
+  a.prefix.own = reinterpret_cast<int2 *>(w + l.own);
   a.prefix.rows = (int)(B * a.group);
   a.prefix_table = prefix_table;
   a.prefix_len = (int)prefix_len;

@@ -476,7 +476,7 @@ tb_status tb_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64
  * rows ldq and ldo elements apart, 16-byte aligned; act_dtype, their type, is
  * TB_F32 or the cache's.  head_dim 64 or 128, any number of query heads per
  * key/value head; batch * heads up to 2^24, and times max_pages * page_size up
- * to 2^37.  Accumulated in fp32; TB_F32 results are accurate to fp32 (no
+ * to 2^36.  Accumulated in fp32; TB_F32 results are accurate to fp32 (no
  * operand is rounded below 22 bits).  Keys, values and queries in use are
  * finite; what lies behind a sequence's last key is never used.  A length
  * below 0 or above max_pages * page_size counts as 0, a page id outside the

@@ -501,6 +501,27 @@ def test_shared_large_scores():
     y.check(y.run(shared=True))
 
 
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-30])
+@pytest.mark.parametrize("act,ct,dim", [("f32", "f16", 64), ("bf16", "bf16", 128), ("f32", "f32", 64)])
+def test_other_scales(act, ct, dim, scale):
+    x = Batch(act, ct, 4, 2, dim, 16, "token", [0, 5, 100] * 4, 300, seed=9)
+    x.scale = scale
+    x.check(x.run(shared=True))
+    x.n_prefix = 0  # the sequences' own keys alone
+    x.check(x.run())
+
+
+def test_queries_of_other_rows_do_not_matter():
+    """Empty slots of a padded batch hold whatever they hold: NaN, infinities, the largest numbers."""
+    for act, ct, dim, rows in (("f32", "f16", 64, 40), ("f32", "bf16", 128, 40), ("f16", "f16", 64, 40), ("f32", "f32", 64, 4)):
+        x = Batch(act, ct, 4, 1, dim, 16, "token", [7] * rows, 200, seed=10)
+        good = x.run(shared=True).clone(), x.run().clone()
+        for b, v in ((1, float("nan")), (2, float("inf")), (3, torch.finfo(TYPES[act]).max)):
+            x.q[b] = v
+        for was, now in zip(good, (x.run(shared=True), x.run())):
+            assert torch.equal(was[0], now[0]) and torch.equal(was[4:], now[4:])
+
+
 def test_shared_bad_prefix_page():
     x = Batch("f32", "f16", 4, 2, 64, 16, "token", [3] * 40, 100, seed=3)
     x.d_prefix[2] = x.kp.shape[0]

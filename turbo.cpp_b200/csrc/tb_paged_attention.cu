@@ -57,7 +57,7 @@ constexpr int kWarps = 4;              // computing warps
 constexpr int kThreads = kWarps * 32;  // their threads
 constexpr int kBlock = kThreads + 32;  // and one warp that loads
 constexpr int kJoinSplits = 16;       // splits of a prefix up to which the decode kernel may join them
-constexpr int kTensorRows = 64;       // query rows of a key/value head from which the prefix runs on tcgen05
+constexpr int kTensorRows = 33;       // query rows of a key/value head from which the prefix runs on tcgen05
 constexpr float kLog2e = 1.4426950408889634f;
 
 // x = hi + lo: hi the leading 11 bits (cut off, so that it neither overflows nor
@@ -282,11 +282,11 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
   }
   for (int k = k0; k < k1; k += STEP) {
     // scores: thread holds keys k + 8 b + 2 t, + 1 of row g (c0, c1: first part of q; c2, c3: second)
-    float c[C::NT][4];
+    float c[C::NT][4], lo[C::NT][4];  // lo: of fp32 keys' second parts, a chain of its own
 #pragma unroll
     for (int b = 0; b < C::NT; ++b)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[b][i] = 0.f;
+      for (int i = 0; i < 4; ++i) c[b][i] = lo[b][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < C::JD; ++j) {
       const int w = 8 * (j >> 1) + 2 * t + (j & 1);
@@ -298,17 +298,16 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
       }
       if constexpr (CT == TB_F32) {
 #pragma unroll
-        for (int b = 0; b < C::NT; ++b) {
-          float f[4];
-          Word<TB_F32>::get(u[b], f);
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int b = 0; b < C::NT; ++b) {
+            float f[4];
+            Word<TB_F32>::get(u[b], f);
             const float(&a)[4] = s.qa[2 * j + e];
             const float h0 = tf32_hi(f[2 * e]), h1 = tf32_hi(f[2 * e + 1]);
             mma_tf32(c[b], a, h0, h1);
-            mma_tf32(c[b], a, tf32_rn(f[2 * e] - h0), tf32_rn(f[2 * e + 1] - h1));
+            mma_tf32(lo[b], a, tf32_rn(f[2 * e] - h0), tf32_rn(f[2 * e + 1] - h1));
           }
-        }
       } else {
 #pragma unroll
         for (int p = 0; p < C::QT; ++p)
@@ -330,7 +329,9 @@ __device__ __forceinline__ void warp_tile(WarpState<C, D> &s, uint32_t stage, in
     for (int b = 0; b < C::NT; ++b)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float v = (C::QR == 4 ? c[b][i] + c[b][i + 2] : c[b][i]) * s.scale2;
+        float v = C::QR == 4 ? c[b][i] + c[b][i + 2] : c[b][i];
+        if (CT == TB_F32) v += lo[b][i] + lo[b][i + 2];
+        v *= s.scale2;
         p[b][i] = k + 8 * b + 2 * t + i < n ? v : -INFINITY;
         mx = fmaxf(mx, p[b][i]);
       }
@@ -742,7 +743,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   pdl_wait();
 }
 
-// The prefix: item (split, row tile, key/value head), rows = the queries of all
+// The prefix: item (row tile, split, key/value head), rows = the queries of all
 // sequences' heads of that key/value head, R of them per CTA.
 template <int CT, int D, int HW, bool A32>
 __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();  // only now: the next kernel relies on everything before this one having ended
-  const int split = blockIdx.x, rt = blockIdx.y, kvh = blockIdx.z;
+  const int split = blockIdx.y, rt = blockIdx.x, kvh = blockIdx.z;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
   const int t0 = (int)((int64_t)split * tiles / a.prefix.splits);
   const int t1 = (int)((int64_t)(split + 1) * tiles / a.prefix.splits);
@@ -925,8 +926,7 @@ tb_status launch_prefix(AttnArgs &a, const PagedMaps &maps, const DeviceState *s
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
   // one wave of CTAs
   set_prefix_splits(a, std::min<int64_t>(tiles, ctas / items));
-  if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
-  return launch_pdl(kern, dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, C::SMEM, s,
+  return launch_pdl(kern, dim3((unsigned)row_tiles, (unsigned)a.prefix.splits, (unsigned)a.kv_heads), kBlock, C::SMEM, s,
                     who, a, maps.k, maps.v, st->err_word);
 }
 
@@ -975,8 +975,8 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
     return fail(TB_EINVAL, "%s: heads must be a positive multiple of kv_heads", who);
   if (B * heads > (1 << 24)) return fail(TB_EINVAL, "%s: more than 2^24 query rows", who);
   if (prefix_len < 0 || prefix_len > 0x7FFFFFFF - 65536) return fail(TB_EINVAL, "%s: bad prefix length", who);
-  if (B * heads * (a.seqs.max_len / 64 + 1) > 0x7FFFFFFF)  // units of work at most
-    return fail(TB_EINVAL, "%s: batch * heads * max_pages * page_size is too large (2^37)", who);
+  if (B * heads * (a.seqs.max_len / 32 + 1) > 0x7FFFFFFF)  // units of work at most
+    return fail(TB_EINVAL, "%s: batch * heads * max_pages * page_size is too large (2^36)", who);
   if (B == 0) return TB_OK;
   if (!q || !out || !ws || (prefix_len > 0 && !prefix_table)) return fail(TB_EINVAL, "%s: null pointer", who);
   const int as = dtype_size(act_dtype);

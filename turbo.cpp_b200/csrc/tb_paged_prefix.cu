@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   // (the warp's number by a shuffle: known to be the same in all lanes, what follows from it stays in uniform registers,
   // which the tensor core's operands come from)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int split = blockIdx.x, kvh = blockIdx.z;
+  const int split = blockIdx.y, kvh = blockIdx.z;
   const int all = (a.prefix_len + C::KT - 1) / C::KT;
   const int t0 = (int)((int64_t)split * all / a.prefix.splits);
   const int n = (int)((int64_t)(split + 1) * all / a.prefix.splits) - t0;  // tiles of this CTA
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   pdl_wait();
   pdl_launch_dependents();  // only now: the next kernel relies on everything before this one having ended
   const int stream = warp >> 2, r = tid & 127;
-  const int row0 = blockIdx.y * (pair ? 2 * kRows : kRows);  // of all rows of the key/value head
+  const int row0 = blockIdx.x * (pair ? 2 * kRows : kRows);  // of all rows of the key/value head
   // ---- queries (all warps but the loading one): D / 8 lanes per row, eight elements each
   if (warp != 8) {
     constexpr int L = D / 8, PER = (kBlock - 32) / L;  // rows at a time
@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     const uint32_t ts = tmem + stream * 256 + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
     float scale2 = fabsf(a.scale2);
     if (A32 && CT == TB_F16) scale2 *= ctl.down[(pair ? stream * kRows : 0) + r];
+    if (scale2 < 1e-37f) scale2 = 1e-37f;  // 0 in effect, but times the -inf of a masked key it is still -inf
     uint64_t acc[C::SUMS ? D / 2 : 1];  // pairs of columns
     float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -570,8 +571,7 @@ tb_status launch(AttnArgs &a, const PagedMaps &maps, const DeviceState *st, cuda
   const int tiles = (a.prefix_len + C::KT - 1) / C::KT;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
   set_prefix_splits(a, std::min<int64_t>(tiles, st->sm_count / items));
-  if (row_tiles > 65535) return fail(TB_EINVAL, "%s: too many rows", who);
-  return launch_pdl(kern, dim3((unsigned)a.prefix.splits, (unsigned)row_tiles, (unsigned)a.kv_heads), kBlock, smem, s,
+  return launch_pdl(kern, dim3((unsigned)row_tiles, (unsigned)a.prefix.splits, (unsigned)a.kv_heads), kBlock, smem, s,
                     who, a, pair, maps.k, maps.v, st->err_word);
 }
 

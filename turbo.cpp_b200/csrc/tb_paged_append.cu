@@ -148,6 +148,8 @@ template <int ACT, int CT, int U>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, uint32_t *__restrict__ err) {
   constexpr int AS = Word<ACT>::size, CS = Word<CT>::size;
   constexpr int W = AS == 4 ? 2 : 1;  // 16-byte words of eight activations
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warps = a.tokens * a.per_token;
   const int half = a.dim / 2;
@@ -311,9 +313,9 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
   do {                                                                                 \
     a.per_token = (int)((groups + U - 1) / U);                                         \
     const int64_t threads = tokens * a.per_token * 32;                                 \
-    paged_append_kernel<ACT, CT, U>                                                    \
-        <<<wave_grid_of<paged_append_kernel<ACT, CT, U>>(threads, st), 256, 0, s>>>(a, st->err_word); \
-    return check_launch("tb_rope_paged_append");                                       \
+    return launch_pdl(paged_append_kernel<ACT, CT, U>,                                 \
+                      dim3((unsigned)wave_grid_of<paged_append_kernel<ACT, CT, U>>(threads, st)), 256, 0, s, \
+                      "tb_rope_paged_append", a, st->err_word);                        \
   } while (0)
 #define TB_APPEND(ACT, CT)               \
   do {                                   \

@@ -465,8 +465,11 @@ tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_paged_batch
 
 /* Bytes of the workspace of the two calls below (host arithmetic, no device
  * needed).  Zero the workspace once before its first use and keep it: every
- * call leaves it ready for the next.  It must be 256-byte aligned, and calls
- * that can overlap on the GPU need one each. */
+ * call leaves it ready for the next, of whatever batch and shape it is large
+ * enough for.  It must be 256-byte aligned, and calls that can overlap on the
+ * GPU need one each.  A wait inside a call that gives up (after 2 s; bit 0 of
+ * the device error word) leaves that call's output undefined; zero the
+ * workspace again then. */
 tb_status tb_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                              size_t *bytes_out);
 /* Attention of one query token per sequence (tb_attention_decode for a batch

@@ -7,7 +7,10 @@
 // with tb_rope's fused multiply-adds in fp32, so an fp32 cache holds what
 // tb_rope and tb_copy would have put there bit for bit.
 //
-// It moves every element once and computes next to nothing, so bytes bound it.
+// It moves every element once and computes next to nothing, so bytes bound it:
+// 33k tokens of 32 + 8 + 8 heads of 128 in fp16 take 124 us (6.5 TB/s of the
+// measured 6.55), 8k tokens of fp32 heads of 64 into bf16 pages 35.9 us (5.9
+// TB/s), one token 2.1 us.
 // A thread takes eight elements of a head's first half and the eight they are
 // paired with (16- or 32-byte loads and stores) for one to four heads of one
 // token, so that its cosines and sines are read once, and the token's sequence,
@@ -304,29 +307,31 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
   a.cos_t = cos_dev;
   a.sin_t = sin_dev;
   a.rope_max_seq = (int)rope_max_seq;
-  // Several groups per warp once that still fills the GPU: a token's lookups are shared and more loads are in flight.
+  // Four groups per warp for 16-bit activations once one group per warp would be more than a wave: the lookups are
+  // shared and more bytes are in flight.  Measured (bf16, 12 groups a token), one and four: 256 tokens 2.9 and 3.7 us,
+  // 700 tokens 5.6 and 4.1, 33k tokens 175 and 125.  fp32 rows have as many bytes in flight with one group (1000
+  // tokens: one 8.5, two 9.1 us; 8k tokens 35.9 and 35.3).
   const int span = 32 / a.per_head;
   const int64_t groups = (heads + 2 * KVH + span - 1) / span;
-  const bool wide = tokens * groups >= (int64_t)st->sm_count * 64;
+  const bool wide = tokens * groups >= (int64_t)st->sm_count * 32;
   cudaStream_t s = as_stream(stream);
-#define TB_APPEND_U(ACT, CT, U)                                                        \
-  do {                                                                                 \
-    a.per_token = (int)((groups + U - 1) / U);                                         \
-    const int64_t threads = tokens * a.per_token * 32;                                 \
-    return launch_pdl(paged_append_kernel<ACT, CT, U>,                                 \
-                      dim3((unsigned)wave_grid_of<paged_append_kernel<ACT, CT, U>>(threads, st)), 256, 0, s, \
-                      "tb_rope_paged_append", a, st->err_word);                        \
+#define TB_APPEND(ACT, CT, U)                                                                                       \
+  do {                                                                                                              \
+    a.per_token = (int)((groups + U - 1) / U);                                                                      \
+    const int ctas = wave_grid_of<paged_append_kernel<ACT, CT, U>>(tokens * a.per_token * 32, st);                  \
+    return launch_pdl(paged_append_kernel<ACT, CT, U>, dim3((unsigned)ctas), 256, 0, s, "tb_rope_paged_append", a, \
+                      st->err_word);                                                                                \
   } while (0)
-#define TB_APPEND(ACT, CT)               \
-  do {                                   \
-    if (wide) TB_APPEND_U(ACT, CT, (ACT == TB_F32 ? 2 : 4)); \
-    TB_APPEND_U(ACT, CT, 1);             \
-  } while (0)
-  if (act_dtype == TB_F16) TB_APPEND(TB_F16, TB_F16);
-  if (act_dtype == TB_BF16) TB_APPEND(TB_BF16, TB_BF16);
-  if (cache->dtype == TB_F16) TB_APPEND(TB_F32, TB_F16);
-  if (cache->dtype == TB_BF16) TB_APPEND(TB_F32, TB_BF16);
-  TB_APPEND(TB_F32, TB_F32);
+  if (act_dtype == TB_F16) {
+    if (wide) TB_APPEND(TB_F16, TB_F16, 4);
+    TB_APPEND(TB_F16, TB_F16, 1);
+  }
+  if (act_dtype == TB_BF16) {
+    if (wide) TB_APPEND(TB_BF16, TB_BF16, 4);
+    TB_APPEND(TB_BF16, TB_BF16, 1);
+  }
+  if (cache->dtype == TB_F16) TB_APPEND(TB_F32, TB_F16, 1);
+  if (cache->dtype == TB_BF16) TB_APPEND(TB_F32, TB_BF16, 1);
+  TB_APPEND(TB_F32, TB_F32, 1);
 #undef TB_APPEND
-#undef TB_APPEND_U
 }

@@ -28,16 +28,26 @@
 // Layout.  Each CTA's fifth warp brings tiles of T keys and values into three
 // stages of shared memory by TMA, one box per page, 128 bytes of each row,
 // swizzled so that every 16-byte fragment load is free of bank conflicts.  Of
-// the four other warps HW take eight query heads each, KW = 4 / HW take T / KW keys each; each warp keeps
-// its own (m, l, acc), joined once per item.  The order of head_dim inside the
-// dot product is chosen so that each thread's fragments are whole 16-byte words
-// of a key; 16-bit values are read transposed by ldmatrix.
+// the four other warps HW take eight query heads each, KW = 4 / HW take T / KW
+// keys each; each warp keeps its own (m, l, acc), joined once per item.  The
+// order of head_dim inside the dot product is chosen so that each thread's
+// fragments are whole 16-byte words of a key; 16-bit values are read transposed
+// by ldmatrix.
+//
+// Bytes bound it: keys and values are read once, and four to eight heads leave
+// the tensor pipe 86 % idle.  Measured (bf16, 32 heads on 8 of 128): 128
+// sequences of up to 8192 keys 324 us, 6.3 TB/s of the measured 6.55; one of
+// 131071 keys 94 us, 5.7 TB/s; (fp16 pages, fp32 queries, heads of 64) 32 of up
+// to 4096 keys 32.5 us; one of 511 fp32 keys 7.5 us, all of it latency.
 //
 // Work split.  An item is one (sequence, key/value head, group of 8 HW query
 // heads); its unit of work is one tile.  The grid is one wave; CTA c takes the
 // units [c U / n, (c + 1) U / n) of all U, found on the device from the
 // lengths, so uneven batches and single long sequences fill the GPU alike and a
-// captured launch follows the lengths.  An item cut by a CTA boundary leaves
+// captured launch follows the lengths.  Four computing warps per CTA and two or
+// three CTAs per SM: a short item's steps (queries, one tile, joining the warps)
+// then overlap with other items' (64 sequences of up to 512 keys behind a prefix
+// 37.3 us, one CTA of eight warps 40.6).  An item cut by a CTA boundary leaves
 // partial results in the workspace; the last of its CTAs to finish (a counter
 // per first CTA, reset by that CTA) joins them.  Behind a prefix there are three
 // kernels: the prefix's (here, or tb_paged_prefix.cu for many rows), this one
@@ -53,11 +63,16 @@ namespace {
 
 constexpr int kMaxCtas = 448;                    // of a decode launch (counters and partial slots)
 constexpr int64_t kPrefixRows = 2 * 148 * 128;   // extra (row, split) pairs of prefix partials
-constexpr int kWarps = 4;              // computing warps
-constexpr int kThreads = kWarps * 32;  // their threads
-constexpr int kBlock = kThreads + 32;  // and one warp that loads
-constexpr int kJoinSplits = 16;       // splits of a prefix up to which the decode kernel may join them
-constexpr int kTensorRows = 33;       // query rows of a key/value head from which the prefix runs on tcgen05
+constexpr int kWarps = 4;                        // computing warps
+constexpr int kThreads = kWarps * 32;            // their threads
+constexpr int kBlock = kThreads + 32;            // and one warp that loads
+// Splits of a prefix up to which the decode kernel may join them: 4 sequences behind 1001 keys (16 splits) 8.0 us so and
+// 9.1 with a kernel of its own, 17 behind 16387 (37 splits) 48.2 and 33.6.
+constexpr int kJoinSplits = 16;
+// Query rows of a key/value head from which the prefix runs on tcgen05.  Here and there: 32 and 36 rows behind 8192 keys
+// of 64 (fp16, fp32 queries) 20.0 and 19.7 us, 60 rows 24.0 and 21.1; behind 32768 keys of 128 (bf16) 45.9 and 40.6,
+// 75.0 and 42.6.
+constexpr int kTensorRows = 33;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // x = hi + lo: hi the leading 11 bits (cut off, so that it neither overflows nor
@@ -127,10 +142,11 @@ __device__ __forceinline__ uint4 ldmatrix_t(uint32_t addr) {
   return v;
 }
 
-// What a CTA keeps in shared memory behind the stages and the merge buffer.
-struct Walk {  // where a CTA stands in the list of all units: tile `tile` of item (b, i)
+// Where a CTA stands in the list of all units: tile `tile` of item (b, i).
+struct Walk {
   int b, i, tile, tiles, len;
 };
+// What it keeps in shared memory behind the stages and the merge buffer.
 constexpr int kMaxStages = 3;
 struct Control {
   uint64_t full[kMaxStages], empty[kMaxStages];
@@ -525,8 +541,8 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   pdl_launch_dependents();
   if (a.prefix.splits == 0) pdl_wait();
 
-  // ---- the units of all sequences, and this CTA's share: with n CTAs, unit r of U goes to r / (U / n) or so, the
-  // first U % n CTAs taking one more (the host has made sure that U < 2^31)
+  // ---- the units of all sequences, and this CTA's share of them: U / n for each of n CTAs, one more for the first
+  // U % n (the host has made sure that U < 2^31)
   const int per = (a.seqs.batch + kBlock - 1) / kBlock;
   const int b0 = min(a.seqs.batch, tid * per), b1 = min(a.seqs.batch, b0 + per);
   int mine = 0;

@@ -16,7 +16,9 @@ Tolerances.  A rounding to a type is off by at most eps/2 of the value.
    16-bit activations behind a prefix may round each p to the cache's type: eps/2
    of p, numerator and denominator alike."""
 import ctypes
-import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -442,6 +444,75 @@ def test_decode_far_offsets():
         v = torch.cat([vp[int(table[b, i]), :min(max(lens[b] - i * page, 0), page)] for i in range(2)])
         want, tol = exact(q[b].view(4, dim), k, v, 0.125)
         check_rows(out[b].view(4, dim), want, tol, torch.float32)
+
+
+def test_many_sequences():
+    """More sequences than rows of one grid dimension, one key each; then all of them behind a prefix."""
+    batch, heads, dim = 150000, 2, 64
+    gen = torch.Generator("cuda").manual_seed(3)
+    kp, vp = (torch.randn((batch + 5, 16, 1, dim), generator=gen, device="cuda").bfloat16() for _ in range(2))
+    table = torch.randperm(batch, generator=gen, device="cuda").int()[:, None].contiguous()
+    lens = torch.ones(batch, dtype=torch.int32, device="cuda")
+    q = torch.randn((batch, heads * dim), generator=gen, device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    ws = workspace(batch, heads, 1, dim)
+    c, b = T.paged_cache(kp, vp), T.paged_batch(lens, table)
+    T.call("tb_paged_attention_decode", T.byref(c), T.byref(b), T.BF16, T.ptr(q), heads * dim, heads, 0.125, T.ptr(out),
+           heads * dim, T.ptr(ws), ws.numel(), T.stream_handle())
+    own = vp[table[:, 0].long(), 0, 0]
+    assert torch.equal(out.view(batch, heads, dim), own[:, None].expand(batch, heads, dim))
+    prefix = torch.arange(batch, batch + 5, dtype=torch.int32, device="cuda")
+    T.call("tb_paged_attention_shared", T.byref(c), T.byref(b), T.ptr(prefix), 77, T.BF16, T.ptr(q), heads * dim, heads,
+           0.125, T.ptr(out), heads * dim, T.ptr(ws), ws.numel(), T.stream_handle())
+    torch.cuda.synchronize()
+    assert T.take_device_errors() == 0
+    pk, pv = (p[batch:].reshape(80, 1, dim)[:77] for p in (kp, vp))
+    for i in (0, 1, 127, 128, 65535, 65536, 99999, batch - 1):
+        k, v = (torch.cat((x, p[table[i, 0].long(), :1])) for x, p in ((pk, kp), (pv, vp)))
+        want, tol = exact(q[i].view(heads, dim), k, v, 0.125, torch.finfo(torch.bfloat16).eps / 2)
+        check_rows(out[i].view(heads, dim), want, tol, torch.bfloat16)
+
+
+def test_first_use_is_captured():
+    """In a new process: the first calls of all are captured, then replayed."""
+    code = """
+import ctypes, torch, turbo_b200 as T
+torch.manual_seed(1)
+kp, vp = (torch.randn((20, 16, 2, 64), device="cuda").half() for _ in range(2))
+table = torch.arange(18, dtype=torch.int32, device="cuda").view(2, 9)
+lens = torch.tensor([140, 3], dtype=torch.int32, device="cuda")
+q, kv = torch.randn((2, 512), device="cuda"), torch.randn((2, 2, 128), device="cuda")
+cos, sin = torch.ones((200, 32), device="cuda"), torch.zeros((200, 32), device="cuda")
+out, again, turned = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+prefix = torch.tensor([18, 19], dtype=torch.int32, device="cuda")
+c, b = T.paged_cache(kp, vp), T.paged_batch(lens, table)
+n = ctypes.c_size_t()
+T.call("tb_paged_attention_workspace_bytes", 2, 8, 2, 64, ctypes.byref(n))
+ws = torch.zeros(n.value, dtype=torch.uint8, device="cuda")
+def step(s, out):
+    T.call("tb_rope_paged_append", T.byref(c), T.byref(b), T.F32, T.ptr(q), 512, T.ptr(kv), 256, kv.data_ptr() + 512, 256, 2,
+           8, None, T.ptr(cos), T.ptr(sin), 200, T.ptr(turned), 512, s)
+    T.call("tb_paged_attention_shared", T.byref(c), T.byref(b), T.ptr(prefix), 25, T.F32, T.ptr(turned), 512, 8, 0.125,
+           T.ptr(out), 512, T.ptr(ws), n.value, s)
+s, g = ctypes.c_void_p(), ctypes.c_void_p()
+T.call("tb_init", 0)
+T.call("tb_stream_create", ctypes.byref(s))
+torch.cuda.synchronize()
+T.call("tb_capture_begin", s)
+step(s, out)
+T.call("tb_capture_end", s, ctypes.byref(g))
+for _ in range(3):
+    T.call("tb_graph_launch", g, s)
+T.call("tb_sync", s)
+step(s, again)
+T.call("tb_sync", s)
+assert torch.equal(out, again) and out.abs().sum() > 0 and T.take_device_errors() == 0
+T.call("tb_graph_destroy", g)
+print("captured")
+"""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, env=env)
+    assert "captured" in r.stdout, r.stdout + r.stderr
 
 
 SHARED = [

@@ -9,14 +9,13 @@
 //
 // It moves every element once and computes next to nothing, so bytes bound it:
 // 33k tokens of 32 + 8 + 8 heads of 128 in fp16 take 124 us (6.5 TB/s of the
-// measured 6.55), 8k tokens of fp32 heads of 64 into bf16 pages 35.9 us (5.9
+// measured 6.55), 8k tokens of fp32 heads of 64 into bf16 pages 34.9 us (6.1
 // TB/s), one token 2.1 us.
-// A thread takes eight elements of a head's first half and the eight they are
-// paired with (16- or 32-byte loads and stores) for one to four heads of one
-// token, so that its cosines and sines are read once, and the token's sequence,
-// position and page are found once per warp: a 32-way search of `starts` by
-// ballot, then one table entry.  The data loads do not depend on that chain and
-// are issued before it.
+// A thread takes 16 bytes of a head's first half and the 16 they are paired
+// with, for one to four heads of one token, so that its cosines and sines are
+// read once, and the token's sequence, position and page are found once per
+// warp: a 32-way search of `starts` by ballot, then one table entry.  The data
+// loads do not depend on that chain and are issued before it.
 #include <algorithm>
 #include <atomic>
 
@@ -112,7 +111,7 @@ struct AppendArgs {
   int64_t ldq_out;
   int64_t tokens;
   int heads, kv_heads, dim;
-  int per_head;   // threads per head: dim / 16
+  int per_head;   // threads per head, 16 bytes of each half
   int per_token;  // warps per token
   const int32_t *starts;
   const float *cos_t, *sin_t;  // null: no rotation
@@ -121,27 +120,15 @@ struct AppendArgs {
   PagedSeqs seqs;
 };
 
-template <int DT>
-__device__ __forceinline__ void put8(void *p, const float (&f)[8]) {
-  uint4 *d = static_cast<uint4 *>(p);
-  if constexpr (DT == TB_F32) {
-    d[0] = Word<TB_F32>::put(f);
-    d[1] = Word<TB_F32>::put(f + 4);
+// E elements (16 bytes of activations) as type DT.
+template <int DT, int E>
+__device__ __forceinline__ void put(void *p, const float (&f)[E]) {
+  if constexpr (DT != TB_F32 && E == 4) {
+    float a = f[0], b = f[1], c = f[2], d = f[3];
+    const uint32_t lo = pack_rest<DT>(a, b), hi = pack_rest<DT>(c, d);
+    *static_cast<uint2 *>(p) = make_uint2(lo, hi);
   } else {
-    d[0] = Word<DT>::put(f);
-  }
-}
-
-template <int ACT>
-__device__ __forceinline__ void words(const uint4 *w, float (&f)[8]) {
-  if constexpr (ACT == TB_F32) {
-    float lo[4], hi[4];
-    Word<TB_F32>::get(w[0], lo);
-    Word<TB_F32>::get(w[1], hi);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
-  } else {
-    Word<ACT>::get(w[0], f);
+    *static_cast<uint4 *>(p) = Word<DT>::put(f);
   }
 }
 
@@ -150,19 +137,19 @@ __device__ __forceinline__ void words(const uint4 *w, float (&f)[8]) {
 template <int ACT, int CT, int U>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, uint32_t *__restrict__ err) {
   constexpr int AS = Word<ACT>::size, CS = Word<CT>::size;
-  constexpr int W = AS == 4 ? 2 : 1;  // 16-byte words of eight activations
+  constexpr int E = Word<ACT>::n;  // elements of each half of a head per thread
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warps = a.tokens * a.per_token;
   const int half = a.dim / 2;
   // a group is 32 / per_head heads; this thread has the same elements of each
-  const int span = 32 / a.per_head, sub = lane / a.per_head, i = (lane - sub * a.per_head) * 8;
+  const int span = 32 / a.per_head, sub = lane / a.per_head, i = (lane - sub * a.per_head) * E;
   const int all = sub < span ? a.heads + 2 * a.kv_heads : 0;
   for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < warps; w += (int64_t)gridDim.x * 8) {
     const int64_t t = w / a.per_token;
     const int head0 = (int)(w - t * a.per_token) * span * U + sub;
-    uint4 r0[U][W], r1[U][W];
+    uint4 r0[U], r1[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int head = head0 + k * span;
@@ -170,11 +157,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
       const ActRows &src = head < a.heads ? a.q : head < a.heads + a.kv_heads ? a.k : a.v;
       const int h = head < a.heads ? head : head < a.heads + a.kv_heads ? head - a.heads : head - a.heads - a.kv_heads;
       const char *at = static_cast<const char *>(src.p) + (t * src.ld + (int64_t)h * a.dim + i) * AS;
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        r0[k][e] = reinterpret_cast<const uint4 *>(at)[e];
-        r1[k][e] = reinterpret_cast<const uint4 *>(at + half * AS)[e];
-      }
+      r0[k] = *reinterpret_cast<const uint4 *>(at);
+      r1[k] = *reinterpret_cast<const uint4 *>(at + half * AS);
     }
     // the token's sequence: the last b with starts[b] <= t
     int b = (int)t, pos;
@@ -211,21 +195,21 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
       if (lane == 0) atomicOr(err, ERR_INDEX);
       continue;
     }
-    float c[8], sn[8];
+    float c[E], sn[E];
     if (a.cos_t && head0 < a.heads + a.kv_heads) {
-      load_act<8>(a.cos_t, (int64_t)pos * half + i, TB_F32, c);
-      load_act<8>(a.sin_t, (int64_t)pos * half + i, TB_F32, sn);
+      load_act<E>(a.cos_t, (int64_t)pos * half + i, TB_F32, c);
+      load_act<E>(a.sin_t, (int64_t)pos * half + i, TB_F32, sn);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int head = head0 + k * span;
       if (head >= all) continue;
-      float x0[8], x1[8];
-      words<ACT>(r0[k], x0);
-      words<ACT>(r1[k], x1);
+      float x0[E], x1[E];
+      Word<ACT>::get(r0[k], x0);
+      Word<ACT>::get(r1[k], x1);
       if (a.cos_t && head < a.heads + a.kv_heads) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < E; ++e) {
           const float y0 = __fmaf_rn(x0[e], c[e], -__fmul_rn(x1[e], sn[e]));
           x1[e] = __fmaf_rn(x0[e], sn[e], __fmul_rn(x1[e], c[e]));
           x0[e] = y0;
@@ -233,14 +217,14 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
       }
       if (head < a.heads) {
         char *d = static_cast<char *>(a.q_out) + (t * a.ldq_out + (int64_t)head * a.dim + i) * AS;
-        put8<ACT>(d, x0);
-        put8<ACT>(d + half * AS, x1);
+        put<ACT>(d, x0);
+        put<ACT>(d + half * AS, x1);
       } else {
         const bool key = head < a.heads + a.kv_heads;
         const int h = head - a.heads - (key ? 0 : a.kv_heads);
         char *d = const_cast<char *>(key ? a.pools.k : a.pools.v) + row + h * a.pools.head_stride + i * CS;
-        put8<CT>(d, x0);
-        put8<CT>(d + half * CS, x1);
+        put<CT>(d, x0);
+        put<CT>(d + half * CS, x1);
       }
     }
   }
@@ -302,15 +286,15 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
   a.heads = (int)heads;
   a.kv_heads = (int)KVH;
   a.dim = (int)D;
-  a.per_head = (int)(D / 16);
+  a.per_head = (int)(D * as / 32);
   a.starts = starts_dev;
   a.cos_t = cos_dev;
   a.sin_t = sin_dev;
   a.rope_max_seq = (int)rope_max_seq;
-  // Four groups per warp for 16-bit activations once one group per warp would be more than a wave: the lookups are
-  // shared and more bytes are in flight.  Measured (bf16, 12 groups a token), one and four: 256 tokens 2.9 and 3.7 us,
-  // 700 tokens 5.6 and 4.1, 33k tokens 175 and 125.  fp32 rows have as many bytes in flight with one group (1000
-  // tokens: one 8.5, two 9.1 us; 8k tokens 35.9 and 35.3).
+  // Several groups per warp (four of 16-bit activations, two of fp32) once one per warp would be more than a wave: the
+  // lookups are shared and more bytes are in flight.  Measured with one and several: bf16, 12 groups a token, 256 tokens
+  // 2.9 and 3.7 us, 700 tokens 5.6 and 4.1, 33k tokens 175 and 125; fp32, 24 groups, 1000 tokens 8.1 and 7.0, 8k tokens
+  // 37.6 and 34.9.
   const int span = 32 / a.per_head;
   const int64_t groups = (heads + 2 * KVH + span - 1) / span;
   const bool wide = tokens * groups >= (int64_t)st->sm_count * 32;
@@ -330,8 +314,15 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
     if (wide) TB_APPEND(TB_BF16, TB_BF16, 4);
     TB_APPEND(TB_BF16, TB_BF16, 1);
   }
-  if (cache->dtype == TB_F16) TB_APPEND(TB_F32, TB_F16, 1);
-  if (cache->dtype == TB_BF16) TB_APPEND(TB_F32, TB_BF16, 1);
+  if (cache->dtype == TB_F16) {
+    if (wide) TB_APPEND(TB_F32, TB_F16, 2);
+    TB_APPEND(TB_F32, TB_F16, 1);
+  }
+  if (cache->dtype == TB_BF16) {
+    if (wide) TB_APPEND(TB_F32, TB_BF16, 2);
+    TB_APPEND(TB_F32, TB_BF16, 1);
+  }
+  if (wide) TB_APPEND(TB_F32, TB_F32, 2);
   TB_APPEND(TB_F32, TB_F32, 1);
 #undef TB_APPEND
 }

@@ -52,6 +52,7 @@ struct PrefixParts {
   int rows;    // batch * group
   int splits;  // 0: no prefix
   int parts;   // splits + 1
+  int few;        // few items and short sequences behind it
   int join_here;  // the kernel of the sequences' own keys joins the parts
   // else per item of that kernel: its first CTA's slot and how many CTAs share it (0: one, its part is the row's last)
   int2 *own;
@@ -258,8 +259,9 @@ struct AttnArgs {
   float *slot_acc;  // [2 kMaxCtas][8 HW][D]
   float2 *slot_ml;  // [2 kMaxCtas][8 HW]
   PrefixParts prefix;
-  const int32_t *prefix_table;  // prefix kernels
+  const int32_t *prefix_table;
   int prefix_len;
+  int lead;  // tiles of a short prefix that the decode kernel takes before each sequence's own, instead of a kernel
   int box_shift;  // a TMA box holds 1 << box_shift tokens
 };
 

@@ -69,6 +69,15 @@ constexpr int kBlock = kThreads + 32;            // and one warp that loads
 // Splits of a prefix up to which the decode kernel may join them: 4 sequences behind 1001 keys (16 splits) 8.0 us so and
 // 9.1 with a kernel of its own, 17 behind 16387 (37 splits) 48.2 and 33.6.
 constexpr int kJoinSplits = 16;
+// ... and tiles of a sequence's own keys: with more of them its items are cut, and the joins in the kernel slow it (17 x
+// up to 777 behind 512: 22.8 us).
+constexpr int kJoinTiles = 4;
+// A short prefix, of up to so many tiles per item and units of work in all, is read by the decode kernel before each
+// sequence's own keys: two launches fewer.  Measured so and with the prefix's kernels: 64 behind 64, 256, 512 and 1024
+// keys of 64 (512, 2048, 4096, 8192 units) 16.1 and 21.4, 18.4 and 22.1, 22.1 and 22.6, 30.3 and 26.1 us; 4 behind 1001
+// (16 tiles per item) 12.4 and 8.4.
+constexpr int kLeadTiles = 8;
+constexpr int64_t kLeadUnits = 4096;
 // Query rows of a key/value head from which the prefix runs on tcgen05.  Here and there: 32 and 36 rows behind 8192 keys
 // of 64 (fp16, fp32 queries) 20.0 and 19.7 us, 60 rows 24.0 and 21.1; behind 32768 keys of 128 (bf16) 45.9 and 40.6,
 // 75.0 and 42.6.
@@ -502,8 +511,8 @@ __device__ __forceinline__ void join_warps(Join<N> &j, const float *merge, int r
 }
 
 template <class C>
-__device__ __forceinline__ int tiles_of(int len) {
-  return max(1, (len + C::T - 1) / C::T);
+__device__ __forceinline__ int tiles_of(const AttnArgs &a, int len) {
+  return max(1, a.lead + (len + C::T - 1) / C::T);
 }
 
 __device__ __forceinline__ int seq_len(const PagedSeqs &s, int b) {
@@ -549,7 +558,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   for (int b = b0; b < b1; ++b) {
     const int len = __ldg(a.seqs.lens + b);
     if (blockIdx.x == 0 && (len < 0 || len > a.seqs.max_len)) atomicOr(err, ERR_INDEX);
-    mine += tiles_of<C>(seq_len(a.seqs, b)) * items;
+    mine += tiles_of<C>(a, seq_len(a.seqs, b)) * items;
   }
   int incl = mine;
 #pragma unroll
@@ -580,7 +589,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   if (u0 >= before && u0 < before + mine) {
     int u = u0 - before;
     for (int b = b0;; ++b) {
-      const int len = seq_len(a.seqs, b), tiles = tiles_of<C>(len);
+      const int len = seq_len(a.seqs, b), tiles = tiles_of<C>(a, len);
       const int n = tiles * items;
       if (u < n) {
         const int i = u / tiles;
@@ -599,12 +608,15 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     uint32_t phase = 1;  // the stages begin empty
     int next_len = cur.b + 1 < a.seqs.batch ? seq_len(a.seqs, cur.b + 1) : 0;
     for (int u = u0; u < u1; ++u) {
-      const int32_t *table = a.seqs.table + (int64_t)cur.b * a.seqs.table_stride;
-      const TileBoxes box = tile_boxes<C::T>(a.pools, a.box_shift, table, cur.len, cur.tile);  // before the wait
+      const bool own = cur.tile >= a.lead;
+      const int32_t *table = own ? a.seqs.table + (int64_t)cur.b * a.seqs.table_stride : a.prefix_table;
+      const int tile = own ? cur.tile - a.lead : cur.tile;
+      const TileBoxes box =  // before the wait
+          tile_boxes<C::T>(a.pools, a.box_shift, table, own ? cur.len : a.prefix_len, tile);
       wait_phase(&ctl.empty[stage], phase, err, dead);
       if (lane == 0) ctl.at[stage] = cur;
       load_rows<C::T, C::RB, Word<CT>::size>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools,
-                                             a.box_shift, table, box, cur.tile, cur.i / a.head_groups, err);
+                                             a.box_shift, table, box, tile, cur.i / a.head_groups, err);
       if (++stage == C::STAGES) stage = 0, phase ^= 1;
       if (++cur.tile < cur.tiles) continue;
       cur.tile = 0;
@@ -612,7 +624,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
       cur.i = 0;
       ++cur.b;
       cur.len = next_len;
-      cur.tiles = tiles_of<C>(next_len);
+      cur.tiles = tiles_of<C>(a, next_len);
       if (cur.b + 1 < a.seqs.batch) next_len = seq_len(a.seqs, cur.b + 1);
     }
     pdl_wait();
@@ -658,7 +670,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
       if (e == 0) a.prefix.ml[at] = make_float2(j.m, j.l);
       return;
     }
-    const bool none = w.len == 0 && a.prefix.splits == 0;
+    const bool none = w.len == 0 && a.prefix_len == 0;
     const int64_t at = (int64_t)w.b * a.ldo + (int64_t)(kvh * a.group + gi) * D + e;
 #pragma unroll
     for (int i = 0; i < n; ++i)
@@ -682,7 +694,9 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     load_q(s, qf, a.scale2);
     for (; u < end; ++u) {
       wait_phase(&ctl.full[stage], phase, err, dead);
-      warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, item.len - (u - item0) * C::T), kw);
+      const int tile = u - item0 - a.lead;  // of the sequence's own; below 0 of the prefix
+      const int keys = tile < 0 ? a.prefix_len - (tile + a.lead) * C::T : item.len - tile * C::T;
+      warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, keys), kw);
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.empty[stage]);
       if (++stage == C::STAGES) stage = 0, phase ^= 1;
@@ -923,7 +937,7 @@ tb_status launch_decode(AttnArgs &a, const PagedMaps &maps, const DeviceState *s
   int ctas;
   TB_TRY((wave_of<C, paged_decode_kernel<CT, D, HW, A32, false>>(st, &ctas)));
   a.max_ctas = std::min(ctas, kMaxCtas);
-  a.prefix.join_here = a.prefix.splits > 0 && a.prefix.splits <= kJoinSplits && (int64_t)a.seqs.batch * a.kv_heads * a.head_groups <= a.max_ctas;
+  a.prefix.join_here = a.prefix.splits > 0 && a.prefix.splits <= kJoinSplits && a.prefix.few;
   if (a.prefix.join_here) {
     TB_TRY((wave_of<C, paged_decode_kernel<CT, D, HW, A32, true>>(st, &ctas)));
     a.max_ctas = std::min(ctas, kMaxCtas);
@@ -959,18 +973,25 @@ tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, c
   TB_TRY(paged_maps(&c, T, who, &maps, &box));
   a.box_shift = 0;
   while ((1 << a.box_shift) < box) ++a.box_shift;
-  if (CT != TB_F32 && a.prefix_len > 0 && a.prefix.rows >= kTensorRows) {
+  const int hw = head_warps(a.group);
+  a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
+  a.prefix.slot_rows = 8 * hw;
+  const int64_t lead = (a.prefix_len + T - 1) / T;
+  const int64_t items = (int64_t)a.seqs.batch * a.kv_heads * a.head_groups;
+  const int64_t own = (a.seqs.max_len + T - 1) / T;  // tiles of a sequence at most
+  a.prefix.few = items <= st->sm_count && own <= kJoinTiles;
+  if (!a.prefix.few && lead <= kLeadTiles && lead * items <= kLeadUnits) {
+    a.lead = (int)lead;
+  } else if (a.prefix_len == 0) {
+  } else if (CT != TB_F32 && a.prefix.rows >= kTensorRows) {
     TB_TRY(launch_prefix_tc(a, maps, CT, D, st, s, who));
-  } else if (a.prefix_len > 0) {
+  } else {
     switch (head_warps(a.prefix.rows)) {
       case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, maps, st, s, who))); break;
       case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, maps, st, s, who))); break;
       default: TB_TRY((launch_prefix<CT, D, 4, A32>(a, maps, st, s, who))); break;
     }
   }
-  const int hw = head_warps(a.group);
-  a.head_groups = (a.group + 8 * hw - 1) / (8 * hw);
-  a.prefix.slot_rows = 8 * hw;
   switch (hw) {
     case 1: TB_TRY((launch_decode<CT, D, 1, A32>(a, maps, st, s, who))); break;
     case 2: TB_TRY((launch_decode<CT, D, 2, A32>(a, maps, st, s, who))); break;
@@ -993,7 +1014,7 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
     return fail(TB_EINVAL, "%s: heads must be a positive multiple of kv_heads", who);
   if (B * heads > (1 << 24)) return fail(TB_EINVAL, "%s: more than 2^24 query rows", who);
   if (prefix_len < 0 || prefix_len > 0x7FFFFFFF - 65536) return fail(TB_EINVAL, "%s: bad prefix length", who);
-  if (B * heads * (a.seqs.max_len / 32 + 1) > 0x7FFFFFFF)  // units of work at most
+  if (B * heads * (a.seqs.max_len / 32 + 1) > 0x7FFFFFFF - kLeadUnits)  // units of work at most
     return fail(TB_EINVAL, "%s: batch * heads * max_pages * page_size is too large (2^36)", who);
   if (B == 0) return TB_OK;
   if (!q || !out || !ws || (prefix_len > 0 && !prefix_table)) return fail(TB_EINVAL, "%s: null pointer", who);

@@ -556,7 +556,16 @@ def test_shared(case):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("rows", [1, 8, 9, 31, 64, 65, 127, 128, 129, 300])
 def test_shared_rows(rows, dim, act, ct):
-    x = Batch(act, ct, 1, 1, dim, 16, "token", [b % 2 for b in range(rows)], 259, seed=rows)
+    for prefix in (259, 643):  # read by the decode kernel, and by kernels of its own
+        x = Batch(act, ct, 1, 1, dim, 16, "token", [b % 2 for b in range(rows)], prefix, seed=rows)
+        x.check(x.run(shared=True))
+
+
+@pytest.mark.parametrize("lens", [[0, 3, 64, 65, 200], [5, 0]])
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 128, 500])
+@pytest.mark.parametrize("act,ct,dim", [("f32", "f16", 64), ("bf16", "bf16", 128), ("f32", "f32", 128)])
+def test_shared_short_prefix(act, ct, dim, prefix, lens):
+    x = Batch(act, ct, 4, 2, dim, 16, "head", lens * 40, prefix, seed=prefix)
     x.check(x.run(shared=True))
 
 
@@ -607,10 +616,12 @@ def test_two_streams_with_a_workspace_each():
     x = Batch("f32", "f16", 4, 2, 64, 16, "token", [5000, 1, 700, 0], seed=1)
     y = Batch("bf16", "bf16", 8, 4, 128, 32, "head", [9, 4000, 333], 1000, seed=2)
     streams = [torch.cuda.Stream() for _ in range(2)]
-    torch.cuda.synchronize()
-    outs = []
-    for _ in range(20):
-        outs.append((x.run(stream=streams[0]), y.run(shared=True, stream=streams[1])))
+    outs = [[torch.full((len(z.lens), z.heads * z.dim + 8), 9.0, dtype=z.act, device="cuda") for z in (x, y)]
+            for _ in range(20)]
+    torch.cuda.synchronize()  # the fills ran on another stream
+    for a, b in outs:
+        x.run(out=a, stream=streams[0])
+        y.run(shared=True, out=b, stream=streams[1])
     torch.cuda.synchronize()
     for a, b in outs:
         assert torch.equal(a, outs[0][0]) and torch.equal(b, outs[0][1])

@@ -51,8 +51,9 @@
 // partial results in the workspace; the last of its CTAs to finish (a counter
 // per first CTA, reset by that CTA) joins them.  Behind a prefix there are three
 // kernels: the prefix's (here, or tb_paged_prefix.cu for many rows), this one
-// for the sequences' own keys, and one that joins the parts of each row; where
-// every item has a CTA of its own this one joins them itself.
+// for the sequences' own keys, and one that joins the parts of each row.  Few
+// short sequences: this one joins them itself.  A short prefix: this one alone,
+// reading it (from L2) before each sequence's own keys.
 #include <algorithm>
 #include <atomic>
 
@@ -944,7 +945,8 @@ tb_status launch_decode(AttnArgs &a, const PagedMaps &maps, const DeviceState *s
     return launch_pdl(paged_decode_kernel<CT, D, HW, A32, true>, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a,
                       maps.k, maps.v, st->err_word);
   }
-  return launch_pdl(paged_decode_kernel<CT, D, HW, A32, false>, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a, maps.k, maps.v, st->err_word);
+  return launch_pdl(paged_decode_kernel<CT, D, HW, A32, false>, dim3((unsigned)a.max_ctas), kBlock, C::SMEM, s, who, a,
+                    maps.k, maps.v, st->err_word);
 }
 
 template <int CT, int D, int HW, bool A32>
@@ -982,10 +984,9 @@ tb_status run(AttnArgs &a, const tb_paged_cache *cache, const DeviceState *st, c
   a.prefix.few = items <= st->sm_count && own <= kJoinTiles;
   if (!a.prefix.few && lead <= kLeadTiles && lead * items <= kLeadUnits) {
     a.lead = (int)lead;
-  } else if (a.prefix_len == 0) {
-  } else if (CT != TB_F32 && a.prefix.rows >= kTensorRows) {
+  } else if (lead > 0 && CT != TB_F32 && a.prefix.rows >= kTensorRows) {
     TB_TRY(launch_prefix_tc(a, maps, CT, D, st, s, who));
-  } else {
+  } else if (lead > 0) {
     switch (head_warps(a.prefix.rows)) {
       case 1: TB_TRY((launch_prefix<CT, D, 1, A32>(a, maps, st, s, who))); break;
       case 2: TB_TRY((launch_prefix<CT, D, 2, A32>(a, maps, st, s, who))); break;

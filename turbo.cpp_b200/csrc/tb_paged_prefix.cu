@@ -4,14 +4,14 @@
 // All sequences' query heads of one key/value head are the rows of a matrix
 // product against the prefix: S = Q K^T, P = exp2(scale S - m), O = P V, with
 // the running maximum m and sum l of each row; each CTA takes a share of the
-// keys and leaves (m, l, acc) per row, which the kernel of the sequences' own
-// keys joins.
+// keys and leaves (m, l, acc) per row, which are joined with the sequences' own
+// keys' later.
 //
 // Accuracy: operands in parts as in tb_paged_attention.cu (a query in QT, a
 // probability in PT parts, one each with 16-bit activations, where a
 // probability is rounded to the cache's type as the output will be; fp16
 // probabilities are scaled by 2^15).  The parts are further MMAs into the same
-// accumulator.  With fp32 activations O starts from zero for each tile and is
+// accumulator, the smallest first.  With fp32 activations O starts from zero for each tile and is
 // added to fp32 registers (one FMA with the rescaling), so no long sum runs
 // inside the tensor core, whose accumulator cuts off rather than rounds (2^-24 a
 // step: some 1e-5 over a share of the keys).  With 16-bit activations, whose
@@ -319,11 +319,11 @@ __global__ void __launch_bounds__(kBlock, 1)
         fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int p = 0; p < C::QT; ++p)
+          for (int p = C::QT - 1; p >= 0; --p)  // the smallest part first: the accumulator cuts off at its own size
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
               mma_ss(to, qd + ((p * C::CB + i / 4) * kRows * 8 + (i % 4) * 2), kd + ((i / 4) * C::KT * 8 + (i % 4) * 2),
-                     C::IDESC_QK, p + i > 0);
+                     C::IDESC_QK, p < C::QT - 1 || i > 0);
           commit_to(&ctl.s_full[w][j % C::NB]);
           commit_to(&ctl.kempty[s]);
         }
@@ -349,13 +349,13 @@ __global__ void __launch_bounds__(kBlock, 1)
         const uint64_t vd = desc(v, C::KT * 128);  // 16 keys further: 2048 bytes
         if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < C::KT / 16; ++i) {
-            if (i >= steps) break;
+          for (int p = C::QT - 1; p >= 0; --p)
 #pragma unroll
-            for (int p = 0; p < C::QT; ++p)
+            for (int i = 0; i < C::KT / 16; ++i) {
+              if (i >= steps) break;
               mma_ts(ts + C::O, p0 + C::pcol(p, i / 2) + 8 * (i % 2), vd + i * 128, C::IDESC_PV,
-                     p + i > 0 || (!C::SUMS && j > 0));
-          }
+                     p < C::QT - 1 || i > 0 || (!C::SUMS && j > 0));
+            }
           commit_to(&ctl.vempty[s]);
           commit_to(&ctl.o_full[w][j % C::NB]);
         }

@@ -492,9 +492,12 @@ tb_status tb_paged_attention_decode(const tb_paged_cache *cache, const tb_paged_
  * prefix_len tokens, held once: its pages are prefix_table_dev[0 ..
  * ceil(prefix_len / page_size) - 1], and seqs describes what follows it
  * (lens[b] >= 0 keys of each sequence behind the prefix, in pages of their
- * own; token i there has position prefix_len + i).  Every key and value of the
- * prefix is read once for all sequences.  prefix_len 0 is
- * tb_paged_attention_decode. */
+ * own; token i there has position prefix_len + i).  The keys and values of a
+ * long prefix are read once for all sequences, those of a short one (up to 512
+ * keys or so) once per sequence, from L2.  prefix_len 0 is
+ * tb_paged_attention_decode.  With TB_F16 or TB_BF16 activations and 33 and more
+ * query rows (batch * heads / kv_heads) a probability is rounded to the cache's
+ * type. */
 tb_status tb_paged_attention_shared(const tb_paged_cache *cache, const tb_paged_batch *seqs,
                                     const int32_t *prefix_table_dev, int64_t prefix_len, int act_dtype,
                                     const void *q_dev, int64_t ldq, int64_t heads, float scale, void *out_dev,

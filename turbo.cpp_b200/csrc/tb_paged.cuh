@@ -265,8 +265,9 @@ struct AttnArgs {
   int box_shift;  // a TMA box holds 1 << box_shift tokens
 };
 
-// Sets the prefix's splits: `want`, at least 1, as far as the workspace holds their results.
-void set_prefix_splits(AttnArgs &a, int64_t want);
+// Sets the prefix's splits: as few as finish first, `items` row tiles of `tiles` key tiles each on `ctas` CTAs at a
+// time, as far as the workspace holds their results.
+void set_prefix_splits(AttnArgs &a, int64_t items, int64_t tiles, int64_t ctas);
 
 // A launch that may begin while the kernel before it ends; the kernel waits
 // (griddepcontrol.wait) before it reads what that one wrote.

@@ -63,7 +63,11 @@ namespace tb {
 namespace {
 
 constexpr int kMaxCtas = 448;                    // of a decode launch (counters and partial slots)
-constexpr int64_t kPrefixRows = 2 * 148 * 128;   // extra (row, split) pairs of prefix partials
+// (row, part) pairs behind a prefix that the workspace holds: two parts of every row, and more of them as long as that
+// is not much memory.
+constexpr int64_t prefix_pairs(int64_t rows) {
+  return 2 * rows + 2 * 148 * 128 + (rows < (1 << 17) ? 2 * rows : (1 << 18));
+}
 constexpr int kWarps = 4;                        // computing warps
 constexpr int kThreads = kWarps * 32;            // their threads
 constexpr int kBlock = kThreads + 32;            // and one warp that loads
@@ -909,7 +913,7 @@ struct Layout {
 };
 Layout layout_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D) {
   const size_t slots = 2 * kMaxCtas * 8 * (size_t)head_warps(heads / kv_heads);
-  const size_t rows = (size_t)(2 * batch * heads + kPrefixRows);
+  const size_t rows = (size_t)prefix_pairs(batch * heads);
   Layout l;
   l.slot_acc = up256(kMaxCtas * sizeof(int));
   l.slot_ml = l.slot_acc + up256(slots * D * sizeof(float));
@@ -960,8 +964,7 @@ tb_status launch_prefix(AttnArgs &a, const PagedMaps &maps, const DeviceState *s
   const int row_tiles = (a.prefix.rows + C::R - 1) / C::R;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
-  // one wave of CTAs
-  set_prefix_splits(a, std::min<int64_t>(tiles, ctas / items));
+  set_prefix_splits(a, items, tiles, ctas);
   return launch_pdl(kern, dim3((unsigned)row_tiles, (unsigned)a.prefix.splits, (unsigned)a.kv_heads), kBlock, C::SMEM, s,
                     who, a, maps.k, maps.v, st->err_word);
 }
@@ -1059,9 +1062,18 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
 
 }  // namespace
 
-void set_prefix_splits(AttnArgs &a, int64_t want) {
-  const int64_t most = 1 + kPrefixRows / ((int64_t)a.prefix.rows * a.kv_heads);
-  a.prefix.splits = (int)std::min(std::max<int64_t>(want, 1), most);
+// Measured against one wave of CTAs wherever that many items are: 300 x 128 heads behind 8192 keys of 64 (152 row tiles)
+// 191 us, with one split 239; 2 x 32 heads (8 row tiles) 12.5 and 15.0.
+void set_prefix_splits(AttnArgs &a, int64_t items, int64_t tiles, int64_t ctas) {
+  constexpr int64_t kStart = 6;  // a CTA's start and end, in tiles
+  const int64_t rows = (int64_t)a.prefix.rows * a.kv_heads;
+  const int64_t most = std::min(prefix_pairs(rows) / rows - 1, tiles);
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t time = (items * n + ctas - 1) / ctas * ((tiles + n - 1) / n + kStart);
+    if (time < least) best = n, least = time;
+  }
+  a.prefix.splits = (int)best;
   a.prefix.parts = a.prefix.splits + 1;
 }
 

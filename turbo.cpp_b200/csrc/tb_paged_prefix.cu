@@ -575,7 +575,7 @@ tb_status launch(AttnArgs &a, const PagedMaps &maps, const DeviceState *st, cuda
   const int row_tiles = (a.prefix.rows + rows - 1) / rows;
   const int tiles = (a.prefix_len + C::KT - 1) / C::KT;
   const int64_t items = (int64_t)row_tiles * a.kv_heads;
-  set_prefix_splits(a, std::min<int64_t>(tiles, st->sm_count / items));
+  set_prefix_splits(a, items, tiles, st->sm_count);
   return launch_pdl(kern, dim3((unsigned)row_tiles, (unsigned)a.prefix.splits, (unsigned)a.kv_heads), kBlock, smem, s,
                     who, a, pair, maps.k, maps.v, st->err_word);
 }

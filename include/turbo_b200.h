@@ -480,7 +480,8 @@ tb_status tb_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64
  * TB_F32 or the cache's.  head_dim 64 or 128, any number of query heads per
  * key/value head; batch * heads up to 2^24, and times max_pages * page_size up
  * to 2^36.  Accumulated in fp32; TB_F32 results are accurate to fp32 (no
- * operand is rounded below 22 bits).  Keys, values and queries in use are
+ * operand is rounded below 22 bits); with TB_F16 and TB_BF16 activations a
+ * probability is held in two parts of that type.  Keys, values and queries in use are
  * finite; what lies behind a sequence's last key is never used.  A length
  * below 0 or above max_pages * page_size counts as 0, a page id outside the
  * pool reads as zeros, and both set bit 1 of the device error word.  The result
@@ -495,9 +496,7 @@ tb_status tb_paged_attention_decode(const tb_paged_cache *cache, const tb_paged_
  * own; token i there has position prefix_len + i).  The keys and values of a
  * long prefix are read once for all sequences, those of a short one (up to 512
  * keys or so) once per sequence, from L2.  prefix_len 0 is
- * tb_paged_attention_decode.  With TB_F16 or TB_BF16 activations and 33 and more
- * query rows (batch * heads / kv_heads) a probability is rounded to the cache's
- * type. */
+ * tb_paged_attention_decode, whose accuracy this call has for any batch. */
 tb_status tb_paged_attention_shared(const tb_paged_cache *cache, const tb_paged_batch *seqs,
                                     const int32_t *prefix_table_dev, int64_t prefix_len, int act_dtype,
                                     const void *q_dev, int64_t ldq, int64_t heads, float scale, void *out_dev,

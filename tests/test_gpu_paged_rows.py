@@ -1,0 +1,61 @@
+"""Attention over the paged cache, held to what single keys and single bits add.
+
+Tolerances as in test_gpu_paged.py, with these for 16-bit activations: a
+probability is two parts of the cache's type, each to nearest, so it is off by
+at most (eps/2)^2 of itself; a tensor core's accumulator is read out after 512
+steps at most, each off by at most one unit of 2^-23."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+import turbo_b200 as T  # noqa: E402
+from test_gpu_paged import (PAIRS, SHARED, TYPES, Batch, _no_errors_left, check_rows, cuda_i32, exact,  # noqa: E402,F401
+                            get_rows, put_rows, randn, workspace)
+
+STEPS = 512 * 2 ** -23
+
+
+def rows_of(x, out, lens=None):
+    """Each sequence's keys and values (the prefix first) and its output rows."""
+    pk, pv = (get_rows(p, x.prefix, x.page, x.n_prefix) for p in (x.kp, x.vp))
+    for b, n in enumerate(x.lens if lens is None else lens):
+        k, v = (torch.cat((y, get_rows(p, x.table[b], x.page, n))) for y, p in ((pk, x.kp), (pv, x.vp)))
+        yield b, k, v, out[b, :x.heads * x.dim].view(x.heads, x.dim)
+
+
+def check_two_parts(x, out):
+    torch.cuda.synchronize()
+    assert T.take_device_errors() == 0
+    p_eps = (torch.finfo(x.ct).eps / 2) ** 2
+    off, least = [], []
+    for b, k, v, got in rows_of(x, out):
+        want, tol = exact(x.rows()[b], k, v, x.scale, p_eps)
+        off.append(got.double() - want)
+        least.append(want.to(x.act).double() - want)
+        if k.shape[0]:  # the steps, relative to sum p |v|
+            tol = tol + exact(x.rows()[b], k, v.abs(), x.scale)[0] * STEPS
+        check_rows(got, want, tol, x.act)
+    # The roundings of parts are independent of each other, so that they add up like the outputs themselves and stay
+    # below (eps/2)^2 of them; the steps take up to 2^-15 of them off.  Beside the output's own rounding, an eighth of a
+    # step of fp16 and 0.3 of it in the mean, that is a few per cent.  (One part: 39 % more.)
+    assert torch.cat(off).norm() <= 1.1 * torch.cat(least).norm()
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [1, 32, 33, 128, 129, 300])
+def test_16_bit_activations_keep_two_parts(rows, dim, act):
+    """However many rows a batch has, and whichever kernel reads its prefix."""
+    for prefix in (259, 643, 5000):
+        x = Batch(act, act, 1, 1, dim, 16, "token", [b % 2 for b in range(rows)], prefix, seed=rows)
+        check_two_parts(x, x.run(shared=True))
+
+
+@pytest.mark.parametrize("lens", [[0, 3, 64, 65, 200], [5, 0]])
+@pytest.mark.parametrize("prefix", [1, 65, 500])
+@pytest.mark.parametrize("act,dim", [("f16", 64), ("bf16", 128)])
+def test_16_bit_activations_behind_a_short_prefix_keep_two_parts(act, dim, prefix, lens):
+    x = Batch(act, act, 4, 2, dim, 16, "head", lens * 40, prefix, seed=prefix)
+    check_two_parts(x, x.run(shared=True))

@@ -8,9 +8,9 @@
 // keys' later.
 //
 // Accuracy: operands in parts as in tb_paged_attention.cu (a query in QT, a
-// probability in PT parts, one each with 16-bit activations, where a
-// probability is rounded to the cache's type as the output will be; fp16
-// probabilities are scaled by 2^15).  The parts are further MMAs into the same
+// probability in PT parts; with 16-bit activations one and two, so that a
+// sequence's results do not get coarser with the batch; fp16 probabilities are
+// scaled by 2^15).  The parts are further MMAs into the same
 // accumulator, the smallest first.  With fp32 activations O starts from zero for each tile and is
 // added to fp32 registers (one FMA with the rescaling), so no long sum runs
 // inside the tensor core, whose accumulator cuts off rather than rounds (2^-24 a
@@ -31,12 +31,13 @@
 //   parts at head_dim 128 leave room for one buffer only).
 // Bounds for 64 keys and two row tiles (cycles per SM): exponentials 1024 on the
 // special function units (a polynomial on the FMA units for some of them gained
-// nothing: 0, 1/8 .. 4/8 of them measured 81, 80, 81, 83, 85 us); products 320 at
-// head_dim 64 and 640 at 128 per row tile (Q is read from shared memory at 128
-// bytes a cycle, 1.5 times the tensor cores' own time for S).  Measured (bf16,
-// 512 rows per key/value head of 128): 1570 cycles, 47 us for 32768 keys of 8
-// heads, 96 us with the sequences' own keys and the joins; the same with heads of
-// 64 74 us; 64 sequences behind 8192 fp16 keys of 64, fp32 queries 34 us.  Two row
+// nothing: 0, 1/8 .. 4/8 of them measured 81, 80, 81, 83, 85 us); products with
+// two parts of a probability 448 at head_dim 64 and 896 at 128 per row tile (Q is
+// read from shared memory at 128 bytes a cycle, 1.5 times the tensor cores' own
+// time for S).  Measured, with the sequences' own keys and the joins (512 rows of
+// each of 8 key/value heads behind 32768 keys): bf16 heads of 128 105 us, of 64 80
+// us; with probabilities in one part, which rounds outputs 1.4 times as far, 97.6
+// and 74.  64 sequences behind 8192 fp16 keys of 64, fp32 queries 34 us.  Two row
 // tiles as streams or alternate keys: 80 and 127 us; 33.8 and 35.5 even where the
 // second tile has 8 rows.
 #include <algorithm>
@@ -137,9 +138,10 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
 template <int CT_, int D, bool A32>
 struct TC {
   static constexpr int CT = CT_;
-  static constexpr int QT = !A32 ? 1 : CT == TB_F16 ? 2 : 3;  // parts of a query and of a probability
+  static constexpr int QT = !A32 ? 1 : CT == TB_F16 ? 2 : 3;  // parts of a query
+  static constexpr int PT = A32 ? QT : 2;                     // parts of a probability
   static constexpr int KT = 64;                               // keys per tile
-  static constexpr int NB = QT == 3 && D == 128 ? 1 : 2;      // buffers of S
+  static constexpr int NB = PT == 3 && D == 128 ? 1 : 2;      // buffers of S
   static constexpr bool SUMS = A32;                           // O summed in registers, tile by tile
   static constexpr bool PAIR_FITS = QT * D <= 192;            // the queries of two row tiles in shared memory
   static constexpr int RB = 2 * D, CB = D / 64;               // bytes and 128-byte columns of a row
@@ -153,11 +155,11 @@ struct TC {
   // D fp32, A and B of type F; N, M = 128; the second product's B is MN-major
   static constexpr uint32_t IDESC_QK = (1u << 4) | (F << 7) | (F << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
   static constexpr uint32_t IDESC_PV = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-  static constexpr int BUF = QT == 3 ? 96 : 64;              // columns of a buffer of S and P
-  static constexpr int O = QT == 3 && D == 64 ? 192 : 128;  // column of a stream's O
+  static constexpr int BUF = PT == 3 ? 96 : 64;              // columns of a buffer of S and P
+  static constexpr int O = PT == 3 && D == 64 ? 192 : 128;  // column of a stream's O
   static_assert(NB * BUF <= O && O + D <= 256, "");
   static __device__ __forceinline__ int pcol(int part, int chunk) {
-    return QT == 1 ? 16 * chunk : part < 2 ? 32 * chunk + 16 * part : 64 + 16 * chunk;
+    return part < 2 ? 32 * chunk + 16 * part : 64 + 16 * chunk;
   }
 };
 
@@ -349,12 +351,12 @@ __global__ void __launch_bounds__(kBlock, 1)
         const uint64_t vd = desc(v, C::KT * 128);  // 16 keys further: 2048 bytes
         if (elect_one()) {
 #pragma unroll
-          for (int p = C::QT - 1; p >= 0; --p)
+          for (int p = C::PT - 1; p >= 0; --p)
 #pragma unroll
             for (int i = 0; i < C::KT / 16; ++i) {
               if (i >= steps) break;
               mma_ts(ts + C::O, p0 + C::pcol(p, i / 2) + 8 * (i % 2), vd + i * 128, C::IDESC_PV,
-                     p < C::QT - 1 || i > 0 || (!C::SUMS && j > 0));
+                     p < C::PT - 1 || i > 0 || (!C::SUMS && j > 0));
             }
           commit_to(&ctl.vempty[s]);
           commit_to(&ctl.o_full[w][j % C::NB]);
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(kBlock, 1)
           sum[i & 1] = add2(sum[i & 1], pack2(p[2 * i], p[2 * i + 1]));
         }
 #pragma unroll
-        for (int k = 0; k < C::QT; ++k) {
+        for (int k = 0; k < C::PT; ++k) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) w[i] = pack_rest<CT>(p[2 * i], p[2 * i + 1]);

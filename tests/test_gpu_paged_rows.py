@@ -59,3 +59,26 @@ def test_16_bit_activations_keep_two_parts(rows, dim, act):
 def test_16_bit_activations_behind_a_short_prefix_keep_two_parts(act, dim, prefix, lens):
     x = Batch(act, act, 4, 2, dim, 16, "head", lens * 40, prefix, seed=prefix)
     check_two_parts(x, x.run(shared=True))
+
+
+@pytest.mark.parametrize("act,dim", [("f16", 64), ("f16", 128), ("bf16", 64)])
+def test_many_rows_behind_a_very_long_prefix(act, dim):
+    """So many rows that one CTA takes 2^20 keys (one page, again and again) by itself."""
+    page, times, group, batch = 1024, 1024, 64, 592
+    kp, vp = (torch.zeros((1, page, 1, dim), dtype=TYPES[act], device="cuda") for _ in range(2))
+    kp[0] = randn((page, 1, dim), 1).cuda().to(TYPES[act])
+    vp[0] = (1 + torch.rand((page, 1, dim), generator=torch.Generator().manual_seed(2))).cuda().to(TYPES[act])
+    q = randn((batch, group * dim), 3, 0.25).cuda().to(TYPES[act])
+    lens, table = cuda_i32([0] * batch), cuda_i32(np.zeros((batch, 1)))
+    prefix = cuda_i32([0] * times)
+    ws, out = workspace(batch, group, 1, dim), torch.zeros_like(q)
+    c, b = T.paged_cache(kp, vp), T.paged_batch(lens, table)
+    scale = dim ** -0.5
+    T.call("tb_paged_attention_shared", T.byref(c), T.byref(b), T.ptr(prefix), page * times, T.dtype_code(q), T.ptr(q),
+           group * dim, group, scale, T.ptr(out), group * dim, T.ptr(ws), ws.numel(), T.stream_handle())
+    torch.cuda.synchronize()
+    assert T.take_device_errors() == 0
+    rows = q.view(-1, dim)  # equal keys: the softmax over one page is the softmax over all of them
+    want, tol = exact(rows, kp[0], vp[0], scale, (torch.finfo(TYPES[act]).eps / 2) ** 2)
+    # read-outs: 2^20 keys are 16384 tiles, 64 at a time added in fp32
+    check_rows(out.view(-1, dim), want, tol + want * (STEPS + 16384 / 64 * 2 ** -24), TYPES[act])

@@ -14,9 +14,11 @@
 // accumulator, the smallest first.  With fp32 activations O starts from zero for each tile and is
 // added to fp32 registers (one FMA with the rescaling), so no long sum runs
 // inside the tensor core, whose accumulator cuts off rather than rounds (2^-24 a
-// step: some 1e-5 over a share of the keys).  With 16-bit activations, whose
-// outputs are rounded to 2^-9 or 2^-12, O stays in tensor memory for the whole
-// share and is rescaled only where a row's maximum has grown by 2^8.
+// step: some 1e-5 over a thousand keys).  With 16-bit activations, whose
+// outputs are rounded to 2^-9 or 2^-12, O stays in tensor memory for KEEP tiles
+// (512 steps, 2^-15 at most) before it is added to an fp32 sum in local memory
+// (in registers, although untouched, it cost 3 % of every call), and is rescaled
+// only where a row's maximum has grown by 2^8.
 //
 // Roles: two streams, each a warpgroup whose threads own one row each (TMEM
 // lane = row), and one warp issuing its MMAs; one warp loading.  A stream's
@@ -35,7 +37,7 @@
 // two parts of a probability 448 at head_dim 64 and 896 at 128 per row tile (Q is
 // read from shared memory at 128 bytes a cycle, 1.5 times the tensor cores' own
 // time for S).  Measured, with the sequences' own keys and the joins (512 rows of
-// each of 8 key/value heads behind 32768 keys): bf16 heads of 128 105 us, of 64 80
+// each of 8 key/value heads behind 32768 keys): bf16 heads of 128 105 us, of 64 82
 // us; with probabilities in one part, which rounds outputs 1.4 times as far, 97.6
 // and 74.  64 sequences behind 8192 fp16 keys of 64, fp32 queries 34 us.  Two row
 // tiles as streams or alternate keys: 80 and 127 us; 33.8 and 35.5 even where the
@@ -143,6 +145,7 @@ struct TC {
   static constexpr int KT = 64;                               // keys per tile
   static constexpr int NB = PT == 3 && D == 128 ? 1 : 2;      // buffers of S
   static constexpr bool SUMS = A32;                           // O summed in registers, tile by tile
+  static constexpr int KEEP = SUMS ? 1 : 512 / (PT * KT / 16);  // tiles whose O is summed in tensor memory
   static constexpr bool PAIR_FITS = QT * D <= 192;            // the queries of two row tiles in shared memory
   static constexpr int RB = 2 * D, CB = D / 64;               // bytes and 128-byte columns of a row
   static constexpr int QTILE = QT * CB * kRows * 128;
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(kBlock, 1)
             for (int i = 0; i < C::KT / 16; ++i) {
               if (i >= steps) break;
               mma_ts(ts + C::O, p0 + C::pcol(p, i / 2) + 8 * (i % 2), vd + i * 128, C::IDESC_PV,
-                     p < C::PT - 1 || i > 0 || (!C::SUMS && j > 0));
+                     p < C::PT - 1 || i > 0 || j % C::KEEP > 0);
             }
           commit_to(&ctl.vempty[s]);
           commit_to(&ctl.o_full[w][j % C::NB]);
@@ -404,6 +407,23 @@ __global__ void __launch_bounds__(kBlock, 1)
         tmem_st32(ts + C::O + 32 * c, o);
       }
     };
+    // not SUMS: the sum of the O before the present one, and the factor that it still needs
+    float kept[C::SUMS ? 1 : D], kept_f = 0.f;
+    auto keep_o = [&](bool first) {
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(ts + C::O + 32 * c, o);
+        tmem_wait_ld();
+        loaded(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float &x = kept[C::SUMS ? 0 : 32 * c + i];
+          x = first ? __uint_as_float(o[i]) : fmaf(x, kept_f, __uint_as_float(o[i]));
+        }
+      }
+      kept_f = 1.f;
+    };
     const int first = pair ? 0 : stream, mine = (n - first + step - 1) / step;
     auto wait_o = [&](int j) { wait_phase(&ctl.o_full[stream][j % C::NB], (j / C::NB) & 1, err, dead); };
     float before = 1.f;  // SUMS: the factor that the sums before the last tile's O still need
@@ -440,6 +460,11 @@ __global__ void __launch_bounds__(kBlock, 1)
       } else if (j == 0) {
         m = top;
       } else {
+        if (j % C::KEEP == 0) {  // the next products begin a new O
+          wait_o(j - 1);
+          fence_after();
+          keep_o(j == C::KEEP);
+        }
         // the reference maximum follows only where a row has outgrown it by 2^SLACK; its O and l are then scaled down
         const bool grown = top > m + C::SLACK;
         if (__any_sync(0xffffffffu, grown)) {
@@ -447,6 +472,7 @@ __global__ void __launch_bounds__(kBlock, 1)
           wait_o(j - 1);
           fence_after();
           scale_o(f);
+          kept_f *= f;
           l *= f;
           if (grown) m = top;
         }
@@ -505,6 +531,10 @@ __global__ void __launch_bounds__(kBlock, 1)
           loaded(o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) out[32 * c + i] = __uint_as_float(o[i]);
+        }
+        if (mine > C::KEEP) {
+#pragma unroll
+          for (int i = 0; i < D; ++i) out[i] = fmaf(kept[C::SUMS ? 0 : i], kept_f, out[i]);
         }
       }
     }

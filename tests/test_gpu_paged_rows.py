@@ -82,3 +82,13 @@ def test_many_rows_behind_a_very_long_prefix(act, dim):
     want, tol = exact(rows, kp[0], vp[0], scale, (torch.finfo(TYPES[act]).eps / 2) ** 2)
     # read-outs: 2^20 keys are 16384 tiles, 64 at a time added in fp32
     check_rows(out.view(-1, dim), want, tol + want * (STEPS + 16384 / 64 * 2 ** -24), TYPES[act])
+
+
+def test_rows_of_a_wider_table():
+    x = Batch("f32", "f16", 4, 2, 64, 16, "token", [100, 0, 3, 40], seed=2)
+    want = x.run().clone()
+    wide = torch.full((4, x.table.shape[1] + 5), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    wide[:, 2:2 + x.table.shape[1]] = x.d_table
+    x.batch = T.paged_batch(x.d_lens, wide[:, 2:2 + x.table.shape[1]])
+    assert torch.equal(x.run(), want)
+    x.check(want)

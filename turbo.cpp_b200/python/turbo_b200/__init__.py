@@ -256,13 +256,16 @@ def paged_cache(k, v):
 
 def paged_batch(lens, table):
     """A tb_paged_batch over int32 tensors lens [batch] and table [batch,
-    max_pages].  The caller keeps the tensors."""
+    max_pages], whose rows may be those of a wider table but not overlap (as
+    those of an expanded one).  The caller keeps the tensors."""
     import torch
     if lens.dtype != torch.int32 or table.dtype != torch.int32:
         raise ValueError("paged_batch: lens and table are int32")
     if lens.dim() != 1 or not lens.is_contiguous() or table.dim() != 2 or table.shape[0] != lens.shape[0] or (
             table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("paged_batch: lens [batch], table [batch, max_pages] with contiguous rows")
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError("paged_batch: the table's rows overlap (an expanded table needs .contiguous())")
     b = PagedBatch()
     b.batch, b.lens, b.table = lens.shape[0], lens.data_ptr(), table.data_ptr()
     b.max_pages, b.table_stride = table.shape[1], max(table.stride(0), table.shape[1])

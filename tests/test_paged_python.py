@@ -10,8 +10,8 @@ LENS = torch.zeros(4, dtype=torch.int32)
 
 @pytest.mark.parametrize("table", [
     torch.zeros((1, 6), dtype=torch.int32).expand(4, 6),           # one row for all: its next row is not 6 entries on
-    torch.zeros(20, dtype=torch.int32).as_strided((4, 6), (2, 1)),  # rows that overlap
-    torch.zeros(20, dtype=torch.int32).as_strided((4, 6), (5, 1)),
+    torch.zeros(24, dtype=torch.int32).as_strided((4, 6), (2, 1)),  # rows that overlap
+    torch.zeros(24, dtype=torch.int32).as_strided((4, 6), (5, 1)),
 ])
 def test_tables_whose_rows_overlap_are_refused(table):
     with pytest.raises(ValueError, match="rows"):

@@ -16,3 +16,11 @@ LENS = torch.zeros(4, dtype=torch.int32)
 def test_tables_whose_rows_overlap_are_refused(table):
     with pytest.raises(ValueError, match="rows"):
         T.paged_batch(LENS, table)
+
+
+def test_tensors_in_host_memory_are_refused():
+    pool = torch.zeros((3, 16, 2, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        T.paged_cache(pool, pool.clone())
+    with pytest.raises(ValueError, match="GPU"):
+        T.paged_batch(LENS, torch.zeros((4, 6), dtype=torch.int32))

@@ -247,6 +247,8 @@ def paged_cache(k, v):
         raise ValueError("paged_cache: k and v need the same 4-d shape, strides and type")
     if k.shape[3] > 1 and k.stride(3) != 1:
         raise ValueError("paged_cache: the elements of a head must be contiguous")
+    if not k.is_cuda or k.device != v.device:
+        raise ValueError("paged_cache: k and v are in one GPU's memory")
     c = PagedCache()
     c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), dtype_code(k)
     c.n_pages, c.page_size, c.kv_heads, c.head_dim = k.shape
@@ -266,6 +268,8 @@ def paged_batch(lens, table):
         raise ValueError("paged_batch: lens [batch], table [batch, max_pages] with contiguous rows")
     if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
         raise ValueError("paged_batch: the table's rows overlap (an expanded table needs .contiguous())")
+    if not lens.is_cuda or lens.device != table.device:
+        raise ValueError("paged_batch: lens and table are in one GPU's memory")
     b = PagedBatch()
     b.batch, b.lens, b.table = lens.shape[0], lens.data_ptr(), table.data_ptr()
     b.max_pages, b.table_stride = table.shape[1], max(table.stride(0), table.shape[1])

@@ -104,8 +104,9 @@ tb_status tb_sync(tb_stream stream);
 tb_status tb_take_device_errors(uint32_t *flags_out);
 /* Limit, in nanoseconds, of the bounded waits of the Q4_0 matmul kernels
  * (tb_matmul_quant / tb_matmul_quant_exact with TB_Q4_0 on the CUDA cores, and
- * tb_matmul_q4_0_static_scratch); default 2e9.  A wait that gives up sets bit 0
- * of the device error word and the kernel leaves its rows unwritten, after
+ * tb_matmul_q4_0_static_scratch) and of the attention over a paged cache;
+ * default 2e9.  A wait that gives up sets bit 0 of the device error word and the
+ * kernel leaves its rows unwritten (the paged attention: undefined), after
  * waiting for its own copies in flight.  0 lets no wait wait at all, a
  * host-side way to exercise that path.  Read at launch (a captured graph keeps
  * the value it was captured with).  No reference counterpart. */
@@ -467,8 +468,8 @@ tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_paged_batch
  * needed).  Zero the workspace once before its first use and keep it: every
  * call leaves it ready for the next, of whatever batch and shape it is large
  * enough for.  It must be 256-byte aligned, and calls that can overlap on the
- * GPU need one each.  A wait inside a call that gives up (after 2 s; bit 0 of
- * the device error word) leaves that call's output undefined; zero the
+ * GPU need one each.  A wait inside a call that gives up (tb_set_wait_limit_ns;
+ * bit 0 of the device error word) leaves that call's output undefined; zero the
  * workspace again then. */
 tb_status tb_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                              size_t *bytes_out);

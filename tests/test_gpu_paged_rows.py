@@ -92,3 +92,35 @@ def test_rows_of_a_wider_table():
     x.batch = T.paged_batch(x.d_lens, wide[:, 2:2 + x.table.shape[1]])
     assert torch.equal(x.run(), want)
     x.check(want)
+
+
+def run_out(x, shared):
+    """A call whose waits all give up: it ends, says so, and leaves the context and what lies beside its rows alone."""
+    want = x.run(shared=shared)
+    torch.cuda.synchronize()
+    assert T.take_device_errors() == 0
+    T.call("tb_set_wait_limit_ns", 0)
+    try:
+        out = x.run(shared=shared)
+        torch.cuda.synchronize()
+    finally:
+        T.call("tb_set_wait_limit_ns", 2000000000)
+    assert T.take_device_errors() == 1
+    assert (out[:, x.heads * x.dim:] == 9.0).all()
+    x.ws.zero_()
+    assert torch.equal(x.run(shared=shared), want)
+    x.check(want)
+
+
+@pytest.mark.parametrize("act,ct,group,kvh,dim,lens,prefix", [
+    ("f32", "f32", 1, 1, 64, [5], 0),
+    ("f32", "f16", 4, 2, 64, [3000, 1, 0, 700], 0),       # long items over many CTAs
+    ("bf16", "bf16", 4, 8, 128, [300] * 200, 0),          # many short ones per CTA
+    ("f32", "bf16", 33, 1, 64, [2000, 64, 5], 0),
+    ("f16", "f16", 4, 2, 64, [0, 65, 3] * 40, 200),       # a short prefix
+    ("f32", "f32", 4, 8, 64, [1, 60, 0, 33], 1001),       # few rows: joined by the kernel of their own keys
+    ("f32", "f16", 4, 2, 128, [300, 5], 9000),            # few rows, joined by a kernel of its own
+    ("f32", "f32", 4, 2, 64, [40] * 70, 2000),
+])
+def test_waits_that_run_out(act, ct, group, kvh, dim, lens, prefix):
+    run_out(Batch(act, ct, group, kvh, dim, 16, "token", lens, prefix, seed=3), prefix > 0)

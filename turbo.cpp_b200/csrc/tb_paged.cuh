@@ -81,9 +81,21 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
 }
 
 // Waits for a barrier's phase; once a wait has run out (bit 0 of the error
-// word is set then), later ones return at once, so that the kernel ends.
-__device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead) {
-  if (!dead && !mbar_wait_bounded(bar, phase, err)) dead = true;
+// word is set then), later ones return at once, so that the kernel ends.  So
+// nothing that decides how often a loop runs or which barriers a thread comes to
+// is read from what such a wait orders: a call whose waits ran out multiplies
+// what is there and ends.
+__device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead,
+                                           uint64_t limit_ns = 2000000000ull) {
+  if (!dead && !mbar_wait_limit(bar, phase, err, limit_ns)) dead = true;
+}
+
+// The end of a loading warp that has issued `issued` tiles into STAGES stages:
+// its last copies have landed, even where no other warp waits for them any more.
+template <int STAGES>
+__device__ __forceinline__ void wait_copies(uint64_t *full, int issued, uint32_t *err) {
+  for (int k = max(issued - STAGES, 0); k < issued; ++k)
+    if (!mbar_wait_bounded(full + k % STAGES, (k / STAGES) & 1, err)) return;
 }
 
 // A tile of T keys or values of a sequence of len tokens, in boxes of one page.
@@ -263,6 +275,7 @@ struct AttnArgs {
   int prefix_len;
   int lead;  // tiles of a short prefix that the decode kernel takes before each sequence's own, instead of a kernel
   int box_shift;  // a TMA box holds 1 << box_shift tokens
+  uint64_t wait_ns;  // limit of the kernels' waits
 };
 
 // Sets the prefix's splits: as few as finish first, `items` row tiles of `tiles` key tiles each on `ctas` CTAs at a

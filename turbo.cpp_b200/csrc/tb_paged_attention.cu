@@ -164,8 +164,7 @@ struct Walk {
 constexpr int kMaxStages = 3;
 struct Control {
   uint64_t full[kMaxStages], empty[kMaxStages];
-  Walk at[kMaxStages];  // what each stage holds
-  Walk first;
+  Walk first, item[2];  // the CTA's first item; the computing warps' further ones in turn, the second in item[1]
   int warp_sum[kWarps + 1];
   int last[2];
 };
@@ -590,6 +589,12 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     const int x = u - more * (share + 1);
     return x < 0 ? u / (share + 1) : more + x / share;
   };
+  // the item after w's, whose sequence, where it is the next one, has next_len keys
+  auto following = [&](Walk w, int next_len) {
+    w.tile = 0;
+    if (++w.i == items) w = {w.b + 1, 0, 0, tiles_of<C>(a, next_len), next_len};
+    return w;
+  };
   const int u0 = first_unit(me), u1 = first_unit(me + 1);
   if (u0 >= before && u0 < before + mine) {
     int u = u0 - before;
@@ -598,7 +603,9 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
       const int n = tiles * items;
       if (u < n) {
         const int i = u / tiles;
-        ctl.first = {b, i, u - i * tiles, tiles, len};
+        const Walk w = {b, i, u - i * tiles, tiles, len};
+        ctl.first = w;
+        ctl.item[1] = following(w, b + 1 < a.seqs.batch ? seq_len(a.seqs, b + 1) : 0);
         break;
       }
       u -= n;
@@ -609,29 +616,25 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   bool dead = false;
 
   if (warp == kWarps) {  // ---- the loading warp
-    int stage = 0;
+    int stage = 0, u = u0;
     uint32_t phase = 1;  // the stages begin empty
     int next_len = cur.b + 1 < a.seqs.batch ? seq_len(a.seqs, cur.b + 1) : 0;
-    for (int u = u0; u < u1; ++u) {
+    for (; u < u1; ++u) {
       const bool own = cur.tile >= a.lead;
       const int32_t *table = own ? a.seqs.table + (int64_t)cur.b * a.seqs.table_stride : a.prefix_table;
       const int tile = own ? cur.tile - a.lead : cur.tile;
       const TileBoxes box =  // before the wait
           tile_boxes<C::T>(a.pools, a.box_shift, table, own ? cur.len : a.prefix_len, tile);
-      wait_phase(&ctl.empty[stage], phase, err, dead);
-      if (lane == 0) ctl.at[stage] = cur;
+      wait_phase(&ctl.empty[stage], phase, err, dead, a.wait_ns);
+      if (__any_sync(0xffffffffu, dead)) break;
       load_rows<C::T, C::RB, Word<CT>::size>(stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools,
                                              a.box_shift, table, box, tile, cur.i / a.head_groups, err);
       if (++stage == C::STAGES) stage = 0, phase ^= 1;
       if (++cur.tile < cur.tiles) continue;
-      cur.tile = 0;
-      if (++cur.i < items) continue;
-      cur.i = 0;
-      ++cur.b;
-      cur.len = next_len;
-      cur.tiles = tiles_of<C>(a, next_len);
-      if (cur.b + 1 < a.seqs.batch) next_len = seq_len(a.seqs, cur.b + 1);
+      cur = following(cur, next_len);
+      if (cur.i == 0 && cur.b + 1 < a.seqs.batch) next_len = seq_len(a.seqs, cur.b + 1);
     }
+    wait_copies<C::STAGES>(ctl.full, u - u0, err);
     pdl_wait();
     return;
   }
@@ -689,7 +692,11 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   // the items that this CTA shares with others: its first, begun before u0, and its last, unfinished at u1
   Walk cut[2];
   int cut_unit[2] = {-1, -1};  // the item's first unit
-  for (int u = u0; u < u1;) {
+  // The items after the first are found by the first warp, one ahead of their use, and read behind the barrier of a join:
+  // all warps agree on them whatever became of the tiles.
+  int odd = 0, next_len = 0;  // parity of this item; keys of the sequence behind the next item's
+  if (warp == 0 && ctl.item[1].b + 1 < a.seqs.batch) next_len = seq_len(a.seqs, ctl.item[1].b + 1);
+  for (int u = u0; u < u1; odd ^= 1) {
     const Walk item = cur;
     const int item0 = u - item.tile, end = min(u1, item0 + item.tiles);
     if (!JOIN && a.prefix.splits > 0 && tid == 0 && item0 >= u0)
@@ -698,7 +705,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     reset(s);
     load_q(s, qf, a.scale2);
     for (; u < end; ++u) {
-      wait_phase(&ctl.full[stage], phase, err, dead);
+      wait_phase(&ctl.full[stage], phase, err, dead, a.wait_ns);
       const int tile = u - item0 - a.lead;  // of the sequence's own; below 0 of the prefix
       const int keys = tile < 0 ? a.prefix_len - (tile + a.lead) * C::T : item.len - tile * C::T;
       warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, keys), kw);
@@ -707,9 +714,13 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
       if (++stage == C::STAGES) stage = 0, phase ^= 1;
     }
     if (u < u1) {  // the next item's queries arrive during this one's joins
-      wait_phase(&ctl.full[stage], phase, err, dead);
-      cur = ctl.at[stage];
+      cur = ctl.item[odd ^ 1];
       fetch_q<C>(qf, a.q, q_at(cur));
+      if (warp == 0) {
+        const Walk w = following(cur, next_len);
+        if (lane == 0) ctl.item[odd] = w;
+        if (w.i == 0 && w.b + 1 < a.seqs.batch) next_len = seq_len(a.seqs, w.b + 1);
+      }
     }
     leave(s, merge);
     computing_warps_sync();
@@ -808,15 +819,17 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   const int t1 = (int)((int64_t)(split + 1) * tiles / a.prefix.splits);
   bool dead = false;
   if (warp == kWarps) {
-    int stage = 0;
+    int stage = 0, t = t0;
     uint32_t phase = 1;
-    for (int t = t0; t < t1; ++t) {
-      wait_phase(&ctl.empty[stage], phase, err, dead);
+    for (; t < t1; ++t) {
+      wait_phase(&ctl.empty[stage], phase, err, dead, a.wait_ns);
+      if (__any_sync(0xffffffffu, dead)) break;
       load_rows<C::T, C::RB, Word<CT>::size>(
           stages + (uint32_t)stage * C::STAGE, &ctl.full[stage], &km, &vm, a.pools, a.box_shift, a.prefix_table,
           tile_boxes<C::T>(a.pools, a.box_shift, a.prefix_table, a.prefix_len, t), t, kvh, err);
       if (++stage == C::STAGES) stage = 0, phase ^= 1;
     }
+    wait_copies<C::STAGES>(ctl.full, t - t0, err);
     return;
   }
   const int hw = warp % HW, kw = warp / HW;
@@ -832,7 +845,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   int stage = 0;
   uint32_t phase = 0;
   for (int t = t0; t < t1; ++t) {
-    wait_phase(&ctl.full[stage], phase, err, dead);
+    wait_phase(&ctl.full[stage], phase, err, dead, a.wait_ns);
     warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw);
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.empty[stage]);
@@ -1051,6 +1064,7 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
   a.prefix.rows = (int)(B * a.group);
   a.prefix_table = prefix_table;
   a.prefix_len = (int)prefix_len;
+  a.wait_ns = wait_limit_ns();
 #define TB_RUN(CT, A32) return D == 64 ? run<CT, 64, A32>(a, cache, st, stream, who) : run<CT, 128, A32>(a, cache, st, stream, who)
   if (act_dtype == TB_F16) TB_RUN(TB_F16, false);
   if (act_dtype == TB_BF16) TB_RUN(TB_BF16, false);

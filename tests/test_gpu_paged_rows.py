@@ -124,3 +124,14 @@ def run_out(x, shared):
 ])
 def test_waits_that_run_out(act, ct, group, kvh, dim, lens, prefix):
     run_out(Batch(act, ct, group, kvh, dim, 16, "token", lens, prefix, seed=3), prefix > 0)
+
+
+@pytest.mark.parametrize("act,ct,group,kvh,dim,batch,prefix", [
+    ("bf16", "bf16", 4, 8, 128, 100, 9000),  # two row tiles a CTA
+    ("f16", "f16", 4, 2, 64, 20, 3000),      # one, alternate keys
+    ("f32", "f16", 4, 8, 64, 64, 5000),
+    ("f32", "f16", 4, 1, 128, 64, 700),
+    ("f32", "bf16", 4, 2, 128, 64, 2000),    # one buffer of scores
+])
+def test_waits_that_run_out_on_tcgen05(act, ct, group, kvh, dim, batch, prefix):
+    run_out(Batch(act, ct, group, kvh, dim, 16, "token", [b % 3 for b in range(batch)], prefix, seed=4), True)

@@ -86,8 +86,14 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
 // is read from what such a wait orders: a call whose waits ran out multiplies
 // what is there and ends.
 __device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead,
-                                           uint64_t limit_ns = 2000000000ull) {
-  if (!dead && !mbar_wait_limit(bar, phase, err, limit_ns)) dead = true;
+                                           uint64_t limit_ns) {
+  if (!dead && !mbar_wait_bounded(bar, phase, err, limit_ns)) dead = true;
+}
+// What `dead` begins as in a warp: with a limit of 0 no wait may wait at all.  (Asked at each wait, the limit cost the
+// tensor cores' loop 3 to 5 %.)
+__device__ __forceinline__ bool begin_dead(uint64_t limit_ns, uint32_t *err) {
+  if (limit_ns == 0 && (threadIdx.x & 31) == 0) atomicOr(err, ERR_TIMEOUT);
+  return limit_ns == 0;
 }
 
 // The end of a loading warp that has issued `issued` tiles into STAGES stages:

@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   }
   __syncthreads();
   Walk cur = ctl.first;
-  bool dead = false;
+  bool dead = begin_dead(a.wait_ns, err);
 
   if (warp == kWarps) {  // ---- the loading warp
     int stage = 0, u = u0;
@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
   const int tiles = (a.prefix_len + C::T - 1) / C::T;
   const int t0 = (int)((int64_t)split * tiles / a.prefix.splits);
   const int t1 = (int)((int64_t)(split + 1) * tiles / a.prefix.splits);
-  bool dead = false;
+  bool dead = begin_dead(a.wait_ns, err);
   if (warp == kWarps) {
     int stage = 0, t = t0;
     uint32_t phase = 1;

@@ -171,6 +171,7 @@ struct PrefixControl {
   // per stream and buffer of S (a barrier then never runs a whole phase ahead of a waiter that skips one: tile j's
   // scores imply the products of tile j - NB)
   uint64_t s_full[2][2], p_full[2][2], o_full[2][2];
+  uint64_t done[2];  // per stream: all products
   uint32_t tmem;
   float down[2 * kRows];  // fp32 queries of an fp16 cache: 2^-e of each row
 };
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       mbar_init(&ctl.p_full[w][1], kRows);
       mbar_init(&ctl.o_full[w][0], 1);
       mbar_init(&ctl.o_full[w][1], 1);
+      mbar_init(&ctl.done[w], 1);
     }
     fence_mbar_init();
   }
@@ -301,17 +303,25 @@ __global__ void __launch_bounds__(kBlock, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 8) {  // ---- loading
+      int keys = 0, values = 0;  // tiles issued
+      dead = begin_dead(a.wait_ns, err);  // (the others find out by waiting)
       for (int t = 0; t < n; ++t) {
         const int s = t % C::STAGES;
         const uint32_t ph = ((t / C::STAGES) & 1) ^ 1;
         const TileBoxes box = tile_boxes<C::KT>(a.pools, a.box_shift, a.prefix_table, a.prefix_len, t0 + t);
-        wait_phase(&ctl.kempty[s], ph, err, dead);
+        wait_phase(&ctl.kempty[s], ph, err, dead, a.wait_ns);
+        if (__any_sync(0xffffffffu, dead)) break;
         load_rows<C::KT, C::RB, 2>(stages + s * 2 * C::HALF, &ctl.kfull[s], &km, nullptr, a.pools, a.box_shift,
                                    a.prefix_table, box, t0 + t, kvh, err);
-        wait_phase(&ctl.vempty[s], ph, err, dead);
+        ++keys;
+        wait_phase(&ctl.vempty[s], ph, err, dead, a.wait_ns);
+        if (__any_sync(0xffffffffu, dead)) break;
         load_rows<C::KT, C::RB, 2>(stages + s * 2 * C::HALF + C::HALF, &ctl.vfull[s], &vm, nullptr, a.pools,
                                    a.box_shift, a.prefix_table, box, t0 + t, kvh, err);
+        ++values;
       }
+      wait_copies<C::STAGES>(ctl.kfull, keys, err);
+      wait_copies<C::STAGES>(ctl.vfull, values, err);
     } else if (warp < 11) {  // ---- products of stream w
       const int w = warp - 9, first = pair ? 0 : w, mine = (n - first + step - 1) / step;
       const uint32_t ts = tmem + w * 256, q = qs + (pair ? w * C::QTILE : 0);
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         const int t = first + j * step, s = t % C::STAGES;
         const uint32_t k = stages + s * 2 * C::HALF, to = ts + (j % C::NB) * C::BUF;
         const uint64_t kd = desc(k, 16);  // 16 elements further: 32 bytes, 2 in the descriptor's address field
-        wait_phase(&ctl.kfull[s], (t / C::STAGES) & 1, err, dead);
+        wait_phase(&ctl.kfull[s], (t / C::STAGES) & 1, err, dead, a.wait_ns);
         fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -339,7 +349,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         const int t = first + j * step, s = t % C::STAGES;
         const uint32_t v = stages + s * 2 * C::HALF + C::HALF, p0 = ts + (j % C::NB) * C::BUF;
         const int keys = min(C::KT, a.prefix_len - (t0 + t) * C::KT), steps = (keys + 15) / 16;
-        wait_phase(&ctl.vfull[s], (t / C::STAGES) & 1, err, dead);
+        wait_phase(&ctl.vfull[s], (t / C::STAGES) & 1, err, dead, a.wait_ns);
         if (keys < steps * 16) {
           // the rows of the last step behind the prefix hold whatever their page held: 0 times that has to be 0
           for (int i = lane; i < (steps * 16 - keys) * (C::RB / 16); i += 32) {
@@ -349,7 +359,7 @@ __global__ void __launch_bounds__(kBlock, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        wait_phase(&ctl.p_full[w][j % C::NB], (j / C::NB) & 1, err, dead);
+        wait_phase(&ctl.p_full[w][j % C::NB], (j / C::NB) & 1, err, dead, a.wait_ns);
         fence_after();
         const uint64_t vd = desc(v, C::KT * 128);  // 16 keys further: 2048 bytes
         if (elect_one()) {
@@ -368,6 +378,10 @@ __global__ void __launch_bounds__(kBlock, 1)
         // into the buffer whose P the products just issued read: the tensor core takes them in order
         if (j + C::NB < mine) scores(j + C::NB);
       }
+      // tensor memory is given back, and the CTA ends, only behind the last product, waited for elsewhere or not
+      if (elect_one()) commit_to(&ctl.done[w]);
+      __syncwarp();
+      mbar_wait_bounded(&ctl.done[w], 0, err);
     }
   } else {  // ---- the exponentials of stream `stream`
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -425,11 +439,11 @@ __global__ void __launch_bounds__(kBlock, 1)
       kept_f = 1.f;
     };
     const int first = pair ? 0 : stream, mine = (n - first + step - 1) / step;
-    auto wait_o = [&](int j) { wait_phase(&ctl.o_full[stream][j % C::NB], (j / C::NB) & 1, err, dead); };
+    auto wait_o = [&](int j) { wait_phase(&ctl.o_full[stream][j % C::NB], (j / C::NB) & 1, err, dead, a.wait_ns); };
     float before = 1.f;  // SUMS: the factor that the sums before the last tile's O still need
     for (int j = 0; j < mine; ++j) {
       const uint32_t sp = ts + (j % C::NB) * C::BUF;
-      wait_phase(&ctl.s_full[stream][j % C::NB], (j / C::NB) & 1, err, dead);
+      wait_phase(&ctl.s_full[stream][j % C::NB], (j / C::NB) & 1, err, dead, a.wait_ns);
       fence_after();
       uint32_t u[C::KT / 32][32];  // the row's scores
 #pragma unroll

@@ -135,3 +135,51 @@ def test_waits_that_run_out(act, ct, group, kvh, dim, lens, prefix):
 ])
 def test_waits_that_run_out_on_tcgen05(act, ct, group, kvh, dim, batch, prefix):
     run_out(Batch(act, ct, group, kvh, dim, 16, "token", [b % 3 for b in range(batch)], prefix, seed=4), True)
+
+
+@pytest.mark.parametrize("act,ct,group,kvh,batch,prefix,room", [
+    ("f16", "f16", 4, 2, 20, 1500, 8),     # 33 and more rows: the prefix on tcgen05
+    ("bf16", "bf16", 4, 8, 80, 3000, 20),
+    ("f32", "f16", 2, 2, 9, 4000, 30),     # fewer
+    ("f32", "f32", 4, 2, 3, 900, 2),       # few short sequences: joined by the kernel of their own keys
+    ("f32", "f32", 4, 2, 30, 100, 9),      # a short prefix
+])
+def test_steps_in_one_stream_without_a_host_wait(act, ct, group, kvh, batch, prefix, room):
+    """Each step changes queries and lengths in place, appends, and attends; nothing waits for the host in between."""
+    steps, dim, page = 24, 64, 16
+    own = [b % 5 for b in range(batch)]
+    x = Batch(act, ct, group, kvh, dim, page, "token", [n + steps + room for n in own], prefix, seed=batch)
+    new = [[randn((batch, h, dim), 100 * s + i).to(TYPES[act]).cuda() for i, h in enumerate((group * kvh, kvh, kvh))]
+           for s in range(steps)]
+    start = cuda_i32(own)
+    q = torch.empty_like(new[0][0])
+    cos, sin = torch.ones((64, dim // 2), device="cuda"), torch.zeros((64, dim // 2), device="cuda")
+    width = group * kvh * dim
+
+    def chain(wait):
+        sync = torch.cuda.synchronize if wait else lambda: None
+        outs = [torch.zeros_like(q) for _ in range(steps)]
+        x.d_lens.copy_(start)
+        sync()
+        for s in range(steps):
+            x.d_lens += 1
+            sync()
+            q.copy_(new[s][0])
+            sync()
+            T.call("tb_rope_paged_append", T.byref(x.cache), T.byref(x.batch), T.dtype_code(q), T.ptr(q), width,
+                   T.ptr(new[s][1]), kvh * dim, T.ptr(new[s][2]), kvh * dim, batch, group * kvh, None, T.ptr(cos),
+                   T.ptr(sin), 64, T.ptr(q), width, T.stream_handle())
+            sync()
+            T.call("tb_paged_attention_shared", T.byref(x.cache), T.byref(x.batch), T.ptr(x.d_prefix), prefix,
+                   T.dtype_code(q), T.ptr(q), width, group * kvh, x.scale, T.ptr(outs[s]), width, T.ptr(x.ws),
+                   x.ws.numel(), T.stream_handle())
+            sync()
+        torch.cuda.synchronize()
+        assert T.take_device_errors() == 0
+        return outs
+
+    want = chain(True)
+    assert not torch.equal(want[0], want[1])
+    for _ in range(5):
+        for a, b in zip(chain(False), want):
+            assert torch.equal(a, b)

@@ -57,7 +57,25 @@ struct PrefixParts {
   // else per item of that kernel: its first CTA's slot and how many CTAs share it (0: one, its part is the row's last)
   int2 *own;
   int slot_rows;  // rows of a slot
+  int *begun;     // 1 once the prefix's kernel has seen every earlier one's end; zero between calls
 };
+
+// The prefix's kernel, one thread of each CTA, behind its griddepcontrol.wait:
+// the next kernel may begin.  That one reads what earlier kernels wrote
+// (lengths, tables, pages, queries) but none of this one's results, and waits
+// for this one only at its end; what makes the earlier writes visible to it is
+// this release, which it acquires (earlier_kernels_seen).
+__device__ __forceinline__ void let_next_begin(const PrefixParts &p) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+    asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(p.begun), "r"(1) : "memory");
+  pdl_launch_dependents();
+}
+// All threads of a CTA of the next kernel: false where it has to wait for the prefix's end instead.
+__device__ __forceinline__ bool earlier_kernels_seen(const PrefixParts &p) {
+  int v = 0;
+  if (threadIdx.x == 0) asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.begun) : "memory");
+  return __syncthreads_or(v == 1) != 0;
+}
 
 // The pools as 4-d tensors [page][token][head][head_dim] for TMA: a box is up
 // to `box_rows` tokens of one page and head, 128 bytes of each row, swizzled.
@@ -114,7 +132,7 @@ __device__ __forceinline__ TileBoxes tile_boxes(const PagedPools &p, int box_shi
   const int lane = threadIdx.x & 31;
   TileBoxes b;
   b.n = (min(max(len - tile * T, 0), T) + (1 << box_shift) - 1) >> box_shift;
-  b.first = lane < b.n ? __ldg(table + ((tile * T + (lane << box_shift)) >> p.shift)) : 0;
+  b.first = lane < b.n ? table[(tile * T + (lane << box_shift)) >> p.shift] : 0;
   return b;
 }
 
@@ -131,7 +149,7 @@ __device__ __forceinline__ void load_rows(uint32_t dst0, uint64_t *full, const C
   __syncwarp();
   for (int i = lane; i < b.n; i += 32) {
     const int t = tile * T + (i << box_shift);
-    int page = i == lane ? b.first : __ldg(table + (t >> p.shift));
+    int page = i == lane ? b.first : table[t >> p.shift];
     if ((uint32_t)page >= p.n_pages) {
       atomicOr(err, ERR_INDEX);
       page = -1;

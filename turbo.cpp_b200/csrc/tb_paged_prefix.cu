@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   __syncthreads();
   fence_after();
   pdl_wait();
-  pdl_launch_dependents();  // only now: the next kernel relies on everything before this one having ended
+  if (tid == kBlock - 1) let_next_begin(a.prefix);
   const int stream = warp >> 2, r = tid & 127;
   const int row0 = blockIdx.x * (pair ? 2 * kRows : kRows);  // of all rows of the key/value head
   // ---- queries (all warps but the loading one): D / 8 lanes per row, eight elements each

@@ -437,7 +437,7 @@ typedef struct tb_paged_batch {
   int64_t batch;
   const int32_t *lens;   /* device [batch]: keys of each sequence, a call's own new tokens included */
   const int32_t *table;  /* device [batch, max_pages] page ids */
-  int64_t max_pages, table_stride;
+  int64_t max_pages, table_stride;  /* max_pages * page_size up to 2^31 - 65537 */
 } tb_paged_batch;
 
 /* RoPE of queries and keys and the append of keys and values to a paged cache,

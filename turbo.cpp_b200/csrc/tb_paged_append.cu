@@ -45,7 +45,8 @@ tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_d
   }
   if (c->n_pages > 0 && (!c->k || !c->v)) return fail(TB_EINVAL, "%s: null pool", who);
   if (!aligned16(c->k) || !aligned16(c->v)) return fail(TB_EINVAL, "%s: the pools must be 16-byte aligned", who);
-  if (b->batch < 0 || b->batch > (1 << 20) || b->max_pages < 0 || b->max_pages > 0x7FFFFFFF / c->page_size ||
+  if (b->batch < 0 || b->batch > (1 << 20) || b->max_pages < 0 ||
+      b->max_pages > (0x7FFFFFFF - 65536) / c->page_size ||  // room to round a length up to a tile
       b->table_stride < b->max_pages)
     return fail(TB_EINVAL, "%s: bad batch extents", who);
   if (b->batch > 0 && (!b->lens || (b->max_pages > 0 && !b->table)))

@@ -183,3 +183,18 @@ def test_steps_in_one_stream_without_a_host_wait(act, ct, group, kvh, batch, pre
     for _ in range(5):
         for a, b in zip(chain(False), want):
             assert torch.equal(a, b)
+
+
+def test_append_lowest_length():
+    """A length so far below zero that the positions of a long prompt would come out above it."""
+    tokens, page, pages = (1 << 20) + 5000, 1 << 20, 2047
+    kp, vp = (torch.full((1, page, 1, 16), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    rows = torch.ones((tokens, 1, 16), dtype=torch.float16, device="cuda")
+    q_out = torch.full_like(rows, 5.0)
+    starts, lens, table = cuda_i32([0, tokens]), cuda_i32([-2 ** 31]), cuda_i32(np.zeros((1, pages)))
+    c, b = T.paged_cache(kp, vp), T.paged_batch(lens, table)
+    T.call("tb_rope_paged_append", T.byref(c), T.byref(b), T.F16, T.ptr(rows), 16, T.ptr(rows), 16, T.ptr(rows), 16,
+           tokens, 1, T.ptr(starts), None, None, 0, T.ptr(q_out), 16, T.stream_handle())
+    torch.cuda.synchronize()
+    assert T.take_device_errors() == 2
+    assert (kp == 7.0).all() and (vp == 7.0).all() and (q_out == 5.0).all()

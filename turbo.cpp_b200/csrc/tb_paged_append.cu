@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
       r1[k] = *reinterpret_cast<const uint4 *>(at + half * AS);
     }
     // the token's sequence: the last b with starts[b] <= t
-    int b = (int)t, pos;
+    int b = (int)t, pos, len;
     bool have = true;
     if (a.starts) {
       int lo = 0, n = a.seqs.batch;  // candidates lo .. lo + n - 1
@@ -176,16 +176,16 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, u
       }
       b = lo;
       const int end = __ldg(a.starts + b + 1);
-      const int len = __ldg(a.seqs.lens + b);
+      len = __ldg(a.seqs.lens + b);
       have = t < end && t >= __ldg(a.starts + b);
-      pos = len - (int)(end - t);
+      pos = (int)((unsigned)len - (unsigned)(end - t));  // (wraps round only where len < 0)
     } else {
-      const int len = __ldg(a.seqs.lens + b);
+      len = __ldg(a.seqs.lens + b);
       have = len != 0;
-      pos = len - 1;
+      pos = (int)((unsigned)len - 1u);
     }
     if (!have) continue;  // an empty slot, or a row behind the last sequence
-    bool ok = pos >= 0 && pos < a.seqs.max_len && (!a.cos_t || pos < a.rope_max_seq);
+    bool ok = len >= 0 && pos >= 0 && pos < a.seqs.max_len && (!a.cos_t || pos < a.rope_max_seq);
     int64_t row = -1;
     if (ok) {
       const int32_t id = __ldg(a.seqs.table + (int64_t)b * a.seqs.table_stride + (pos >> a.pools.shift));

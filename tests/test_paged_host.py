@@ -1,5 +1,7 @@
 """Limits and host arithmetic of the paged cache's entry points, no GPU needed."""
+import ctypes
 import os
+import random
 
 import pytest
 
@@ -22,3 +24,35 @@ def test_tables_of_nearly_2_to_the_31_tokens(page):
     # a call of no tokens: checked in full, launched never
     append(c=c, b=batch(batch=0, max_pages=MOST // page, table_stride=MOST // page), tokens=0)
     decode(c=c, b=batch(batch=0, max_pages=MOST // page, table_stride=MOST // page))
+
+
+def selfcheck(name, *args):
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(T.LIB_PATH), "libturbo_b200_selfcheck.so"))
+    fn = getattr(lib, name)
+    fn.argtypes, fn.restype = [ctypes.c_int64] * len(args), ctypes.c_int64
+    return fn(*args)
+
+
+def test_prefix_splits_finish_first():
+    """Against every number of splits: waves of CTAs times a share's tiles and a start, within 2 %."""
+    r = random.Random(5)
+    for _ in range(600):
+        items, tiles = r.choice([1, 2, 8, 12, 100, 147, 148, 149, 300, r.randint(1, 2000)]), r.randint(1, 3000)
+        ctas, most = r.choice([148, 296, 444, r.randint(1, 500)]), r.randint(1, 4000)
+
+        def time(n):
+            return -(-items * n // ctas) * (-(-tiles // n) + 6)
+
+        n = selfcheck("tb_selfcheck_prefix_splits", items, tiles, ctas, most)
+        assert 1 <= n <= min(most, tiles)
+        assert time(n) <= 1.02 * min(time(m) for m in range(1, min(most, tiles) + 1))
+        assert all(time(m) > time(n) for m in range(1, n))
+
+
+def test_prefix_splits_look_at_few():
+    """The choice is made at every call: its cost must not grow with the prefix (rows and most as a call has them)."""
+    for rows in (1, 2, 8, 16, 64, 300, 4096, 1 << 17):
+        most = (2 * rows + 2 * 148 * 128 + (2 * rows if rows < 1 << 17 else 1 << 18)) // rows - 1
+        for items in {max(1, rows // 256), max(1, rows // 8), max(1, rows)}:
+            for tiles in (512, 2048, 16384, 1 << 24):
+                assert selfcheck("tb_selfcheck_prefix_splits_looks", items, tiles, 148, most) <= 16

@@ -302,8 +302,29 @@ struct AttnArgs {
   uint64_t wait_ns;  // limit of the kernels' waits
 };
 
-// Sets the prefix's splits: as few as finish first, `items` row tiles of `tiles` key tiles each on `ctas` CTAs at a
-// time, as far as the workspace holds their results.
+// The fewest splits that finish first: `items` row tiles of `tiles` key tiles each on `ctas` CTAs at a time, `most`
+// splits at most.  Only the most splits of a number of waves can be that, and waves beyond the first sixteen numbers that
+// add a split gain next to nothing (each number tried costs a call two divisions).  Measured against one wave of CTAs
+// wherever that many items are: 300 x 128 heads behind 8192 keys of 64 (152 row tiles) 191 us, with one split 239; 2 x 32
+// heads (8 row tiles) 12.5 and 15.0.
+inline int64_t prefix_splits(int64_t items, int64_t tiles, int64_t ctas, int64_t most, int64_t *looks = nullptr) {
+  constexpr int64_t kStart = 6;  // a CTA's start and end, in tiles
+  if (most > tiles) most = tiles;
+  int64_t best = 1, least = INT64_MAX, waves = (items + ctas - 1) / ctas;
+  for (int look = 0; look < 16; ++look) {
+    const int64_t n = waves * ctas / items < most ? waves * ctas / items : most;
+    const int64_t share = (tiles + n - 1) / n, fewest = (tiles + share - 1) / share;  // the fewest of the same share
+    const int64_t time = (items * fewest + ctas - 1) / ctas * (share + kStart);
+    if (time < least) best = fewest, least = time;
+    if (looks) ++*looks;
+    if (n == most) break;
+    const int64_t next = (items * (n + 1) + ctas - 1) / ctas;
+    waves = next > waves ? next : waves + 1;
+  }
+  return best;
+}
+
+// Sets the prefix's splits, as far as the workspace holds their results.
 void set_prefix_splits(AttnArgs &a, int64_t items, int64_t tiles, int64_t ctas);
 
 // A launch that may begin while the kernel before it ends; the kernel waits

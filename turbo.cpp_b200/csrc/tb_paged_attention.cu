@@ -1082,18 +1082,9 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
 
 }  // namespace
 
-// Measured against one wave of CTAs wherever that many items are: 300 x 128 heads behind 8192 keys of 64 (152 row tiles)
-// 191 us, with one split 239; 2 x 32 heads (8 row tiles) 12.5 and 15.0.
 void set_prefix_splits(AttnArgs &a, int64_t items, int64_t tiles, int64_t ctas) {
-  constexpr int64_t kStart = 6;  // a CTA's start and end, in tiles
   const int64_t rows = (int64_t)a.prefix.rows * a.kv_heads;
-  const int64_t most = std::min(prefix_pairs(rows) / rows - 1, tiles);
-  int64_t best = 1, least = INT64_MAX;
-  for (int64_t n = 1; n <= most; ++n) {
-    const int64_t time = (items * n + ctas - 1) / ctas * ((tiles + n - 1) / n + kStart);
-    if (time < least) best = n, least = time;
-  }
-  a.prefix.splits = (int)best;
+  a.prefix.splits = (int)prefix_splits(items, tiles, ctas, prefix_pairs(rows) / rows - 1);
   a.prefix.parts = a.prefix.splits + 1;
 }
 

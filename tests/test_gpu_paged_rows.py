@@ -198,3 +198,62 @@ def test_append_lowest_length():
     torch.cuda.synchronize()
     assert T.take_device_errors() == 2
     assert (kp == 7.0).all() and (vp == 7.0).all() and (q_out == 5.0).all()
+
+
+def selective(x):
+    """Row r of a key/value head's rows takes the keys t with (t + head) % dim == r % dim, each with the same weight, and
+    key t's value is a one in column (t // dim) % dim: an output counts a share of the keys, a dim-th of a dim-th of
+    them, and one left out or taken twice changes it by one of few.  With dim rows every key is counted, with fewer some of
+    every dim keys in a row."""
+    c = 64.0  # c c scale > 360: the other keys' weights are 0 in 32 bits
+    eye = torch.eye(x.dim, device="cuda")
+    head = torch.arange(x.kvh, device="cuda")
+
+    def put(table_row, n, first):
+        t = first + torch.arange(n, device="cuda")
+        put_rows(x.kp, table_row, x.page, c * eye[(t[:, None] + head) % x.dim])
+        put_rows(x.vp, table_row, x.page, eye[(t // x.dim) % x.dim][:, None].expand(n, x.kvh, x.dim))
+
+    put(x.prefix, x.n_prefix, 0)
+    for b, n in enumerate(x.lens):
+        put(x.table[b], n, x.n_prefix)
+    group = x.heads // x.kvh
+    r = torch.arange(len(x.lens) * group, device="cuda").view(len(x.lens), 1, group)
+    x.rows().copy_(c * eye[r.expand(len(x.lens), x.kvh, group).reshape(len(x.lens), x.heads) % x.dim])
+
+
+def check_counts(x, out):
+    torch.cuda.synchronize()
+    assert T.take_device_errors() == 0
+    for b, k, v, got in rows_of(x, out):
+        if k.shape[0] == 0:
+            assert (got == 0).all()
+            continue
+        # The taken keys' weights are the same number, off by (eps/2)^2 once rounded to parts (bf16 2^-16); the sums by
+        # STEPS = 2^-14, or by one unit of 2^-24 for each of (keys / 8 + 200) additions.
+        want, _ = exact(x.rows()[b], k, v, x.scale)
+        rel = 2 ** -16 + STEPS + (k.shape[0] / 8 + 200) * 2 ** -24
+        check_rows(got, want, want * rel, x.act)
+        # one key more or less would be seen
+        assert 1 / (k.shape[0] // x.dim ** 2 + 1) > 2 * (rel + torch.finfo(x.act).eps)
+
+
+@pytest.mark.parametrize("case", range(len(SHARED)))
+def test_every_key_behind_a_prefix_counts_once(case):
+    *a, lens, prefix = SHARED[case]
+    x = Batch(*a, lens, prefix, seed=case)
+    selective(x)
+    check_counts(x, x.run(shared=True))
+
+
+@pytest.mark.parametrize("act,ct", PAIRS)
+@pytest.mark.parametrize("group,kvh,dim,lens", [
+    (4, 8, 64, [0, 1, 16, 63, 64, 65, 700, 4096, 4097]),
+    (16, 2, 128, [12000, 3, 0, 130]),
+    (33, 1, 64, [9000, 257, 40]),
+    (2, 1, 128, [300] * 700),
+])
+def test_every_key_of_a_batch_counts_once(group, kvh, dim, lens, act, ct):
+    x = Batch(act, ct, group, kvh, dim, 16, "token", lens, seed=group)
+    selective(x)
+    check_counts(x, x.run())

@@ -56,3 +56,22 @@ def test_prefix_splits_look_at_few():
         for items in {max(1, rows // 256), max(1, rows // 8), max(1, rows)}:
             for tiles in (512, 2048, 16384, 1 << 24):
                 assert selfcheck("tb_selfcheck_prefix_splits_looks", items, tiles, 148, most) <= 16
+
+
+def test_rows_of_the_pools_that_the_kernels_get():
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(T.LIB_PATH), "libturbo_b200_selfcheck.so"))
+    row = lib.tb_selfcheck_paged_row_of
+    row.argtypes = [ctypes.POINTER(T.PagedCache)] + [ctypes.c_int64] * 3
+    row.restype = ctypes.c_int64
+    for c in (cache(), cache(dtype=T.F32), cache(token_stride=64, head_stride=1024),
+              cache(n_pages=0x7FFFFFFF, page_stride=1 << 20), cache(n_pages=1, page_stride=-7),
+              cache(page_size=1, token_stride=-7, page_stride=128), cache(kv_heads=1, head_stride=-7, token_stride=64)):
+        size = 4 if c.dtype == T.F32 else 2
+        for page in {0, c.n_pages // 2, c.n_pages - 1}:
+            for t in (0, 1, c.page_size - 1, c.page_size, 12345, MOST - 1):
+                for h in (0, c.kv_heads - 1):
+                    want = (page * c.page_stride if c.n_pages > 1 else 0) + t % c.page_size * c.token_stride + (
+                        h * c.head_stride)
+                    assert row(c, page, t, h) == size * want
+        for bad in (-1, -2 ** 31, c.n_pages, 2 ** 31 - 1):
+            assert row(c, bad, 5, 0) == -1

@@ -28,6 +28,22 @@ struct PagedSeqs {
   int max_len;  // max_pages * page_size
 };
 
+// The pools of a cache whose descriptor has been checked.
+inline PagedPools paged_pools(const tb_paged_cache *c) {
+  const int size = dtype_size(c->dtype);
+  PagedPools p = {};
+  p.k = static_cast<const char *>(c->k);
+  p.v = static_cast<const char *>(c->v);
+  // the stride of a single element is never used, and may be anything
+  p.page_stride = c->n_pages > 1 ? c->page_stride * size : 0;
+  p.token_stride = c->page_size > 1 ? c->token_stride * size : 0;
+  p.head_stride = c->kv_heads > 1 ? c->head_stride * size : 0;
+  p.n_pages = (uint32_t)c->n_pages;
+  p.mask = c->page_size - 1;
+  while ((1 << p.shift) < c->page_size) ++p.shift;
+  return p;
+}
+
 // Byte offset of a key/value head's row at slot t & mask of page `id`, or -1
 // where the page id lies outside the pool: the only way from a page table to
 // an address in this code (TMA checks its coordinates itself).

@@ -51,15 +51,7 @@ tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_d
     return fail(TB_EINVAL, "%s: bad batch extents", who);
   if (b->batch > 0 && (!b->lens || (b->max_pages > 0 && !b->table)))
     return fail(TB_EINVAL, "%s: null lengths or page table", who);
-  pools->k = static_cast<const char *>(c->k);
-  pools->v = static_cast<const char *>(c->v);
-  pools->page_stride = c->n_pages > 1 ? c->page_stride * size : 0;
-  pools->token_stride = c->page_size > 1 ? c->token_stride * size : 0;
-  pools->head_stride = c->kv_heads > 1 ? c->head_stride * size : 0;
-  pools->n_pages = (uint32_t)c->n_pages;
-  pools->mask = c->page_size - 1;
-  pools->shift = 0;
-  while ((1 << pools->shift) < c->page_size) ++pools->shift;
+  *pools = paged_pools(c);
   seqs->lens = b->lens;
   seqs->table = b->table;
   seqs->table_stride = b->table_stride;

@@ -321,8 +321,8 @@ struct AttnArgs {
 // The fewest splits that finish first: `items` row tiles of `tiles` key tiles each on `ctas` CTAs at a time, `most`
 // splits at most.  Only the most splits of a number of waves can be that, and waves beyond the first sixteen numbers that
 // add a split gain next to nothing (each number tried costs a call two divisions).  Measured against one wave of CTAs
-// wherever that many items are: 300 x 128 heads behind 8192 keys of 64 (152 row tiles) 191 us, with one split 239; 2 x 32
-// heads (8 row tiles) 12.5 and 15.0.
+// wherever that many items are (with 16-bit probabilities in one part): 300 x 128 heads behind 8192 keys of 64 (152 row
+// tiles) 191 us, with one split 239; 2 x 32 heads (8 row tiles) 12.5 and 15.0.
 inline int64_t prefix_splits(int64_t items, int64_t tiles, int64_t ctas, int64_t most, int64_t *looks = nullptr) {
   constexpr int64_t kStart = 6;  // a CTA's start and end, in tiles
   if (most > tiles) most = tiles;

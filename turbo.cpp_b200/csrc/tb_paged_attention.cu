@@ -36,9 +36,10 @@
 //
 // Bytes bound it: keys and values are read once, and four to eight heads leave
 // the tensor pipe 86 % idle.  Measured (bf16, 32 heads on 8 of 128): 128
-// sequences of up to 8192 keys 324 us, 6.3 TB/s of the measured 6.55; one of
-// 131071 keys 94 us, 5.7 TB/s; (fp16 pages, fp32 queries, heads of 64) 32 of up
-// to 4096 keys 32.5 us; one of 511 fp32 keys 7.5 us, all of it latency.
+// sequences of up to 8192 keys 316 us, 6.5 TB/s of the measured 6.55; one of
+// 131071 keys 93 us, 5.8 TB/s; (fp16 pages, fp32 queries, heads of 64) 32 of up
+// to 4096 keys 31.5 us; one of 511 fp32 keys 7.5 to 7.9 us, all of it latency;
+// fp32 pages, 128 of up to 4096 keys of 128 370 us, 5.5 TB/s.
 //
 // Work split.  An item is one (sequence, key/value head, group of 8 HW query
 // heads); its unit of work is one tile.  The grid is one wave; CTA c takes the
@@ -47,7 +48,8 @@
 // captured launch follows the lengths.  Four computing warps per CTA and two or
 // three CTAs per SM: a short item's steps (queries, one tile, joining the warps)
 // then overlap with other items' (64 sequences of up to 512 keys behind a prefix
-// 37.3 us, one CTA of eight warps 40.6).  An item cut by a CTA boundary leaves
+// took 37.3 us with the change from one CTA of eight warps, 40.6 before; 34.2
+// with what came later).  An item cut by a CTA boundary leaves
 // partial results in the workspace; the last of its CTAs to finish (a counter
 // per first CTA, reset by that CTA) joins them.  Behind a prefix there are three
 // kernels: the prefix's (here, or tb_paged_prefix.cu for many rows), this one
@@ -71,21 +73,25 @@ constexpr int64_t prefix_pairs(int64_t rows) {
 constexpr int kWarps = 4;                        // computing warps
 constexpr int kThreads = kWarps * 32;            // their threads
 constexpr int kBlock = kThreads + 32;            // and one warp that loads
-// Splits of a prefix up to which the decode kernel may join them: 4 sequences behind 1001 keys (16 splits) 8.0 us so and
-// 9.1 with a kernel of its own, 17 behind 16387 (37 splits) 48.2 and 33.6.
+// Splits of a prefix up to which the decode kernel may join them, and with a kernel of its own.  4 sequences of up to 60
+// own keys, fp32 pages and heads of 64: behind 300 keys (5 splits) 7.5 and 8.2 us, 1001 (16) 8.8 and 10.4, 2000 (37) 11.0
+// and 11.8; bf16 heads of 128: behind 1001 10.0 and 10.8, 2000 (32) 13.7 and 12.8; 17 sequences behind 16387 (37) 48 and
+// 34.  So it pays up to 16 everywhere, and from some 32 on only for little data.
 constexpr int kJoinSplits = 16;
-// ... and tiles of a sequence's own keys: with more of them its items are cut, and the joins in the kernel slow it (17 x
-// up to 777 behind 512: 22.8 us).
+// ... and tiles of a sequence's own keys: with more of them its items are cut, and the joins in the kernel slow it.  Here
+// and there: 4 behind 1001, own keys up to 60 (1 tile) 8.6 and 9.9 us, 200 (4) 11.8 and 11.2, 500 (8) 12.5 and 11.5; 17 x
+// 8 heads behind 512, own keys up to 200 14.6 and 15.1, 500 15.8 and 15.2, 777 (13) 23.5 and 15.4.
+// (Own keys count as the table has room for: the lengths are on the device.)
 constexpr int kJoinTiles = 4;
 // A short prefix, of up to so many tiles per item and units of work in all, is read by the decode kernel before each
 // sequence's own keys: two launches fewer.  Measured so and with the prefix's kernels: 64 behind 64, 256, 512 and 1024
-// keys of 64 (512, 2048, 4096, 8192 units) 16.1 and 21.4, 18.4 and 22.1, 22.1 and 22.6, 30.3 and 26.1 us; 4 behind 1001
-// (16 tiles per item) 12.4 and 8.4.
+// keys of 64 (512, 2048, 4096, 8192 units) 15.8 and 21.4, 17.9 and 21.8, 21.5 and 22.6, 29.3 and 25.9 us; 4 with up to 300
+// own keys behind 1001 (16 tiles per item) 12.3 and 11.4.
 constexpr int kLeadTiles = 8;
 constexpr int64_t kLeadUnits = 4096;
-// Query rows of a key/value head from which the prefix runs on tcgen05.  Here and there: 32 and 36 rows behind 8192 keys
-// of 64 (fp16, fp32 queries) 20.0 and 19.7 us, 60 rows 24.0 and 21.1; behind 32768 keys of 128 (bf16) 45.9 and 40.6,
-// 75.0 and 42.6.
+// Query rows of a key/value head from which the prefix runs on tcgen05.  There and here: 32 rows behind 8192 keys of 64
+// (fp16, fp32 queries) 18.9 and 16.8 us, 36 rows 19.2 and 19.6, 60 rows 19.4 and 20.8; behind 32768 keys of 128 (bf16)
+// 46.5 and 44.9, 46.7 and 69.7, 46.7 and 71.6; behind 4096 18.3 and 19.9, 18.5 and 20.0, 18.9 and 22.7.
 constexpr int kTensorRows = 33;
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -38,10 +38,12 @@
 // read from shared memory at 128 bytes a cycle, 1.5 times the tensor cores' own
 // time for S).  Measured, with the sequences' own keys and the joins (512 rows of
 // each of 8 key/value heads behind 32768 keys): bf16 heads of 128 105 us, of 64 82
-// us; with probabilities in one part, which rounds outputs 1.4 times as far, 97.6
-// and 74.  64 sequences behind 8192 fp16 keys of 64, fp32 queries 34 us.  Two row
+// us; with probabilities in one part, which left outputs 1.4 times as far off, 97.6
+// and 74.  (The prefix's kernel by itself, cold: 84 us for those 32768 keys of 128,
+// 48 for 16384, the tensor pipe 61 % and the special function units 37 % busy.)
+// 64 sequences behind 8192 fp16 keys of 64, fp32 queries 34 us.  Two row
 // tiles as streams or alternate keys: 80 and 127 us; 33.8 and 35.5 even where the
-// second tile has 8 rows.
+// second tile has 8 rows (with probabilities in one part).
 #include <algorithm>
 
 #include "tb_paged.cuh"

@@ -4,6 +4,8 @@ Tolerances as in test_gpu_paged.py, with these for 16-bit activations: a
 probability is two parts of the cache's type, each to nearest, so it is off by
 at most (eps/2)^2 of itself; a tensor core's accumulator is read out after 512
 steps at most, each off by at most one unit of 2^-23."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -257,3 +259,50 @@ def test_every_key_of_a_batch_counts_once(group, kvh, dim, lens, act, ct):
     x = Batch(act, ct, group, kvh, dim, 16, "token", lens, seed=group)
     selective(x)
     check_counts(x, x.run())
+
+
+@pytest.mark.parametrize("act,ct,group,kvh,batch,prefix,room", [
+    ("f16", "f16", 4, 2, 20, 1500, 8),
+    ("f32", "f32", 4, 2, 3, 900, 2),
+    ("bf16", "bf16", 2, 2, 9, 4000, 30),
+    ("f32", "f16", 4, 2, 5, 0, 40),
+])
+def test_a_captured_step_follows_its_inputs(act, ct, group, kvh, batch, prefix, room):
+    """One captured step, replayed while queries and lengths change in place ahead of it, without a host wait."""
+    steps, dim = 20, 128
+    x = Batch(act, ct, group, kvh, dim, 16, "head", [b % 7 + steps + room for b in range(batch)], prefix, seed=batch)
+    qs = [randn(x.q.shape, 50 + s).to(x.act).cuda() for s in range(steps)]
+    start = cuda_i32([b % 7 for b in range(batch)])
+    out = torch.zeros((batch, x.heads * dim + 8), dtype=x.act, device="cuda")
+    s, g = ctypes.c_void_p(), ctypes.c_void_p()
+    T.call("tb_stream_create", ctypes.byref(s))
+    stream = torch.cuda.ExternalStream(s.value)
+    torch.cuda.synchronize()
+    T.call("tb_capture_begin", s)
+    x.run(shared=True, out=out, stream=stream)
+    T.call("tb_capture_end", s, ctypes.byref(g))
+
+    def replay(wait):
+        sync = torch.cuda.synchronize if wait else lambda: None
+        outs = [torch.zeros_like(out) for _ in range(steps)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            x.d_lens.copy_(start)
+            for i in range(steps):
+                x.d_lens += 1
+                x.q.copy_(qs[i])
+                sync()
+                T.call("tb_graph_launch", g, s)
+                sync()
+                outs[i].copy_(out)
+        torch.cuda.synchronize()
+        assert T.take_device_errors() == 0
+        return outs
+
+    want = replay(True)
+    assert not torch.equal(want[0], want[1])
+    for _ in range(5):
+        for a, b in zip(replay(False), want):
+            assert torch.equal(a, b)
+    T.call("tb_graph_destroy", g)
+    T.call("tb_stream_destroy", s)

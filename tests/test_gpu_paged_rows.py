@@ -306,3 +306,30 @@ def test_a_captured_step_follows_its_inputs(act, ct, group, kvh, batch, prefix, 
             assert torch.equal(a, b)
     T.call("tb_graph_destroy", g)
     T.call("tb_stream_destroy", s)
+
+
+@pytest.mark.parametrize("act,ct,group,kvh,dim,lens,prefix", [
+    ("f32", "f16", 4, 2, 64, [3000, 1, 0, 700], 0),
+    ("bf16", "bf16", 4, 8, 128, [300] * 200, 0),
+    ("f32", "f32", 4, 8, 64, [1, 60, 0, 33], 1001),
+    ("bf16", "bf16", 4, 8, 128, [3, 70] * 50, 9000),
+    ("f16", "f16", 4, 2, 64, [5] * 20, 3000),
+    ("f32", "bf16", 4, 2, 128, [5] * 64, 2000),
+])
+def test_waits_that_may_run_out(act, ct, group, kvh, dim, lens, prefix):
+    """The shortest limit there is: some waits end in time and some do not."""
+    x = Batch(act, ct, group, kvh, dim, 16, "token", lens, prefix, seed=6)
+    want = x.run(shared=prefix > 0)
+    torch.cuda.synchronize()
+    T.call("tb_set_wait_limit_ns", 1)
+    try:
+        for _ in range(3):
+            out = x.run(shared=prefix > 0)
+            torch.cuda.synchronize()
+            assert T.take_device_errors() in (0, 1)
+            assert (out[:, x.heads * x.dim:] == 9.0).all()
+            x.ws.zero_()
+    finally:
+        T.call("tb_set_wait_limit_ns", 2000000000)
+    assert torch.equal(x.run(shared=prefix > 0), want)
+    x.check(want)

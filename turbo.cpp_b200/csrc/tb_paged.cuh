@@ -118,7 +118,9 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
 // word is set then), later ones return at once, so that the kernel ends.  So
 // nothing that decides how often a loop runs or which barriers a thread comes to
 // is read from what such a wait orders: a call whose waits ran out multiplies
-// what is there and ends.
+// what is there and ends.  A reader that gave up on a stage does not hand it
+// back: a copy into it may still be under way, and its barrier must not be told
+// to expect another one on top.
 __device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t phase, uint32_t *err, bool &dead,
                                            uint64_t limit_ns) {
   if (!dead && !mbar_wait_bounded(bar, phase, err, limit_ns)) dead = true;

@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
       const int keys = tile < 0 ? a.prefix_len - (tile + a.lead) * C::T : item.len - tile * C::T;
       warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, keys), kw);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.empty[stage]);
+      if (lane == 0 && !dead) mbar_arrive(&ctl.empty[stage]);
       if (++stage == C::STAGES) stage = 0, phase ^= 1;
     }
     if (u < u1) {  // the next item's queries arrive during this one's joins
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kBlock, Cfg<CT, D, HW, A32>::CTAS)
     wait_phase(&ctl.full[stage], phase, err, dead, a.wait_ns);
     warp_tile(s, stages + (uint32_t)stage * C::STAGE, min(C::T, a.prefix_len - t * C::T), kw);
     __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.empty[stage]);
+    if (lane == 0 && !dead) mbar_arrive(&ctl.empty[stage]);
     if (++stage == C::STAGES) stage = 0, phase ^= 1;
   }
   leave(s, merge);

@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kBlock, 1)
               mma_ss(to, qd + ((p * C::CB + i / 4) * kRows * 8 + (i % 4) * 2), kd + ((i / 4) * C::KT * 8 + (i % 4) * 2),
                      C::IDESC_QK, p < C::QT - 1 || i > 0);
           commit_to(&ctl.s_full[w][j % C::NB]);
-          commit_to(&ctl.kempty[s]);
+          if (!dead) commit_to(&ctl.kempty[s]);
         }
         __syncwarp();
       };
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kBlock, 1)
               mma_ts(ts + C::O, p0 + C::pcol(p, i / 2) + 8 * (i % 2), vd + i * 128, C::IDESC_PV,
                      p < C::PT - 1 || i > 0 || j % C::KEEP > 0);
             }
-          commit_to(&ctl.vempty[s]);
+          if (!dead) commit_to(&ctl.vempty[s]);
           commit_to(&ctl.o_full[w][j % C::NB]);
         }
         __syncwarp();

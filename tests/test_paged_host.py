@@ -75,3 +75,12 @@ def test_rows_of_the_pools_that_the_kernels_get():
                     assert row(c, page, t, h) == size * want
         for bad in (-1, -2 ** 31, c.n_pages, 2 ** 31 - 1):
             assert row(c, bad, 5, 0) == -1
+
+
+def test_lists_of_integers_are_aligned():
+    """A list at an odd address would fault the kernels."""
+    for f in (append, decode, shared):
+        refused(f, b=batch(lens=(1 << 20) + 2))
+        refused(f, b=batch(table=(1 << 20) + 1))
+    refused(append, starts=(1 << 20) + 2)
+    refused(shared, prefix=(1 << 20) + 3)

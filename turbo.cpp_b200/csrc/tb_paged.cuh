@@ -53,6 +53,7 @@ __host__ __device__ inline int64_t row_offset(const PagedPools &p, int32_t id, i
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // Checks and converts the two descriptors; `who` names the entry point.
 tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_dtype, const char *who,

@@ -51,6 +51,8 @@ tb_status paged_args(const tb_paged_cache *c, const tb_paged_batch *b, int act_d
     return fail(TB_EINVAL, "%s: bad batch extents", who);
   if (b->batch > 0 && (!b->lens || (b->max_pages > 0 && !b->table)))
     return fail(TB_EINVAL, "%s: null lengths or page table", who);
+  if (!aligned4(b->lens) || !aligned4(b->table))
+    return fail(TB_EINVAL, "%s: lengths and page table must be 4-byte aligned", who);
   *pools = paged_pools(c);
   seqs->lens = b->lens;
   seqs->table = b->table;
@@ -254,6 +256,7 @@ extern "C" tb_status tb_rope_paged_append(const tb_paged_cache *cache, const tb_
     return fail(TB_EINVAL, "tb_rope_paged_append: bad extents");
   if (!starts_dev && tokens != seqs->batch)
     return fail(TB_EINVAL, "tb_rope_paged_append: without starts, tokens must equal batch");
+  if (!aligned4(starts_dev)) return fail(TB_EINVAL, "tb_rope_paged_append: starts must be 4-byte aligned");
   if ((cos_dev == nullptr) != (sin_dev == nullptr))
     return fail(TB_EINVAL, "tb_rope_paged_append: one RoPE table without the other");
   if (cos_dev && (rope_max_seq <= 0 || rope_max_seq > 0x7FFFFFFF))

@@ -1049,6 +1049,7 @@ tb_status attention(const tb_paged_cache *cache, const tb_paged_batch *seqs, con
     return fail(TB_EINVAL, "%s: batch * heads * max_pages * page_size is too large (2^36)", who);
   if (B == 0) return TB_OK;
   if (!q || !out || !ws || (prefix_len > 0 && !prefix_table)) return fail(TB_EINVAL, "%s: null pointer", who);
+  if (!aligned4(prefix_table)) return fail(TB_EINVAL, "%s: the prefix's pages must be 4-byte aligned", who);
   const int as = dtype_size(act_dtype);
   if (ldq < heads * D || ldo < heads * D) return fail(TB_EINVAL, "%s: row strides too small", who);
   if (!aligned16(q) || !aligned16(out) || ldq * as % 16 != 0 || ldo * as % 16 != 0)
